@@ -28,6 +28,9 @@ typedef struct vkc_ctx vkc_ctx;
 typedef void          *vkc_stream;
 
 enum { VKC_F32 = 0, VKC_F16 = 1, VKC_BF16 = 2, VKC_I32 = 3 };
+/* Types of an 8-bit key/value cache (vkc_kv_append_q8, vkc_attn_decode_q8): fp8 e4m3 (4 exponent, 3 mantissa bits, largest
+ * value 448) and signed 8-bit integers. */
+enum { VKC_E4M3 = 4, VKC_I8 = 5 };
 
 enum {
     VKC_OK              = 0,
@@ -137,6 +140,24 @@ VKC_API int vkc_attn_prefill_plan(int sm_count, int64_t B, int64_t Hq, int64_t S
 VKC_API int vkc_attn_prefill_items(int sm_count, int64_t B, int64_t Hq, int64_t Sq, int64_t Skv, int64_t D, int causal, int has_kv_len, int cta,
                                    int32_t *items, int max_items);
 
+/* ---- K7: prefill attention over packed sequences: `nseq` sequences of different lengths stored one behind the other, no
+ * padding between them. Sequence b owns the rows [cu_q[b], cu_q[b+1]) of Q and O and the rows [cu_k[b], cu_k[b+1]) of K and V;
+ * a row attends to the keys of its own sequence only. It has no counterpart in the reference, which runs one batch shape per
+ * graph (the arithmetic is vkc_attn_prefill's: ops/matmul.cpp:14-116, ops/softmax.cpp:9-47).
+ *   Q/O [total_q,Hq,D], K/V [total_k,Hkv,D]; *_strides = element strides {token, head} with D contiguous, or NULL for dense
+ *   (views of one packed projection [tokens, Hq+2*Hkv, D] are fine); query head h uses kv head h / (Hq/Hkv);
+ *   cu_q, cu_k: device int32 [nseq+1], non-decreasing; cu_k NULL = cu_q (then total_k must equal total_q). Values outside
+ *   [0, total] are clamped to it. Rows that belong to no sequence (behind cu_q[nseq]) are left as they were;
+ *   causal masks key j > i + (len_k - len_q), i and j counted within the sequence: a sequence with more keys than queries
+ *   continues a prefix. A row that sees no key stores NaN, as in vkc_attn_prefill. Other sequences' values never reach a row,
+ *   not even infinities or NaN; within a sequence a key that the causal mask hides from a row may, if its V is not finite.
+ *   f32, f16, bf16; D <= 256. The tensor-core kernel runs 16-bit storage with D in {64,128}, strides and bases that are
+ *   multiples of 16 bytes and scale > 0; other shapes run the SIMT kernel. ---- */
+VKC_API int vkc_attn_prefill_packed(vkc_ctx *ctx, const void *Q, const void *K, const void *V, void *O, int64_t nseq, int64_t Hq, int64_t Hkv,
+                                    int64_t D, int64_t total_q, int64_t total_k, const int32_t *cu_q, const int32_t *cu_k,
+                                    const int64_t *q_strides, const int64_t *k_strides, const int64_t *v_strides, const int64_t *o_strides,
+                                    float scale, int causal, int dtype, vkc_stream stream);
+
 /* ---- prefill attention with its output fanned out to several GPUs (the all-gather at the attention-output boundary of a
  * head-sharded encoder, done by the kernel that produces the tiles instead of a collective after it). The reference has no
  * multi-device path (docs/LIMITATIONS.md:15-32); the arithmetic is vkc_attn_prefill's (MatMulCpu / SoftmaxCpu chain,
@@ -235,6 +256,39 @@ VKC_API size_t vkc_attn_decode_noalloc_max_bytes(void);
 VKC_API int    vkc_attn_decode_noalloc(vkc_ctx *ctx, const void *Q, const void *Kc, const void *Vc, void *O, int64_t B, int64_t Hq,
                                        int64_t Hkv, int64_t Lmax, int64_t D, const int32_t *kv_len, float scale, int dtype,
                                        vkc_stream stream);
+
+/* ---- K8: appending keys and values to an 8-bit cache. No counterpart in the reference (its 8-bit tensors are weights).
+ *   The cache: Kc/Vc [B,Hkv,Lmax,D] of cache_dtype (VKC_E4M3 or VKC_I8) and k_scale/v_scale fp32 [B,Hkv,Lmax/block]: one scale
+ *   per `block` consecutive tokens of one head; a stored value stands for code * scale. block is 32, 64 or 128, Lmax a multiple
+ *   of it, D 64, 128 or 256; Kc, Vc 16-byte aligned.
+ *   The new rows: K/V [total,Hkv,D], `dtype` f32, f16 or bf16, element strides {token, head} with D contiguous (NULL = dense).
+ *   cu: device int32 [B+1], non-decreasing, clamped to [0, total]: sequence b brings the rows [cu[b], cu[b+1]); NULL: every
+ *   sequence brings one row (total must equal B). kv_len: device int32 [B], the tokens each sequence holds already (NULL =
+ *   none); its rows go to the positions kv_len[b], kv_len[b]+1, ... . Rows at or behind Lmax are dropped, a sequence with a
+ *   negative kv_len is left alone. The call does not change kv_len.
+ *   Scale of a block: the largest magnitude `a` of its tokens decides. e4m3: the least power of two 2^e >= 2^-126 with
+ *   a <= 448 * 2^e; int8: a / 127 rounded to fp32, at least 2^-126; 0 when every value is 0. A code is the quotient
+ *   value / scale rounded once to the nearest code, ties to even. A block that held tokens before keeps the larger of its old
+ *   scale and the new tokens'; if that is larger than the old one, the older codes are requantised the same way (with e4m3,
+ *   whose scales are powers of two, this only rounds codes that reach the subnormal range). A block that receives an infinity or NaN gets the scale
+ *   NaN and codes 0 for the new tokens, so that attention over it answers NaN; it stays so until it is written from its first
+ *   token on. ---- */
+VKC_API int vkc_kv_append_q8(vkc_ctx *ctx, const void *K, const void *V, void *Kc, void *Vc, float *k_scale, float *v_scale, int64_t B,
+                             int64_t Hkv, int64_t Lmax, int64_t D, int64_t block, int64_t total, const int32_t *cu, const int32_t *kv_len,
+                             const int64_t *k_strides, const int64_t *v_strides, int dtype, int cache_dtype, vkc_stream stream);
+
+/* ---- K9: single-query (decode) attention over the 8-bit cache of vkc_kv_append_q8: vkc_attn_decode with
+ * K = Kc * k_scale, V = Vc * v_scale (block scales), half the cache bytes.
+ *   Q/O [B,Hq,D] f16 or bf16 (dtype), cache as above; kv_len device int32 [B] (NULL = Lmax for all), clamped to [0, Lmax];
+ *   a sequence with no key stores NaN, as in vkc_attn_decode. What lies behind kv_len in the cache is never used, whatever
+ *   its bits. Sums and softmax statistics are fp32; Q keeps its precision.
+ *   workspace: device scratch of at least vkc_attn_decode_q8_workspace_bytes(...) bytes (16-byte aligned) for the partial
+ *   results; NULL lets the context keep (and grow) its own. Two calls that may run at the same time need workspaces of their
+ *   own. ---- */
+VKC_API size_t vkc_attn_decode_q8_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Lmax, int64_t D);
+VKC_API int    vkc_attn_decode_q8(vkc_ctx *ctx, const void *Q, const void *Kc, const void *Vc, const float *k_scale, const float *v_scale, void *O,
+                                  int64_t B, int64_t Hq, int64_t Hkv, int64_t Lmax, int64_t D, int64_t block, const int32_t *kv_len, float scale,
+                                  void *workspace, size_t workspace_bytes, int dtype, int cache_dtype, vkc_stream stream);
 
 /* ---- K4: LayerNorm over the trailing `norm` elements. Reference: LayerNormCpu::run
  * src/backend/cpu/ops/layernorm.cpp:12-75 (oracle), shaders/flat_layernorm.comp:8-50 + LayerNormOp

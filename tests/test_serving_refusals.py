@@ -1,0 +1,97 @@
+"""CPU tests of the serving operators' boundary: what the C entry points refuse without a context, and the argument checks of
+the Python binding, run against a stand-in for the library (nothing is launched)."""
+import pytest
+import torch
+
+import vknn_b200
+
+
+class Recorder:
+    """Stands in for the loaded library: notes the calls and succeeds."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        return lambda *a: self.calls.append((name, a)) or 0
+
+
+@pytest.fixture
+def fake():
+    c = vknn_b200.Context.__new__(vknn_b200.Context)
+    c.lib, c.h, c.device = Recorder(), None, -1  # -1 is what CPU tensors answer for their device
+    c._stream = lambda stream: None
+    return c
+
+
+def z(*s, dt=torch.float16):
+    return torch.zeros(*s, dtype=dt)
+
+
+def cache(b=2, hkv=2, lmax=64, d=64, block=32, dt=torch.float8_e4m3fn):
+    return z(b, hkv, lmax, d, dt=dt), z(b, hkv, lmax, d, dt=dt), z(b, hkv, lmax // block, dt=torch.float32), z(b, hkv, lmax // block, dt=torch.float32)
+
+
+def test_null_context_is_refused():
+    lib = vknn_b200.load_library()
+    assert lib.vkc_attn_prefill_packed(None, None, None, None, None, 1, 1, 1, 64, 1, 1, None, None, None, None, None, None, 1.0, 1, 1, None) == -1
+    assert lib.vkc_kv_append_q8(None, None, None, None, None, None, None, 1, 1, 32, 64, 32, 1, None, None, None, None, 1, 4, None) == -1
+    assert lib.vkc_attn_decode_q8(None, None, None, None, None, None, None, 1, 1, 1, 32, 64, 32, None, 1.0, None, 0, 1, 4, None) == -1
+    assert lib.vkc_attn_decode_q8_workspace_bytes(0, 1, 1, 32, 64) == 0 and lib.vkc_attn_decode_q8_workspace_bytes(2, 8, 2, 4096, 128) > 0
+
+
+def test_packed_arguments_reach_the_library_as_given(fake):
+    qkv, o, cu = z(10, 8, 64), z(10, 4, 64), z(3, dt=torch.int32)
+    fake.attn_prefill_packed(qkv[:, :4], qkv[:, 4:6], qkv[:, 6:], o, 0.5, cu, causal=False)
+    (name, a), = fake.lib.calls
+    assert name == "vkc_attn_prefill_packed" and a[5:11] == (2, 4, 2, 64, 10, 10) and a[11] == cu.data_ptr() and a[12] is None
+    assert [list(s) for s in a[13:17]] == [[512, 64]] * 3 + [[256, 64]] and a[17:20] == (0.5, 0, vknn_b200.F16)
+
+
+def test_cache_arguments_reach_the_library_as_given(fake):
+    c = cache(b=3, lmax=128, block=32, dt=torch.int8)
+    lens = z(3, dt=torch.int32)
+    fake.kv_append_q8(z(3, 2, 64), z(3, 2, 64), *c, lens)
+    fake.attn_decode_q8(z(3, 6, 64), *c, z(3, 6, 64), 0.25, kv_len=lens)
+    (n1, a), (n2, b) = fake.lib.calls
+    assert n1 == "vkc_kv_append_q8" and a[7:13] == (3, 2, 128, 64, 32, 3) and a[13] is None and a[14] == lens.data_ptr() and a[17:19] == (vknn_b200.F16, vknn_b200.I8)
+    assert n2 == "vkc_attn_decode_q8" and b[7:13] == (3, 6, 2, 128, 64, 32) and b[15:19] == (None, 0, vknn_b200.F16, vknn_b200.I8)
+
+
+def test_packed_refusals(fake):
+    q, kv, lens = z(6, 4, 64), z(6, 2, 64), z(2, dt=torch.int32)
+    for args, more in (((q, kv, kv, q, 1.0, lens.long()), {}), ((q, kv, kv[:5], q, 1.0, lens), {}), ((q, kv.float(), kv, q, 1.0, lens), {}),
+                       ((q, kv, kv, q[:5], 1.0, lens), {}), ((q, kv, kv, q, 1.0, lens), {"cu_k": lens[:1]}), ((q, z(6, 2, 32), z(6, 2, 32), q, 1.0, lens), {}),
+                       ((q.transpose(0, 2), kv, kv, q.transpose(0, 2), 1.0, lens), {})):
+        with pytest.raises(ValueError):
+            fake.attn_prefill_packed(*args, **more)
+    assert not fake.lib.calls
+
+
+def test_append_refusals(fake):
+    k, lens = z(2, 2, 64), z(2, dt=torch.int32)
+    kc, vc, ks, vs = cache()
+    for args in ((k, k, kc, vc, ks[..., :1], vs, lens), (k, k, kc, vc[:1], ks, vs, lens), (k, k, kc, vc.view(torch.int8), ks, vs, lens),
+                 (k, k, kc.half(), vc.half(), ks, vs, lens), (k, k, kc, vc, ks.half(), vs.half(), lens), (k, k[:1], kc, vc, ks, vs, lens),
+                 (z(2, 4, 64), z(2, 4, 64), kc, vc, ks, vs, lens), (k, k.float(), kc, vc, ks, vs, lens), (k, k, kc, vc, ks, vs, lens.long()),
+                 (k, k, kc, vc, ks, vs, lens[:1]), (k, k, kc, vc, z(2, 2, 3, dt=torch.float32), z(2, 2, 3, dt=torch.float32), lens),
+                 (k, k, kc.transpose(0, 1), vc.transpose(0, 1), ks, vs, lens)):
+        with pytest.raises(ValueError):
+            fake.kv_append_q8(*args)
+    with pytest.raises(ValueError):
+        fake.kv_append_q8(k, k, kc, vc, ks, vs, lens, cu=lens)  # three offsets are wanted
+    assert not fake.lib.calls
+
+
+def test_decode_refusals(fake):
+    q, lens, c = z(2, 4, 64), z(2, dt=torch.int32), cache()
+    for args in ((z(3, 4, 64), *c, z(3, 4, 64), 1.0), (q, *c, q.bfloat16(), 1.0), (q, *c, z(2, 2, 64), 1.0), (q.transpose(0, 1).contiguous().transpose(0, 1), *c, q, 1.0),
+                 (z(2, 4, 128), *c, z(2, 4, 128), 1.0)):
+        with pytest.raises(ValueError):
+            fake.attn_decode_q8(*args, kv_len=lens)
+    with pytest.raises(ValueError):
+        fake.attn_decode_q8(q, *c, z(2, 4, 64), 1.0, kv_len=lens.float())
+    fake.device = 0  # tensors that lie somewhere else
+    with pytest.raises(ValueError):
+        fake.attn_decode_q8(q, *c, z(2, 4, 64), 1.0, kv_len=lens)
+    assert not fake.lib.calls

@@ -7,6 +7,6 @@ memory, streams and the process group. There is no CPU or eager fallback: import
 every compute call needs the built library and a B200, and fails loudly otherwise.
 """
 from .capi import (  # noqa: F401
-    F32, F16, BF16, EPI_NONE, EPI_BIAS, EPI_GELU_ERF, EPI_RESIDUAL, B_KN, B_NK, IMPL_AUTO, IMPL_SIMT, IMPL_TCGEN05,
+    F32, F16, BF16, E4M3, I8, EPI_NONE, EPI_BIAS, EPI_GELU_ERF, EPI_RESIDUAL, B_KN, B_NK, IMPL_AUTO, IMPL_SIMT, IMPL_TCGEN05,
     VkcError, Context, lib_path, load_library, exported_symbols, declared_symbols,
 )

@@ -9,7 +9,7 @@ import re
 HERE = os.path.dirname(os.path.abspath(__file__))
 HEADER = os.path.join(os.path.dirname(HERE), "include", "vknn_cuda.h")
 
-F32, F16, BF16, I32 = 0, 1, 2, 3
+F32, F16, BF16, I32, E4M3, I8 = 0, 1, 2, 3, 4, 5
 EPI_NONE, EPI_BIAS, EPI_GELU_ERF, EPI_RESIDUAL = 0, 1, 2, 4
 B_KN, B_NK = 0, 1
 IMPL_AUTO, IMPL_SIMT, IMPL_TCGEN05 = 0, 1, 2
@@ -86,6 +86,11 @@ def load_library():
     L.vkc_attn_decode_noalloc_max_bytes.argtypes = []
     L.vkc_attn_decode_noalloc_max_bytes.restype = sz
     L.vkc_attn_decode_noalloc.argtypes = [vp, vp, vp, vp, vp] + [i64] * 5 + [vp, f32, i32, vp]
+    L.vkc_attn_prefill_packed.argtypes = [vp, vp, vp, vp, vp] + [i64] * 6 + [vp, vp, vp, vp, vp, vp, f32, i32, i32, vp]
+    L.vkc_kv_append_q8.argtypes = [vp, vp, vp, vp, vp, vp, vp] + [i64] * 6 + [vp, vp, vp, vp, i32, i32, vp]
+    L.vkc_attn_decode_q8_workspace_bytes.argtypes = [i64] * 5
+    L.vkc_attn_decode_q8_workspace_bytes.restype = sz
+    L.vkc_attn_decode_q8.argtypes = [vp, vp, vp, vp, vp, vp, vp] + [i64] * 6 + [vp, f32, vp, sz, i32, i32, vp]
     L.vkc_layernorm.argtypes = [vp, vp, vp, vp, vp, i64, i64, f32, i32, vp]
     L.vkc_pointwise.argtypes = [vp, vp, vp, vp, i32, i32, vp, vp, i32, vp, vp, i32, vp]
     L.vkc_softmax.argtypes = [vp, vp, vp, i64, i64, i32, vp]
@@ -110,6 +115,16 @@ def load_library():
 def _dtype_code(t):
     import torch
     return {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}[t.dtype]
+
+
+_code_of = {}  # torch dtype -> code, filled by the first call (torch is imported late)
+
+
+def _any_dtype_code(t):
+    if not _code_of:
+        import torch
+        _code_of.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.float8_e4m3fn: E4M3, torch.int8: I8})
+    return _code_of[t.dtype]
 
 
 def _np_dtype_code(a):
@@ -297,6 +312,86 @@ class Context:
                                               st(Q), st(K), st(V), st(O), float(scale), int(bool(causal)),
                                               mask.data_ptr() if mask is not None else None, kv_len.data_ptr() if kv_len is not None else None,
                                               _dtype_code(Q), self._stream(stream)))
+
+    def _int32(self, t, n, what):
+        """The pointer of an int32 tensor of n elements on this device, or None."""
+        if t is None:
+            return None
+        import torch
+        if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() or t.get_device() != self.device:
+            raise ValueError("%s must be a contiguous int32 tensor of %d elements on cuda:%d" % (what, n, self.device))
+        return t.data_ptr()
+
+    def _here(self, *tensors):
+        for t in tensors:
+            if t.get_device() != self.device:
+                raise ValueError("the context belongs to cuda:%d, a tensor lies on %s" % (self.device, t.device))
+
+    def attn_prefill_packed(self, Q, K, V, O, scale, cu_q, cu_k=None, causal=True, stream=None):
+        """Attention over sequences of different lengths packed one behind the other: Q/O [total_q,Hq,D], K/V [total_k,Hkv,D], any
+        strides with D contiguous (views of a packed qkv projection are fine). Sequence b owns the rows cu_q[b]..cu_q[b+1] of
+        Q and O and cu_k[b]..cu_k[b+1] of K and V (int32 device tensors of nseq + 1 offsets; cu_k None = cu_q). Rows of O that
+        belong to no sequence are left as they were; a row that sees no key becomes NaN."""
+        total_q, Hq, D = Q.shape
+        total_k, Hkv, _ = K.shape
+        self._here(Q, K, V, O)
+        if K.shape != V.shape or K.shape[2] != D or O.shape != Q.shape or not (Q.dtype == K.dtype == V.dtype == O.dtype):
+            raise ValueError("attn_prefill_packed: Q %s, K %s, V %s and O %s do not go together" % tuple("%s %s" % (tuple(t.shape), t.dtype) for t in (Q, K, V, O)))
+        strides = []
+        for t in (Q, K, V, O):
+            a, b, c = t.stride()
+            if c != 1 and D > 1:
+                raise ValueError("attn_prefill_packed: the last dimension must be contiguous")
+            strides.append((C.c_int64 * 2)(a, b))
+        nseq = cu_q.shape[0] - 1
+        self._check(self.lib.vkc_attn_prefill_packed(self.h, Q.data_ptr(), K.data_ptr(), V.data_ptr(), O.data_ptr(), nseq, Hq, Hkv, D, total_q, total_k,
+                                                     self._int32(cu_q, nseq + 1, "cu_q"), self._int32(cu_k, nseq + 1, "cu_k"), *strides, float(scale),
+                                                     1 if causal else 0, _any_dtype_code(Q), self._stream(stream)))
+
+    def _q8_cache(self, Kc, Vc, k_scale, v_scale):
+        """Shape of an 8-bit cache, (B, Hkv, Lmax, D, block, type code), after checking that its four tensors go together."""
+        import torch
+        B, Hkv, Lmax, D = Kc.shape
+        nb = k_scale.shape[-1]
+        self._here(Kc, Vc, k_scale, v_scale)
+        if (Vc.shape != Kc.shape or Vc.dtype != Kc.dtype or k_scale.shape != (B, Hkv, nb) or v_scale.shape != (B, Hkv, nb) or nb < 1 or Lmax % nb or
+                k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32 or not (Kc.is_contiguous() and Vc.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous())):
+            raise ValueError("the cache is Kc, Vc [B,Hkv,Lmax,D] and float32 k_scale, v_scale [B,Hkv,Lmax/block], all contiguous: got %s, %s, %s, %s"
+                             % tuple("%s %s" % (tuple(t.shape), t.dtype) for t in (Kc, Vc, k_scale, v_scale)))
+        code = _any_dtype_code(Kc)
+        if code != E4M3 and code != I8:
+            raise ValueError("the cache holds float8_e4m3fn or int8 codes, not %s" % Kc.dtype)
+        return B, Hkv, Lmax, D, Lmax // nb, code
+
+    def kv_append_q8(self, K, V, Kc, Vc, k_scale, v_scale, kv_len=None, cu=None, stream=None):
+        """Appends K/V [total,Hkv,D] to an 8-bit cache: Kc/Vc [B,Hkv,Lmax,D] (float8_e4m3fn or int8) with one float32 scale per
+        block of Lmax // k_scale.shape[2] tokens and head. kv_len int32 [B]: the tokens each sequence holds (None: none; not
+        changed by the call); cu int32 [B+1]: sequence b brings the rows cu[b]..cu[b+1] (None: one row each)."""
+        B, Hkv, Lmax, D, block, code = self._q8_cache(Kc, Vc, k_scale, v_scale)
+        total = K.shape[0]
+        self._here(K, V)
+        if K.shape != (total, Hkv, D) or V.shape != K.shape or V.dtype != K.dtype or K.stride(2) != 1 or V.stride(2) != 1:
+            raise ValueError("kv_append_q8: K and V must be [total,%d,%d] with the last dimension contiguous" % (Hkv, D))
+        self._check(self.lib.vkc_kv_append_q8(self.h, K.data_ptr(), V.data_ptr(), Kc.data_ptr(), Vc.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), B, Hkv,
+                                              Lmax, D, block, total, self._int32(cu, B + 1, "cu"), self._int32(kv_len, B, "kv_len"),
+                                              (C.c_int64 * 2)(K.stride(0), K.stride(1)), (C.c_int64 * 2)(V.stride(0), V.stride(1)), _any_dtype_code(K), code,
+                                              self._stream(stream)))
+
+    def attn_decode_q8_workspace_bytes(self, B, Hq, Hkv, Lmax, D):
+        return int(self.lib.vkc_attn_decode_q8_workspace_bytes(B, Hq, Hkv, Lmax, D))
+
+    def attn_decode_q8(self, Q, Kc, Vc, k_scale, v_scale, O, scale, kv_len=None, workspace=None, stream=None):
+        """attn_decode over the 8-bit cache that kv_append_q8 fills: Q/O [B,Hq,D] contiguous, float16 or bfloat16."""
+        B, Hkv, Lmax, D, block, code = self._q8_cache(Kc, Vc, k_scale, v_scale)
+        Hq = Q.shape[1]
+        self._here(Q, O)
+        if Q.shape != (B, Hq, D) or O.shape != Q.shape or O.dtype != Q.dtype or not (Q.is_contiguous() and O.is_contiguous()):
+            raise ValueError("attn_decode_q8: Q and O must be contiguous [%d,Hq,%d] of one type" % (B, D))
+        self._check(self.lib.vkc_attn_decode_q8(self.h, Q.data_ptr(), Kc.data_ptr(), Vc.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), O.data_ptr(), B,
+                                                Hq, Hkv, Lmax, D, block, self._int32(kv_len, B, "kv_len"), float(scale),
+                                                workspace.data_ptr() if workspace is not None else None,
+                                                workspace.numel() * workspace.element_size() if workspace is not None else 0, _any_dtype_code(Q), code,
+                                                self._stream(stream)))
 
     def attn_prefill_fanout(self, Q, K, V, dests, flags, state, o_strides, scale, causal=False, kv_len=None, stream=None, mcast=None):
         """attn_prefill whose output rows are stored into every buffer of `dests` (raw device pointers mapped on this GPU,

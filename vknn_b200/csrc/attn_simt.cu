@@ -22,6 +22,8 @@ namespace {
         int            causal;
         const float   *mask;
         const int32_t *kv_len;
+        // packed sequences (B of them): a CTA's rows are a piece of one sequence; Sq and Skv hold the totals, strides[0] is 0
+        const int32_t *cu_q, *cu_k;
     };
 
     template <typename T>
@@ -33,25 +35,37 @@ namespace {
         float        *Vs   = Ks + kKeys * (D + 1);        // [kKeys][D]
         float        *Qs   = Vs + kKeys * D;              // [kRows][D]
         const int     warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-        const int64_t b = blockIdx.z, h = blockIdx.y, hk = h / (p.Hq / p.Hkv);
-        const int64_t i0 = (int64_t) blockIdx.x * kRows, i = i0 + warp;
-        const bool    row_ok = i < p.Sq;
-        const T      *qb = Q + b * p.qs[0] + h * p.qs[1];
-        const T      *kb = K + b * p.ks[0] + hk * p.ks[1];
-        const T      *vb = V + b * p.vs[0] + hk * p.vs[1];
+        int64_t       b = blockIdx.z, i0 = (int64_t) blockIdx.x * kRows;
+        const int64_t h = blockIdx.y, hk = h / (p.Hq / p.Hkv);
+        int64_t       Sq = p.Sq, Skv = p.Skv, q0 = 0, k0 = 0; // the sequence's lengths and first rows
+        if (p.cu_q) {
+            int64_t first;
+            b   = vkc_packed_find(p.cu_q, p.B, p.Sq, blockIdx.x, kRows, 1, &first);
+            i0  = (blockIdx.x - first) * kRows;
+            q0  = vkc_packed_clamp(p.cu_q[b], p.Sq);
+            k0  = vkc_packed_clamp(p.cu_k[b], p.Skv);
+            Sq  = vkc_packed_clamp(p.cu_q[b + 1], p.Sq) - q0;
+            Skv = vkc_packed_clamp(p.cu_k[b + 1], p.Skv) - k0;
+            if (i0 < 0 || i0 >= Sq) return; // (the whole CTA)
+        }
+        const int64_t i = i0 + warp;
+        const bool    row_ok = i < Sq;
+        const T      *qb = Q + b * p.qs[0] + h * p.qs[1] + q0 * p.qs[2];
+        const T      *kb = K + b * p.ks[0] + hk * p.ks[1] + k0 * p.ks[2];
+        const T      *vb = V + b * p.vs[0] + hk * p.vs[1] + k0 * p.vs[2];
 
         for (int d = lane; d < D; d += 32) Qs[warp * D + d] = row_ok ? St<T>::ld(qb + i * p.qs[2] + d) : 0.f;
 
-        int64_t len = p.kv_len ? (int64_t) p.kv_len[b] : p.Skv;
-        if (len > p.Skv) len = p.Skv;
+        int64_t len = p.kv_len ? (int64_t) p.kv_len[b] : Skv;
+        if (len > Skv) len = Skv;
         int64_t kend = len; // keys any row of this CTA can see
         if (p.causal) {
             int64_t last = i0 + kRows - 1;
-            if (last > p.Sq - 1) last = p.Sq - 1;
-            int64_t lim = last + (p.Skv - p.Sq) + 1;
+            if (last > Sq - 1) last = Sq - 1;
+            int64_t lim = last + (Skv - Sq) + 1;
             if (lim < kend) kend = lim;
         }
-        const int64_t my_lim = p.causal ? i + (p.Skv - p.Sq) : p.Skv; // keys j <= my_lim are visible
+        const int64_t my_lim = p.causal ? i + (Skv - Sq) : Skv; // keys j <= my_lim are visible
 
         float     m = -INFINITY, l = 0.f;
         float     o[kMaxD / 32];
@@ -101,7 +115,7 @@ namespace {
             }
         }
         if (row_ok) {
-            T          *ob  = O + b * p.os[0] + h * p.os[1] + i * p.os[2];
+            T          *ob  = O + b * p.os[0] + h * p.os[1] + (q0 + i) * p.os[2];
             const float inv = 1.0f / l; // l == 0 (every key masked) yields NaN, as the reference's 0/0 does
 #pragma unroll
             for (int dd = 0; dd < kMaxD / 32; ++dd) {
@@ -119,6 +133,7 @@ namespace {
             if (int rc = vkc_configure_smem(ctx, kern, 100 * 1024)) return rc;
         }
         dim3 grid((unsigned) ((p.Sq + kRows - 1) / kRows), (unsigned) p.Hq, (unsigned) p.B);
+        if (p.cu_q) grid = dim3((unsigned) (p.Sq / kRows + p.B), (unsigned) p.Hq, 1);
         kern<<<grid, kRows * 32, smem, st>>>((const T *) Q, (const T *) K, (const T *) V, (T *) O, p);
         return vkc_post_launch(ctx, "attn_simt");
     }
@@ -150,6 +165,7 @@ extern "C" int vkc_attn_prefill(vkc_ctx *ctx, const void *Q, const void *K, cons
         p.os[i] = o_strides ? o_strides[i] : dq[i];
     }
     p.scale = scale, p.causal = causal ? 1 : 0, p.mask = mask, p.kv_len = kv_len;
+    p.cu_q = p.cu_k = nullptr;
 
     const bool tc_shape = dtype != VKC_F32 && !mask && (D == 64 || D == 128);
     if (tc_shape && ctx->impl != VKC_IMPL_SIMT) {
@@ -187,4 +203,41 @@ extern "C" int vkc_attn_prefill_fanout(vkc_ctx *ctx, const void *Q, const void *
     }
     return vkc_attn_prefill_tcgen05(ctx, Q, K, V, nullptr, B, Hq, Hkv, Sq, Skv, D, qs, ks, vs, os, scale, causal ? 1 : 0, kv_len, dtype, fan,
                                     vkc_pick_stream(ctx, stream));
+}
+
+extern "C" int vkc_attn_prefill_packed(vkc_ctx *ctx, const void *Q, const void *K, const void *V, void *O, int64_t nseq, int64_t Hq, int64_t Hkv,
+                                       int64_t D, int64_t total_q, int64_t total_k, const int32_t *cu_q, const int32_t *cu_k,
+                                       const int64_t *q_strides, const int64_t *k_strides, const int64_t *v_strides, const int64_t *o_strides,
+                                       float scale, int causal, int dtype, vkc_stream stream) {
+    if (!ctx) return VKC_ERR_INVALID;
+    VKC_REQUIRE(ctx, nseq >= 0 && Hq >= 1 && Hkv >= 1 && D >= 1 && total_q >= 0 && total_k >= 0, "attn_prefill_packed: bad extents");
+    VKC_REQUIRE(ctx, Hq % Hkv == 0, "attn_prefill_packed: Hq=%lld is not a multiple of Hkv=%lld", (long long) Hq, (long long) Hkv);
+    VKC_REQUIRE(ctx, dtype == VKC_F32 || dtype == VKC_F16 || dtype == VKC_BF16, "attn_prefill_packed: bad dtype %d", dtype);
+    VKC_REQUIRE(ctx, D <= kMaxD, "attn_prefill_packed: head dim %lld exceeds %d", (long long) D, kMaxD);
+    VKC_REQUIRE(ctx, total_q <= INT32_MAX - 1024 && total_k <= INT32_MAX - 1024, "attn_prefill_packed: more rows than 32-bit offsets reach");
+    if (nseq == 0 || total_q == 0) return VKC_OK;
+    VKC_REQUIRE(ctx, cu_q, "attn_prefill_packed: null sequence offsets");
+    VKC_REQUIRE(ctx, cu_k || total_k == total_q, "attn_prefill_packed: without cu_k the keys are the queries' rows (total_k=%lld, total_q=%lld)",
+                (long long) total_k, (long long) total_q);
+    VKC_REQUIRE(ctx, Q && O && (total_k == 0 || (K && V)), "attn_prefill_packed: null tensor");
+    VKC_REQUIRE(ctx, Hq <= 65535 && nseq <= (1 << 24), "attn_prefill_packed: grid too large");
+    VkcDeviceGuard guard(ctx);
+    cudaStream_t   st = vkc_pick_stream(ctx, stream);
+
+    AttnSimtParams p;
+    p.B = nseq, p.Hq = Hq, p.Hkv = Hkv, p.Sq = total_q, p.Skv = total_k, p.D = D;
+    const int64_t dq[2] = {Hq * D, D}, dk[2] = {Hkv * D, D}; // {token, head}
+    auto          set   = [](int64_t(&to)[3], const int64_t *given, const int64_t *dense) {
+        const int64_t *s = given ? given : dense;
+        to[0] = 0, to[1] = s[1], to[2] = s[0];
+    };
+    set(p.qs, q_strides, dq), set(p.ks, k_strides, dk), set(p.vs, v_strides, dk), set(p.os, o_strides, dq);
+    p.scale = scale, p.causal = causal ? 1 : 0, p.mask = nullptr, p.kv_len = nullptr;
+    p.cu_q = cu_q, p.cu_k = cu_k ? cu_k : cu_q;
+    if (ctx->impl == VKC_IMPL_TCGEN05) return vkc_fail(ctx, VKC_ERR_UNSUPPORTED, "attn_prefill_packed: no tensor-core kernel");
+    switch (dtype) {
+        case VKC_F32: return launch_attn_simt<float>(ctx, Q, K, V, O, p, st);
+        case VKC_F16: return launch_attn_simt<__half>(ctx, Q, K, V, O, p, st);
+        default: return launch_attn_simt<__nv_bfloat16>(ctx, Q, K, V, O, p, st);
+    }
 }

@@ -122,7 +122,39 @@ __device__ __forceinline__ void vkc_grid_dep_wait() { asm volatile("griddepcontr
 __device__ __forceinline__ void vkc_grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 #endif
 
-inline size_t vkc_dtype_size(int dt) { return dt == VKC_F32 || dt == VKC_I32 ? 4 : 2; }
+inline size_t vkc_dtype_size(int dt) { return dt == VKC_F32 || dt == VKC_I32 ? 4 : dt == VKC_E4M3 || dt == VKC_I8 ? 1 : 2; }
+
+// Makes the context's device current for the lifetime of the guard (launches go to the calling thread's current device).
+struct VkcDeviceGuard {
+    int  before = -1;
+    bool moved  = false;
+    explicit VkcDeviceGuard(const vkc_ctx *ctx) { moved = cudaGetDevice(&before) == cudaSuccess && before != ctx->device && cudaSetDevice(ctx->device) == cudaSuccess; }
+    ~VkcDeviceGuard() {
+        if (moved) cudaSetDevice(before);
+    }
+    VkcDeviceGuard(const VkcDeviceGuard &)            = delete;
+    VkcDeviceGuard &operator=(const VkcDeviceGuard &) = delete;
+};
+
+#ifdef __CUDACC__
+// Packed sequences: which sequence the work unit `u` belongs to when the units of sequence b begin at
+// first(b) = cu[b] / step + extra * b (integer division, cu clamped to [0, total]). A sequence of n rows that is cut into
+// pieces of `step` rows counted from its own beginning has at most n / step + 1 of them, and from any other beginning one more:
+// with extra = 1 or 2 that many units always lie between first(b) and first(b + 1), and there are
+// total / step + extra * nseq units in all. No list of the units is needed, only this search. One thread, log2(nseq) loads.
+__device__ __forceinline__ int64_t vkc_packed_clamp(int32_t v, int64_t total) { return v < 0 ? 0 : ((int64_t) v > total ? total : (int64_t) v); }
+__device__ __forceinline__ int vkc_packed_find(const int32_t *cu, int64_t nseq, int64_t total, int64_t u, int step, int extra, int64_t *first) {
+    int64_t lo = 0, hi = nseq; // first(lo) <= u < first(hi)
+    int64_t at = vkc_packed_clamp(cu[0], total) / step;
+    while (hi - lo > 1) {
+        const int64_t mid = (lo + hi) >> 1, f = vkc_packed_clamp(cu[mid], total) / step + extra * mid;
+        if (f <= u) lo = mid, at = f;
+        else hi = mid;
+    }
+    *first = at;
+    return (int) lo;
+}
+#endif
 
 int vkc_ensure_scratch(vkc_ctx *ctx, size_t bytes, cudaStream_t st);
 

@@ -1,0 +1,112 @@
+// The 8-bit cache format shared by the kernels that write and read it: codes and scales, and the checks of its shape.
+#pragma once
+#include "common.cuh"
+#include <cuda_fp8.h>
+
+// Shape rules of the cache, common to every entry point that takes one.
+inline int vkc_q8_check(vkc_ctx *ctx, const char *who, int64_t B, int64_t Hkv, int64_t Lmax, int64_t D, int64_t block, int cache_dtype) {
+    VKC_REQUIRE(ctx, cache_dtype == VKC_E4M3 || cache_dtype == VKC_I8, "%s: the cache type is %d, not VKC_E4M3 or VKC_I8", who, cache_dtype);
+    if (D != 64 && D != 128 && D != 256) return vkc_fail(ctx, VKC_ERR_UNSUPPORTED, "%s: head dim %lld not in {64,128,256}", who, (long long) D);
+    if (block != 32 && block != 64 && block != 128) return vkc_fail(ctx, VKC_ERR_UNSUPPORTED, "%s: block of %lld tokens not in {32,64,128}", who, (long long) block);
+    VKC_REQUIRE(ctx, Lmax % block == 0, "%s: Lmax=%lld is not a multiple of the block of %lld tokens", who, (long long) Lmax, (long long) block);
+    VKC_REQUIRE(ctx, Lmax <= INT32_MAX - 1024 && B <= 65535 && Hkv <= 65535, "%s: extents too large", who);
+    return VKC_OK;
+}
+
+#ifdef __CUDACC__
+namespace q8 {
+
+    __device__ __forceinline__ float nan_value() { return __int_as_float(0x7fc00000); }
+
+    // Scale of a block whose largest magnitude has the fp32 bits `top` (sign cleared).
+    template <bool kE4m3> __device__ __forceinline__ float scale_of(uint32_t top) {
+        if (top >= 0x7f800000u) return nan_value();
+        if (top == 0) return 0.f;
+        if (kE4m3) {
+            // top = 1.m * 2^(E-127); 448 = 1.75 * 2^8: the exponent of the scale is E - 8, one more when 1.m > 1.75, at least 1 (2^-126)
+            int e = (int) (top >> 23) - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+            e     = e < 1 ? 1 : e;
+            return __uint_as_float((uint32_t) e << 23);
+        }
+        return fmaxf(__fdiv_rn(__uint_as_float(top), 127.0f), __uint_as_float(1u << 23));
+    }
+
+    __device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
+        return (uint32_t) (a & 0xff) | (uint32_t) (b & 0xff) << 8 | (uint32_t) (c & 0xff) << 16 | (uint32_t) d << 24;
+    }
+    __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+        return lo | hi << 16;
+    }
+    __device__ __forceinline__ float e4m3_value(uint32_t code) { // low 8 bits
+        return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t) (code & 0xff), __NV_E4M3)));
+    }
+    __device__ __forceinline__ int clamp127(int v) { return v > 127 ? 127 : (v < -127 ? -127 : v); }
+
+    // x / s to the nearest code. A scale that this library wrote is a power of two for e4m3, so that the product with its
+    // reciprocal is exact; any other one (a caller's own cache) takes the quotient rounded to fp32. For int8 the product with
+    // the rounded reciprocal is off by less than 2^-15 of a step, which decides every value that is not that close to the
+    // middle between two codes; those few take the correctly rounded quotient, and where even that lies exactly in the middle,
+    // the sign of the remainder.
+    template <bool kE4m3> struct Quant {
+        float s, inv;
+        bool  none, exact; // none: the scale is 0 or NaN, every code is 0; exact: inv is exactly 1 / s
+        __device__ __forceinline__ explicit Quant(float scale) : s(scale) {
+            const uint32_t bits = __float_as_uint(scale);
+            none                = !(scale > 0.f);
+            exact               = (bits & 0x7fffffu) == 0 && (bits >> 23) >= 1 && (bits >> 23) <= 253;
+            inv                 = kE4m3 && exact ? __uint_as_float(0x7f000000u - bits) : __fdiv_rn(1.0f, scale);
+        }
+        __device__ __forceinline__ int near_middle(float x) const {
+            const float y = __fdiv_rn(x, s);
+            float       r = rintf(y);
+            if (fabsf(y - truncf(y)) == 0.5f) {
+                const float rest = fmaf(-y, s, x); // x - y * s, rounded once: its sign is the true one
+                if (rest > 0.f) r = ceilf(y);
+                else if (rest < 0.f) r = floorf(y);
+            }
+            return clamp127((int) r);
+        }
+        __device__ __forceinline__ int one(float x) const {
+            const float y = x * inv, r = rintf(y);
+            if (fabsf(fabsf(y - r) - 0.5f) < 3.0517578125e-5f) return near_middle(x);
+            return clamp127((int) r);
+        }
+        __device__ __forceinline__ uint32_t four(float a, float b, float c, float d) const {
+            if (none) return 0u;
+            if (kE4m3) {
+                if (exact) return e4m3x4(a * inv, b * inv, c * inv, d * inv);
+                return e4m3x4(__fdiv_rn(a, s), __fdiv_rn(b, s), __fdiv_rn(c, s), __fdiv_rn(d, s));
+            }
+            return pack4(one(a), one(b), one(c), one(d));
+        }
+    };
+
+    // code * s_old / s to the nearest code, s > s_old >= 0. e4m3 with powers of two: the product is exact. int8: as above, the
+    // close cases in double, where the quotient of the 31-bit product by the 24-bit scale keeps its side of the middle.
+    template <bool kE4m3> struct Requant {
+        float  ratio;
+        double s_old, s;
+        bool   exact;
+        __device__ __forceinline__ Requant(float old_scale, float scale) : s_old(old_scale), s(scale) {
+            exact = ((__float_as_uint(old_scale) | __float_as_uint(scale)) & 0x7fffffu) == 0;
+            ratio = __fdiv_rn(old_scale, scale);
+        }
+        __device__ __forceinline__ int int8(int c) const {
+            const float y = (float) c * ratio, r = rintf(y);
+            if (fabsf(fabsf(y - r) - 0.5f) < 3.0517578125e-5f) return clamp127((int) rint((double) c * s_old / s));
+            return clamp127((int) r);
+        }
+        __device__ __forceinline__ float e4m3(uint32_t code) const {
+            const float v = e4m3_value(code);
+            return exact ? v * ratio : (float) ((double) v * s_old / s);
+        }
+        __device__ __forceinline__ uint32_t four(uint32_t c) const {
+            if (kE4m3) return e4m3x4(e4m3(c), e4m3(c >> 8), e4m3(c >> 16), e4m3(c >> 24));
+            return pack4(int8((int8_t) c), int8((int8_t) (c >> 8)), int8((int8_t) (c >> 16)), int8((int8_t) (c >> 24)));
+        }
+    };
+
+} // namespace q8
+#endif
