@@ -4,7 +4,10 @@ it, each against a plain implementation in 64 bits, and a run of the three toget
 Tolerances. Attention: with u the half step of the storage type and A = sum_j p_j |v_j|, the output is off by at most
 u |o| (its own rounding) + w A, where w covers the rounding of a probability to 16 bits on its way into the matrix product
 (u of that type; nothing where probabilities stay in fp32), the 2^x of the kernels (below 7.5e-5) and the fp32 scores
-(D products: below 1e-4 of a nat for the sizes here). Codes and scales of the 8-bit cache have to be equal."""
+(D products: below 1e-4 of a nat for the sizes here). A probability that is rounded to f16 is stored times 2^7 relative to a
+running maximum m that the true one does not fall short of: the spacing of f16 is 2^-24 below 2^-14, so that a probability far
+below the largest is off by at most 2^-25 * 2^-7 = 2^-32 of 2^m, and the output by at most 2^-32 sum_j |v_j| (the sum that
+divides it is at least 2^m). Codes and scales of the 8-bit cache have to be equal."""
 import numpy as np
 import pytest
 import torch
@@ -31,7 +34,7 @@ def randn(g, *shape):
 
 
 def attention64(q, k, v, scale, causal):
-    """q [nq,Hq,D], k/v [nk,Hkv,D] in float64; (o, sum p|v|), NaN rows where nothing is visible."""
+    """q [nq,Hq,D], k/v [nk,Hkv,D] in float64: o and the two sums of its bound, NaN rows where nothing is visible."""
     group = q.shape[1] // k.shape[1]
     k, v = k.repeat_interleave(group, 1), v.repeat_interleave(group, 1)
     x = torch.einsum("qhd,khd->hqk", q, k) * scale
@@ -42,15 +45,20 @@ def attention64(q, k, v, scale, causal):
     seen = torch.isfinite(p).all(-1).T[..., None] if k.shape[0] else torch.zeros(q.shape[0], q.shape[1], 1, dtype=torch.bool, device=q.device)
     o, a = (torch.einsum("hqk,khd->qhd", torch.nan_to_num(p), t) for t in (v, v.abs()))
     nan = torch.full_like(o, torch.nan)
-    return torch.where(seen, o, nan), torch.where(seen, a, nan)
+    if not k.shape[0]:
+        return nan, nan
+    vsum = torch.einsum("hqk,khd->qhd", torch.isfinite(x).to(v.dtype), torch.nan_to_num(v.abs()))
+    return torch.where(seen, o, nan), torch.where(seen, torch.stack([a, 2.0 ** -32 * vsum]), nan)
 
 
-def check(got, ref, a, dt, p_dt, what=""):
+def check(got, ref, sums, dt, p_dt, what=""):
+    """sums: (sum_j p_j |v_j|, 2^-32 sum_j |v_j|)."""
+    a, far = sums if sums.dim() > ref.dim() else (sums, torch.zeros_like(sums))
     got = got.double()
     assert torch.equal(torch.isnan(got), torch.isnan(ref)), (what, "NaN in other places", int(torch.isnan(got).sum()), int(torch.isnan(ref).sum()))
     off = torch.nan_to_num((got - ref).abs())
     w = (half_step(p_dt) if p_dt is not None else 0.0) + SMALL
-    tol = torch.nan_to_num(half_step(dt) * ref.abs() + w * a) + (6e-8 if dt == torch.float16 else 1e-30)
+    tol = torch.nan_to_num(half_step(dt) * ref.abs() + w * a + (far if p_dt == torch.float16 else 0.0)) + (6e-8 if dt == torch.float16 else 1e-30)
     assert bool((off <= tol).all()), (what, "largest excess", float((off / tol.clamp(min=1e-30)).max()))
 
 
@@ -478,8 +486,8 @@ def decode64(q, cache, lens, scale):
         k, v = (t[i, :, :n].double() * s[i].double().repeat_interleave(cache.block, 1)[:, :n, None] for t, s in ((cache.k, cache.ks), (cache.v, cache.vs)))
         r, a = attention64(q[i:i + 1].double(), k.transpose(0, 1), v.transpose(0, 1), scale, False)
         refs.append(r)
-        sums.append(a)
-    return torch.cat(refs), torch.cat(sums)
+        sums.append(a if a.dim() > r.dim() else torch.stack([a, a]))
+    return torch.cat(refs), torch.cat(sums, 1)
 
 
 def check_decode(ctx, q, cache, lens, scale, what=""):

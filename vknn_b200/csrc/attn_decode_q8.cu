@@ -1,6 +1,29 @@
-// K9 — single-query attention over the 8-bit cache (kv_q8.cuh): scores and sums in fp32, each block's scale applied to the
-// score (K) and to the probability (V).
+// K9 — single-query attention over the 8-bit cache (kv_q8.cuh), bound by the bytes of the cache: 2 * Hkv * len * D per
+// sequence and the scales (8 / (block * D) of that). All arithmetic on the sums is fp32; each block's scale multiplies the
+// score (K) and the tile's product (V), never a 16-bit operand.
+//
+// Streaming form. The cache is cut into tiles of 32 keys; the tiles of all (sequence, kv head) units lie on one line and every
+// CTA (one per SM) takes an equal run of it, so that the lengths of the sequences do not matter. The eight warps of a CTA take
+// the run's tiles in turn. Each warp has a ring of shared-memory stages of its own that its lane 0 fills with two bulk-tensor
+// copies per tile (K, V; 128-byte swizzle), so no warp waits for another one before the end of a unit: 192 KB are on the way to
+// every SM. A tile is consumed by warp-level 16x8x16 matrix instructions straight from 8-bit codes:
+//   S[heads, 8 keys] += Q[heads, 16 dims] . K^T      B fragments: 4 code bytes of a key -> two f16 pairs
+//   O^T[16 dims, heads] += V^T[16 dims, 16 keys] . P^T  A fragments: the bytes of two keys interleaved -> f16 pairs
+// The fragment layouts leave two freedoms that make this cheap. The dims of a dot product may be taken in any order as long as Q
+// is laid out the same way, so a thread reads whole 16-byte chunks of a key and uses them 4 bytes at a time; and the rows of
+// O^T may be any dims, so a thread reads 16 consecutive bytes of each of its keys. The accumulator of S is already the B
+// fragment of the second product. e4m3 and int8 codes are exact in f16, and so is Q (bf16 rows are scaled by a power of two
+// first), so the products are those of the values; P is rounded to f16 (11 bits, also for bf16 outputs), times 2^7 so that
+// probabilities down to 2^-21 of the largest keep all of them.
+// Why not tcgen05: at the memory's rate an SM has to convert and multiply 23 codes per clock. The warp-level instructions need
+// about a quarter of the issue slots for that and keep scores and probabilities in registers, where the tensor-memory route
+// would carry every tile through it twice (two round trips per 32 keys); the tensor rate is of no concern at 8 or 16
+// columns.
+// A unit that lies in one CTA's run is finished there; one that is cut leaves a partial (maximum, sum, O) per CTA in the workspace
+// (slot 0: the unit began in an earlier CTA, slot 1: in this one) and a second kernel joins them in the order of the CTAs.
 #include "kv_q8.cuh"
+#include "ptx.cuh"
+#include "tensormap.cuh"
 
 namespace {
 
@@ -68,6 +91,503 @@ namespace {
         }
     }
 
+    // ---------------------------------------------------------------------------------------------------------------------
+    constexpr int kTile    = 32;   // keys per tile
+    constexpr int kMaxCtas = 256;  // rows of the workspace
+    constexpr int kSliceB  = 1024; // sequences per launch (prefix table in shared memory)
+
+    struct StreamParams {
+        DecQ8Params q;
+        int         B, G; // sequences of this launch, query heads per kv head
+        int         block_log2;
+        int         min_tiles;
+        float      *part_o;  // [CTAs][2][G][D]
+        float      *part_ml; // [CTAs][2][G][2]
+        int        *cut;     // [CTAs][4]: sequence, kv head, last CTA of the cut unit that begins in this CTA (-1: none)
+        int        *dev_err;
+    };
+
+    // NT = groups of eight query heads. W warps, S ring stages each.
+    template <int D, int NT> struct Stream {
+        static constexpr int      W = D == 256 ? 4 : 8;
+        static constexpr int      S = (D == 64 ? 6 : 3) * (NT == 1 ? 3 : 2) / 3;
+        static constexpr int      CH = D / 64;   // 16-byte chunks of a key row per thread (QK)
+        static constexpr int      MT = D / 16;   // 16-dim row tiles of O^T
+        static constexpr int      R = MT * 4 * NT; // accumulator registers
+        static constexpr uint32_t TILE  = kTile * D; // bytes of a K or V tile
+        static constexpr uint32_t oRing = 0;
+        static constexpr uint32_t oBuf  = oRing + W * S * 2 * TILE;              // merge: W / 2 register images, rows of 33
+        static constexpr uint32_t oMl   = oBuf + (W / 2) * R * 33 * 4;           // [2][W][NT * 8][2]
+        static constexpr uint32_t oBar  = (oMl + 2 * W * NT * 8 * 2 * 4 + 7) & ~7u;
+        static constexpr uint32_t oSc   = oBar + W * S * 8;                      // [W][S][2]
+        static constexpr uint32_t oCtl  = oSc + W * S * 8;                       // abort flag
+        static constexpr uint32_t oTab  = oCtl + 16;                             // first line position of each sequence
+        static constexpr uint32_t total = oTab + (kSliceB + 1) * 4 + 1024;
+        static_assert(total <= 227 * 1024, "shared memory budget");
+    };
+
+    // D[16x8] += A[16x16] * B[16x8], f16 operands, fp32 accumulator
+    __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    }
+    // four codes -> two f16 pairs, low pair first
+    template <bool kE4m3> __device__ __forceinline__ void codes_to_f16(uint32_t x, uint32_t &lo, uint32_t &hi) {
+        if (kE4m3) {
+            asm("{.reg .b16 a, b; mov.b32 {a, b}, %2; cvt.rn.f16x2.e4m3x2 %0, a; cvt.rn.f16x2.e4m3x2 %1, b;}" : "=r"(lo), "=r"(hi) : "r"(x));
+        } else {
+            // code + 128 as the low byte of 0x6400 is 1024 + 128 + code in f16; subtracting 1152 is exact
+            const uint32_t  u = x ^ 0x80808080u;
+            const uint32_t  l = __byte_perm(u, 0x64646464u, 0x4140), h = __byte_perm(u, 0x64646464u, 0x4342);
+            const __half2   off = __half2half2(__ushort_as_half((unsigned short) 0x6480));
+            const __half2   a = __hsub2(*reinterpret_cast<const __half2 *>(&l), off), b = __hsub2(*reinterpret_cast<const __half2 *>(&h), off);
+            lo = *reinterpret_cast<const uint32_t *>(&a), hi = *reinterpret_cast<const uint32_t *>(&b);
+        }
+    }
+    __device__ __forceinline__ float ex2(float x) {
+        float y;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+        return y;
+    }
+    __device__ __forceinline__ uint32_t f16x2(float a, float b) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+
+    // Where a line position lies: unit (b, hk), the unit's first position and its length in tiles.
+    struct Unit {
+        int b, hk, off, n;
+    };
+    // the first unit (from sequence b on) that holds position `pos`; tab[b] = first position of sequence b
+    __device__ __forceinline__ Unit unit_at(const int *tab, int Hkv, int b, int pos) {
+        while (tab[b + 1] <= pos) ++b;
+        Unit u;
+        u.b = b, u.n = (tab[b + 1] - tab[b]) / Hkv;
+        u.hk  = (pos - tab[b]) / u.n;
+        u.off = tab[b] + u.hk * u.n;
+        return u;
+    }
+
+    template <typename T, int D, int NT, bool kE4m3>
+    __global__ void __launch_bounds__(Stream<D, NT>::W * 32, 1)
+        attn_decode_q8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const StreamParams p) {
+        using L          = Stream<D, NT>;
+        constexpr int W = L::W, S = L::S, CH = L::CH, MT = L::MT;
+        extern __shared__ uint8_t smem_raw[];
+        const uint32_t raw  = ptx::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+        uint8_t       *gb   = smem_raw + (base - raw);
+        volatile int  *ctl  = (volatile int *) (gb + L::oCtl);
+        int           *tab  = (int *) (gb + L::oTab);
+        const int      warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+        const int      Hkv = (int) p.q.Hkv;
+
+        if (threadIdx.x < W * S) ptx::mbar_init(base + L::oBar + 8u * threadIdx.x, 2); // the copies' arrival and the scales'
+        if (threadIdx.x == 0) {
+            ctl[0] = 0;
+            ptx::prefetch_tmap(&tmK);
+            ptx::prefetch_tmap(&tmV);
+        }
+        if (threadIdx.x < W * S) ptx::fence_mbar_init();
+        vkc_grid_dep_wait();
+        vkc_grid_dep_launch();
+        // line positions: sequence b begins at tab[b] and has Hkv * ceil(len / 32) tiles
+        {
+            __shared__ int wsum[W];
+            int            run = 0;
+            for (int b0 = 0; b0 < p.B; b0 += W * 32) {
+                const int b = b0 + threadIdx.x;
+                int       n = b < p.B ? (int) ((q8_len(p.q, b) + kTile - 1) / kTile) * Hkv : 0, incl = n;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int up = __shfl_up_sync(0xffffffffu, incl, o);
+                    if (lane >= o) incl += up;
+                }
+                if (lane == 31) wsum[warp] = incl;
+                __syncthreads();
+                int before = run, all = run;
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    if (w < warp) before += wsum[w];
+                    all += wsum[w];
+                }
+                if (b < p.B) tab[b] = before + incl - n;
+                run = all;
+                __syncthreads();
+            }
+            if (threadIdx.x == 0) tab[p.B] = run;
+        }
+        __syncthreads();
+        const int total = tab[p.B];
+        int       quota = (total + (int) gridDim.x - 1) / (int) gridDim.x;
+        if (quota < p.min_tiles) quota = p.min_tiles;
+        const int64_t c0 = (int64_t) blockIdx.x * quota;
+        const int     P0 = c0 < total ? (int) c0 : total, P1 = c0 + quota < total ? (int) (c0 + quota) : total;
+        // sequences without a key: 0 / 0
+        for (int b = blockIdx.x; b < p.B; b += gridDim.x)
+            if (tab[b] == tab[b + 1])
+                for (int i = threadIdx.x; i < (int) p.q.Hq * D; i += W * 32) St<T>::st((T *) p.q.O + (int64_t) b * p.q.Hq * D + i, q8::nan_value());
+        if (threadIdx.x == 0) p.cut[blockIdx.x * 4 + 2] = -1; // (overwritten below by the same thread where a unit is cut)
+        if (P0 >= P1) return;
+
+        int b_first = 0; // sequence that holds P0
+        {
+            int lo = 0, hi = p.B;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (tab[mid] <= P0) lo = mid;
+                else hi = mid;
+            }
+            b_first = lo;
+        }
+        const int      rows_per_tile = kTile * D / 128, rows_per_unit = (int) (p.q.Lmax * D / 128);
+        const int      nb            = (int) (p.q.Lmax >> p.block_log2);
+        const uint32_t ring = base + L::oRing + (uint32_t) warp * S * 2 * L::TILE, bars = base + L::oBar + 8u * (uint32_t) (warp * S);
+        float         *sc   = (float *) (gb + L::oSc) + warp * S * 2;
+        const uint32_t sc_a = base + L::oSc + (uint32_t) warp * S * 8;
+
+        // ---- producer (lane 0 of the warp): the tile at line position `pp` into stage `ps`
+        int  pp = P0 + warp, ps = 0;
+        Unit pu;
+        pu.b = b_first, pu.off = 0, pu.n = 0, pu.hk = 0;
+        auto fetch = [&]() {
+            if (pp >= P1) return;
+            if (pp >= pu.off + pu.n) pu = unit_at(tab, Hkv, pu.b, pp);
+            const int      tile = pp - pu.off;
+            const int64_t  unit = (int64_t) pu.b * Hkv + pu.hk;
+            const uint32_t bar = bars + 8u * ps, dst = ring + (uint32_t) ps * 2 * L::TILE;
+            const int      row  = (int) (unit * rows_per_unit) + tile * rows_per_tile;
+            ptx::mbar_expect_tx(bar, 2 * L::TILE);
+            ptx::tma_load_2d(dst, &tmK, 0, row, bar);
+            ptx::tma_load_2d(dst + L::TILE, &tmV, 0, row, bar);
+            const int64_t si = unit * nb + ((tile * kTile) >> p.block_log2);
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sc_a + 8u * ps), "l"(p.q.ks + si) : "memory");
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sc_a + 8u * ps + 4u), "l"(p.q.vs + si) : "memory");
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+            pp += W;
+            ps = ps + 1 == S ? 0 : ps + 1;
+        };
+        if (lane == 0)
+            for (int i = 0; i < S; ++i) fetch();
+        __syncwarp();
+
+        int      stage = 0, items = 0;
+        uint32_t phase = 0;
+        bool     ok    = true;
+        int      pos = P0 + warp; // this warp's next tile
+        Unit     u;
+        u.b = b_first;
+        for (int at = P0; at < P1; ++items) { // one item: the part of a unit in this CTA's run
+            u               = unit_at(tab, Hkv, u.b, at);
+            const int end   = u.off + u.n < P1 ? u.off + u.n : P1;
+            const int len   = (int) q8_len(p.q, u.b);
+            const int hq0   = u.hk * p.G;
+            float     o[NT][MT][4], m[NT], l[NT], fac[NT];
+            uint32_t  qa[NT][D / 16][2];
+            // Q of this kv head's group: row g (and g + 8) of the A fragments, dims in the order the key chunks are read in
+#pragma unroll
+            for (int h = 0; h < NT; ++h) {
+                m[h] = -INFINITY, l[h] = 0.f, fac[h] = p.q.scale_log2;
+                const bool have = h * 8 + g < p.G;
+                const T   *qr   = (const T *) p.q.Q + ((int64_t) u.b * p.q.Hq + hq0 + (have ? h * 8 + g : 0)) * D;
+#pragma unroll
+                for (int c = 0; c < CH; ++c) {
+                    const int chunk = D == 256 ? (c >> 1) * 8 + (t & 1) + (t >> 1) * 4 + 2 * (c & 1) : t * CH + c;
+                    uint4     v[2]; // 16 dims
+                    v[0] = have ? __ldg(reinterpret_cast<const uint4 *>(qr + chunk * 16)) : make_uint4(0, 0, 0, 0);
+                    v[1] = have ? __ldg(reinterpret_cast<const uint4 *>(qr + chunk * 16) + 1) : make_uint4(0, 0, 0, 0);
+                    const uint32_t *w = reinterpret_cast<const uint32_t *>(v);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) qa[h][c * 4 + k][0] = w[2 * k], qa[h][c * 4 + k][1] = w[2 * k + 1];
+                }
+                if (!std::is_same<T, __half>::value) {
+                    // bf16: times the power of two that brings the row's largest value to [2^14, 2^15), exact in f16 for everything down
+                    // to 2^-29 of it; the score takes the inverse. A row of zeros, or with infinities, stays as it is.
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const uint32_t x = qa[h][k][e], a = (x << 16) & 0x7fffffffu, c = x & 0x7fff0000u;
+                            top              = a > top ? a : top;
+                            top              = c > top ? c : top;
+                        }
+                    uint32_t other = __shfl_xor_sync(0xffffffffu, top, 1);
+                    top            = other > top ? other : top;
+                    other          = __shfl_xor_sync(0xffffffffu, top, 2);
+                    top            = other > top ? other : top;
+                    const int e  = (int) (top >> 23) - 127;                                   // top in [2^e, 2^(e+1))
+                    const int up = top == 0 || top >= 0x7f800000u ? 0 : (14 - e > 126 ? 126 : 14 - e);
+                    const float mul = __uint_as_float((uint32_t) (127 + up) << 23);
+                    fac[h] *= __uint_as_float((uint32_t) (127 - up) << 23);
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) qa[h][k][i] = f16x2(__uint_as_float(qa[h][k][i] << 16) * mul, __uint_as_float(qa[h][k][i] & 0xffff0000u) * mul);
+                }
+#pragma unroll
+                for (int i = 0; i < MT; ++i) o[h][i][0] = o[h][i][1] = o[h][i][2] = o[h][i][3] = 0.f;
+            }
+
+            for (; pos < end && ok; pos += W) {
+                ok = ptx::mbar_wait(bars + 8u * stage, phase, ctl, p.dev_err);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const uint32_t sK = ring + (uint32_t) stage * 2 * L::TILE, sV = sK + L::TILE;
+                const float    ks = sc[2 * stage], vs = sc[2 * stage + 1];
+                const int      nv = len - (pos - u.off) * kTile; // valid keys of the tile
+                // scores: four groups of eight keys
+                float s[4][4];
+#pragma unroll
+                for (int n = 0; n < 4; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+                for (int c = 0; c < CH; ++c) {
+                    const int chunk = D == 256 ? (c >> 1) * 8 + (t & 1) + (t >> 1) * 4 + 2 * (c & 1) : t * CH + c;
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        const uint32_t byte = (uint32_t) (n * 8 + g) * D + chunk * 16;
+                        const uint4    kv   = ptx::ld_shared_v4(sK + (byte ^ (((byte >> 7) & 7u) << 4)));
+                        const uint32_t w[4] = {kv.x, kv.y, kv.z, kv.w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            uint32_t b0, b1;
+                            codes_to_f16<kE4m3>(w[k], b0, b1);
+                            if (NT == 1) mma16816(s[n], qa[0][c * 4 + k][0], 0u, qa[0][c * 4 + k][1], 0u, b0, b1);
+                            else mma16816(s[n], qa[0][c * 4 + k][0], qa[NT - 1][c * 4 + k][0], qa[0][c * 4 + k][1], qa[NT - 1][c * 4 + k][1], b0, b1);
+                        }
+                    }
+                }
+                uint32_t pb[NT][4]; // P^T as B fragments: keys n * 8 + 2t, + 1 of head g (+ 8)
+#pragma unroll
+                for (int h = 0; h < NT; ++h) {
+                    const float f = fac[h] * ks;
+                    float       x[8], mx = -INFINITY;
+#pragma unroll
+                    for (int n = 0; n < 4; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float v = s[n][h * 2 + e] * f;
+                            x[n * 2 + e]  = n * 8 + 2 * t + e < nv ? v : -INFINITY;
+                            mx            = fmaxf(mx, x[n * 2 + e]);
+                        }
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                    // the maximum is raised only when it grows by more than 2^8: P stays below 2^15 in f16
+                    const bool raise = mx > m[h] + 8.f || (m[h] == -INFINITY && mx > m[h]);
+                    if (__any_sync(0xffffffffu, raise)) {
+                        const float a = raise ? ex2(m[h] - mx) : 1.f; // (0 for the first tile)
+                        if (raise) m[h] = mx;
+                        l[h] *= a;
+                        const float a0 = __shfl_sync(0xffffffffu, a, t * 8), a1 = __shfl_sync(0xffffffffu, a, t * 8 + 4); // heads 2t, 2t + 1
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) o[h][i][0] *= a0, o[h][i][1] *= a1, o[h][i][2] *= a0, o[h][i][3] *= a1;
+                    }
+                    const float up = 7.f - m[h];
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        const float e0 = ex2(x[n * 2] + up), e1 = ex2(x[n * 2 + 1] + up);
+                        l[h] += e0 + e1;
+                        pb[h][n] = f16x2(e0, e1);
+                    }
+                }
+                // O^T += V^T . P^T, 16 keys a step; word w of a thread's bytes holds the dims of two row tiles
+                constexpr int WPT = D / 32; // 4-byte words of a key per thread
+#pragma unroll
+                for (int q4 = 0; q4 < (WPT + 3) / 4; ++q4) {
+                    constexpr int NW = WPT < 4 ? WPT : 4;
+                    uint32_t      x[2][4][NW]; // [step][key][word]
+#pragma unroll
+                    for (int st = 0; st < 2; ++st)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const int      key  = st * 16 + 2 * t + (k & 1) + (k >> 1) * 8;
+                            const uint32_t byte = (uint32_t) key * D + g * (D / 8) + q4 * 16, a = sV + (byte ^ (((byte >> 7) & 7u) << 4));
+                            if (NW == 4) {
+                                const uint4 v = ptx::ld_shared_v4(a);
+                                x[st][k][0] = v.x, x[st][k][1] = v.y, x[st][k][NW - 2] = v.z, x[st][k][NW - 1] = v.w;
+                            } else {
+                                asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(x[st][k][0]), "=r"(x[st][k][1]) : "r"(a));
+                            }
+                            if (key >= nv) // the cache behind the last key may hold any bits
+#pragma unroll
+                                for (int w = 0; w < NW; ++w) x[st][k][w] = 0u;
+                        }
+#pragma unroll
+                    for (int w = 0; w < NW; ++w)
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            float d[NT][4];
+#pragma unroll
+                            for (int h = 0; h < NT; ++h) d[h][0] = d[h][1] = d[h][2] = d[h][3] = 0.f;
+#pragma unroll
+                            for (int st = 0; st < 2; ++st) {
+                                uint32_t a0, a1, a2, a3;
+                                codes_to_f16<kE4m3>(__byte_perm(x[st][0][w], x[st][1][w], half ? 0x7362 : 0x5140), a0, a1);
+                                codes_to_f16<kE4m3>(__byte_perm(x[st][2][w], x[st][3][w], half ? 0x7362 : 0x5140), a2, a3);
+#pragma unroll
+                                for (int h = 0; h < NT; ++h) mma16816(d[h], a0, a1, a2, a3, pb[h][2 * st], pb[h][2 * st + 1]);
+                            }
+                            const int i = (q4 * 4 + w) * 2 + half;
+#pragma unroll
+                            for (int h = 0; h < NT; ++h)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) o[h][i][e] = fmaf(vs, d[h][e], o[h][i][e]);
+                        }
+                }
+                __syncwarp(); // every lane has read the stage
+                if (lane == 0) fetch();
+                if (++stage == S) stage = 0, phase ^= 1;
+            }
+
+            // ---- end of the item: the warps' (m, l, O) become one
+            float(*ml)[NT * 8][2] = reinterpret_cast<float(*)[NT * 8][2]>(gb + L::oMl + (items & 1) * (W * NT * 8 * 8));
+#pragma unroll
+            for (int h = 0; h < NT; ++h) {
+                l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+                l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+                if (t == 0) ml[warp][h * 8 + g][0] = m[h], ml[warp][h * 8 + g][1] = l[h];
+            }
+            __syncthreads();
+            // weight of warp w for head `hd`, against the largest maximum
+            auto top_of = [&](int hd) {
+                float r = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < W; ++w) r = fmaxf(r, ml[w][hd][0]);
+                return r;
+            };
+            auto weight = [&](int w, int hd, float top) { return ml[w][hd][0] == -INFINITY && ml[w][hd][1] == 0.f ? 0.f : ex2(ml[w][hd][0] - top); };
+            float *buf = (float *) (gb + L::oBuf) + (warp % (W / 2)) * L::R * 33 + lane;
+#pragma unroll
+            for (int h = 0; h < NT; ++h) {
+                const int   h0 = h * 8 + 2 * t;
+                const float f0 = weight(warp, h0, top_of(h0)), f1 = weight(warp, h0 + 1, top_of(h0 + 1));
+#pragma unroll
+                for (int i = 0; i < MT; ++i) o[h][i][0] *= f0, o[h][i][1] *= f1, o[h][i][2] *= f0, o[h][i][3] *= f1;
+            }
+            if (warp >= W / 2) {
+#pragma unroll
+                for (int h = 0; h < NT; ++h)
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) buf[((h * MT + i) * 4 + e) * 33] = o[h][i][e];
+            }
+            __syncthreads();
+            if (warp < W / 2) {
+#pragma unroll
+                for (int h = 0; h < NT; ++h)
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) buf[((h * MT + i) * 4 + e) * 33] += o[h][i][e];
+            }
+            __syncthreads();
+            const bool whole = at == u.off && end == u.off + u.n;
+            const int  slot  = at == u.off ? 1 : 0; // (of a cut unit)
+            for (int i = threadIdx.x; i < p.G * D; i += W * 32) {
+                const int    hd = i / D, d = i % D, r = ((hd >> 3) * MT + ((d % (D / 8)) >> 1)) * 4 + (d & 1) * 2 + (hd & 1);
+                const float *x  = (const float *) (gb + L::oBuf) + r * 33 + (d / (D / 8)) * 4 + ((hd & 7) >> 1);
+                float        ov = 0.f;
+#pragma unroll
+                for (int w = 0; w < W / 2; ++w) ov += x[w * L::R * 33];
+                const float top = top_of(hd);
+                float       lv  = 0.f;
+#pragma unroll
+                for (int w = 0; w < W; ++w) lv += ml[w][hd][1] * weight(w, hd, top);
+                if (whole) {
+                    St<T>::st((T *) p.q.O + ((int64_t) u.b * p.q.Hq + hq0 + hd) * D + d, ov / lv);
+                } else {
+                    const int64_t row       = ((int64_t) blockIdx.x * 2 + slot) * p.G + hd;
+                    p.part_o[row * D + d] = ov;
+                    if (d == 0) p.part_ml[row * 2] = top, p.part_ml[row * 2 + 1] = lv;
+                }
+            }
+            if (!whole && slot == 1 && threadIdx.x == 0) {
+                int *cut = p.cut + blockIdx.x * 4;
+                cut[0] = u.b, cut[1] = u.hk, cut[2] = (u.off + u.n - 1) / quota;
+            }
+            at = end;
+        }
+        if (ctl[0])
+            for (int i = 0; i < 50; ++i) __nanosleep(20000); // aborted: let copies in flight land
+    }
+
+    // Joins the partials of the cut unit that begins in CTA blockIdx.x's run: its slot 1, then slot 0 of the CTAs behind it.
+    template <typename T> __global__ void __launch_bounds__(256) attn_decode_q8_join_kernel(const StreamParams p, int D) {
+        vkc_grid_dep_wait();
+        vkc_grid_dep_launch();
+        const int c = blockIdx.x, last = p.cut[c * 4 + 2];
+        if (last < 0) return;
+        const int64_t b = p.cut[c * 4], hk = p.cut[c * 4 + 1];
+        auto          row = [&](int cc, int hd) { return ((int64_t) cc * 2 + (cc == c ? 1 : 0)) * p.G + hd; };
+        for (int i = threadIdx.x; i < p.G * D; i += blockDim.x) {
+            const int hd = i / D, d = i % D;
+            float     top = -INFINITY, lt = 0.f, ot = 0.f;
+            for (int cc = c; cc <= last; ++cc) top = fmaxf(top, p.part_ml[row(cc, hd) * 2]);
+            for (int cc = c; cc <= last; ++cc) {
+                const float a = ex2(p.part_ml[row(cc, hd) * 2] - top);
+                lt += p.part_ml[row(cc, hd) * 2 + 1] * a;
+                ot += p.part_o[row(cc, hd) * D + d] * a;
+            }
+            St<T>::st((T *) p.q.O + (b * p.q.Hq + hk * p.G + hd) * D + d, ot / lt);
+        }
+    }
+
+    // Bytes of the workspace: partials of two cut units per CTA, and what was cut.
+    size_t stream_ws(int64_t G, int64_t D) { return (size_t) kMaxCtas * 2 * (size_t) G * (size_t) (D + 2) * 4 + (size_t) kMaxCtas * 16; }
+
+    template <typename T, int D, int NT, bool kE4m3>
+    int launch_stream(vkc_ctx *ctx, const StreamParams &p, int grid, const CUtensorMap &tk, const CUtensorMap &tv, cudaStream_t st) {
+        auto          kern = attn_decode_q8_kernel<T, D, NT, kE4m3>;
+        constexpr int smem = (int) Stream<D, NT>::total;
+        if (int rc = vkc_configure_smem(ctx, kern, smem)) return rc;
+        vkc_launch(ctx, kern, dim3((unsigned) grid), dim3(Stream<D, NT>::W * 32), smem, st, tk, tv, p);
+        if (int rc = vkc_post_launch(ctx, "attn_decode_q8")) return rc;
+        vkc_launch(ctx, attn_decode_q8_join_kernel<T>, dim3((unsigned) grid), dim3(256), 0, st, p, D);
+        return vkc_post_launch(ctx, "attn_decode_q8_join");
+    }
+    template <typename T, int D> int pick_stream_form(vkc_ctx *ctx, const StreamParams &p, bool e4m3, int grid, const CUtensorMap &tk, const CUtensorMap &tv, cudaStream_t st) {
+        if (p.G <= 8) return e4m3 ? launch_stream<T, D, 1, true>(ctx, p, grid, tk, tv, st) : launch_stream<T, D, 1, false>(ctx, p, grid, tk, tv, st);
+        return e4m3 ? launch_stream<T, D, 2, true>(ctx, p, grid, tk, tv, st) : launch_stream<T, D, 2, false>(ctx, p, grid, tk, tv, st);
+    }
+
+    // The streaming form for the whole call, kSliceB sequences per launch.
+    int run_stream(vkc_ctx *ctx, const DecQ8Params &q, int64_t B, int64_t D, bool e4m3, int dtype, void *ws, cudaStream_t st) {
+        const int64_t G = q.Hq / q.Hkv;
+        for (int64_t b0 = 0; b0 < B; b0 += kSliceB) {
+            StreamParams p;
+            p.q = q, p.B = (int) (B - b0 < kSliceB ? B - b0 : kSliceB), p.G = (int) G, p.block_log2 = q.block == 32 ? 5 : q.block == 64 ? 6 : 7;
+            const int64_t per = q.Hkv * q.Lmax, cache0 = b0 * per * D, scale0 = b0 * (per / q.block);
+            p.q.Q = (const char *) q.Q + b0 * q.Hq * D * 2, p.q.O = (char *) q.O + b0 * q.Hq * D * 2;
+            p.q.Kc += cache0, p.q.Vc += cache0, p.q.ks += scale0, p.q.vs += scale0;
+            if (q.kv_len) p.q.kv_len += b0;
+            p.min_tiles = 8;
+            p.dev_err   = ctx->dev_err;
+            const int64_t tiles = p.B * q.Hkv * ((q.Lmax + kTile - 1) / kTile);
+            int           grid  = ctx->sm_count < kMaxCtas ? ctx->sm_count : kMaxCtas;
+            if ((tiles + p.min_tiles - 1) / p.min_tiles < grid) grid = (int) ((tiles + p.min_tiles - 1) / p.min_tiles);
+            p.part_o  = (float *) ws;
+            p.part_ml = p.part_o + (size_t) kMaxCtas * 2 * G * D;
+            p.cut     = (int *) (p.part_ml + (size_t) kMaxCtas * 2 * G * 2);
+            // both caches as rows of 128 bytes, whatever D is
+            CUtensorMap    tk, tv;
+            const uint64_t dims[2] = {64, (uint64_t) (p.B * per * D / 128)}, stride[1] = {128};
+            const uint32_t box[2]  = {64, (uint32_t) (kTile * D / 128)};
+            if (int rc = vkc_make_tmap(ctx, &tk, VKC_F16, p.q.Kc, 2, dims, stride, box)) return rc;
+            if (int rc = vkc_make_tmap(ctx, &tv, VKC_F16, p.q.Vc, 2, dims, stride, box)) return rc;
+            int rc;
+            if (dtype == VKC_F16)
+                rc = D == 64 ? pick_stream_form<__half, 64>(ctx, p, e4m3, grid, tk, tv, st) : D == 128 ? pick_stream_form<__half, 128>(ctx, p, e4m3, grid, tk, tv, st)
+                                                                                                       : pick_stream_form<__half, 256>(ctx, p, e4m3, grid, tk, tv, st);
+            else
+                rc = D == 64 ? pick_stream_form<__nv_bfloat16, 64>(ctx, p, e4m3, grid, tk, tv, st)
+                             : D == 128 ? pick_stream_form<__nv_bfloat16, 128>(ctx, p, e4m3, grid, tk, tv, st)
+                                        : pick_stream_form<__nv_bfloat16, 256>(ctx, p, e4m3, grid, tk, tv, st);
+            if (rc) return rc;
+        }
+        return VKC_OK;
+    }
+
     template <typename T, int D> void launch_simt(vkc_ctx *ctx, bool e4m3, dim3 grid, cudaStream_t st, const DecQ8Params &p) {
         if (e4m3) vkc_launch(ctx, attn_decode_q8_simt_kernel<T, D, true>, grid, dim3(kSimtWarps * 32), 0, st, p);
         else vkc_launch(ctx, attn_decode_q8_simt_kernel<T, D, false>, grid, dim3(kSimtWarps * 32), 0, st, p);
@@ -77,7 +597,7 @@ namespace {
 
 extern "C" size_t vkc_attn_decode_q8_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Lmax, int64_t D) {
     if (B <= 0 || Hq <= 0 || Hkv <= 0 || Lmax <= 0 || D <= 0) return 0;
-    return 16;
+    return stream_ws(Hq / Hkv, D);
 }
 
 extern "C" int vkc_attn_decode_q8(vkc_ctx *ctx, const void *Q, const void *Kc, const void *Vc, const float *k_scale, const float *v_scale, void *O,
@@ -95,7 +615,6 @@ extern "C" int vkc_attn_decode_q8(vkc_ctx *ctx, const void *Q, const void *Kc, c
     const size_t need = vkc_attn_decode_q8_workspace_bytes(B, Hq, Hkv, Lmax, D);
     VKC_REQUIRE(ctx, !workspace || (workspace_bytes >= need && !((uintptr_t) workspace & 15)),
                 "attn_decode_q8: workspace of %zu bytes is smaller than the %zu required, or not 16-byte aligned", workspace_bytes, need);
-    if (ctx->impl == VKC_IMPL_TCGEN05) return vkc_fail(ctx, VKC_ERR_UNSUPPORTED, "attn_decode_q8: no tensor-core kernel");
     VkcDeviceGuard guard(ctx);
     cudaStream_t   st = vkc_pick_stream(ctx, stream);
     DecQ8Params    p;
@@ -104,6 +623,16 @@ extern "C" int vkc_attn_decode_q8(vkc_ctx *ctx, const void *Q, const void *Kc, c
     p.scale_log2 = scale * 1.4426950408889634f;
     const dim3 grid((unsigned) Hq, (unsigned) B);
     const bool e4m3 = cache_dtype == VKC_E4M3;
+    // The streaming form holds a group of up to 16 query heads and counts line positions and 128-byte rows in 32 bits.
+    const bool fits = Hq / Hkv <= 16 && (B < kSliceB ? B : kSliceB) * Hkv * (Lmax / kTile) < INT32_MAX / 2 && (B < kSliceB ? B : kSliceB) * Hkv * Lmax * (D / 64) < INT32_MAX;
+    if (fits && ctx->impl != VKC_IMPL_SIMT) {
+        if (!workspace) {
+            if (int rc = vkc_ensure_scratch(ctx, need, st)) return rc;
+            workspace = ctx->scratch;
+        }
+        return run_stream(ctx, p, B, D, e4m3, dtype, workspace, st);
+    }
+    if (ctx->impl == VKC_IMPL_TCGEN05) return vkc_fail(ctx, VKC_ERR_UNSUPPORTED, "attn_decode_q8: more than 16 query heads per kv head, or too large a cache, for the tensor-core form");
 #define VKC_Q8_SIMT(T)                                              \
     switch (D) {                                                    \
         case 64: launch_simt<T, 64>(ctx, e4m3, grid, st, p); break;   \
