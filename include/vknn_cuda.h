@@ -279,7 +279,7 @@ VKC_API int vkc_kv_append_q8(vkc_ctx *ctx, const void *K, const void *V, void *K
 
 /* ---- K9: single-query (decode) attention over the 8-bit cache of vkc_kv_append_q8: vkc_attn_decode with
  * K = Kc * k_scale, V = Vc * v_scale (block scales), half the cache bytes.
- *   Q/O [B,Hq,D] f16 or bf16 (dtype), cache as above; kv_len device int32 [B] (NULL = Lmax for all), clamped to [0, Lmax];
+ *   Q/O [B,Hq,D] f16 or bf16 (dtype), 16-byte aligned, cache as above; kv_len device int32 [B] (NULL = Lmax for all), clamped to [0, Lmax];
  *   a sequence with no key stores NaN, as in vkc_attn_decode. What lies behind kv_len in the cache is never used, whatever
  *   its bits. Sums and softmax statistics are fp32; Q keeps its precision.
  *   workspace: device scratch of at least vkc_attn_decode_q8_workspace_bytes(...) bytes (16-byte aligned) for the partial

@@ -3,10 +3,11 @@
 // score (K) and the tile's product (V), never a 16-bit operand.
 //
 // Streaming form. The cache is cut into tiles of 32 keys; the tiles of all (sequence, kv head) units lie on one line and every
-// CTA (one per SM) takes an equal run of it, so that the lengths of the sequences do not matter. The eight warps of a CTA take
-// the run's tiles in turn. Each warp has a ring of shared-memory stages of its own that its lane 0 fills with two bulk-tensor
-// copies per tile (K, V; 128-byte swizzle), so no warp waits for another one before the end of a unit: 192 KB are on the way to
-// every SM. A tile is consumed by warp-level 16x8x16 matrix instructions straight from 8-bit codes:
+// WARP takes an equal run of it, so that the lengths of the sequences do not matter. Each warp has a ring of shared-memory
+// stages of its own that its lane 0 fills with two bulk-tensor copies per tile (K, V; 128-byte swizzle), across the ends of
+// units: no warp ever waits for another one, and 192 KB are on the way to every SM. (Runs per CTA whose tiles the warps took in
+// turn cost three barriers and a merge in shared memory per unit, some 6000 cycles: 64 short sequences took 44 us.) A tile is
+// consumed by warp-level 16x8x16 matrix instructions straight from 8-bit codes:
 //   S[heads, 8 keys] += Q[heads, 16 dims] . K^T      B fragments: 4 code bytes of a key -> two f16 pairs
 //   O^T[16 dims, heads] += V^T[16 dims, 16 keys] . P^T  A fragments: the bytes of two keys interleaved -> f16 pairs
 // The fragment layouts leave two freedoms that make this cheap. The dims of a dot product may be taken in any order as long as Q
@@ -19,8 +20,8 @@
 // about a quarter of the issue slots for that and keep scores and probabilities in registers, where the tensor-memory route
 // would carry every tile through it twice (two round trips per 32 keys); the tensor rate is of no concern at 8 or 16
 // columns.
-// A unit that lies in one CTA's run is finished there; one that is cut leaves a partial (maximum, sum, O) per CTA in the workspace
-// (slot 0: the unit began in an earlier CTA, slot 1: in this one) and a second kernel joins them in the order of the CTAs.
+// A unit that lies in one run is finished there; one that is cut leaves a partial (maximum, sum, O) per run in the workspace
+// (slot 0: the unit began in an earlier run, slot 1: in this one) and a second kernel joins them in the order of the runs.
 #include "kv_q8.cuh"
 #include "ptx.cuh"
 #include "tensormap.cuh"
@@ -92,33 +93,30 @@ namespace {
     }
 
     // ---------------------------------------------------------------------------------------------------------------------
-    constexpr int kTile    = 32;   // keys per tile
-    constexpr int kMaxCtas = 256;  // rows of the workspace
-    constexpr int kSliceB  = 1024; // sequences per launch (prefix table in shared memory)
+    constexpr int kTile     = 32;   // keys per tile
+    constexpr int kMaxCtas  = 160;
+    constexpr int kMinTiles = 2;    // tiles of a run, at least
+    constexpr int kSliceB   = 1024; // sequences per launch (prefix table in shared memory)
 
     struct StreamParams {
         DecQ8Params q;
         int         B, G; // sequences of this launch, query heads per kv head
         int         block_log2;
-        int         min_tiles;
-        float      *part_o;  // [CTAs][2][G][D]
-        float      *part_ml; // [CTAs][2][G][2]
-        int        *cut;     // [CTAs][4]: sequence, kv head, last CTA of the cut unit that begins in this CTA (-1: none)
+        float      *part_o;  // [runs][2][G][D]
+        float      *part_ml; // [runs][2][G][2]
+        int4       *cut;     // [runs]: sequence, kv head, last run of the cut unit that begins in this run (-1: none)
         int        *dev_err;
     };
 
     // NT = groups of eight query heads. W warps, S ring stages each.
     template <int D, int NT> struct Stream {
         static constexpr int      W = D == 256 ? 4 : 8;
-        static constexpr int      S = (D == 64 ? 6 : 3) * (NT == 1 ? 3 : 2) / 3;
+        static constexpr int      S = D == 64 ? 6 : 3;
         static constexpr int      CH = D / 64;   // 16-byte chunks of a key row per thread (QK)
         static constexpr int      MT = D / 16;   // 16-dim row tiles of O^T
-        static constexpr int      R = MT * 4 * NT; // accumulator registers
         static constexpr uint32_t TILE  = kTile * D; // bytes of a K or V tile
         static constexpr uint32_t oRing = 0;
-        static constexpr uint32_t oBuf  = oRing + W * S * 2 * TILE;              // merge: W / 2 register images, rows of 33
-        static constexpr uint32_t oMl   = oBuf + (W / 2) * R * 33 * 4;           // [2][W][NT * 8][2]
-        static constexpr uint32_t oBar  = (oMl + 2 * W * NT * 8 * 2 * 4 + 7) & ~7u;
+        static constexpr uint32_t oBar  = oRing + W * S * 2 * TILE;
         static constexpr uint32_t oSc   = oBar + W * S * 8;                      // [W][S][2]
         static constexpr uint32_t oCtl  = oSc + W * S * 8;                       // abort flag
         static constexpr uint32_t oTab  = oCtl + 16;                             // first line position of each sequence
@@ -155,19 +153,17 @@ namespace {
         return *reinterpret_cast<const uint32_t *>(&h);
     }
 
-    // Where a line position lies: unit (b, hk), the unit's first position and its length in tiles.
-    struct Unit {
-        int b, hk, off, n;
-    };
-    // the first unit (from sequence b on) that holds position `pos`; tab[b] = first position of sequence b
-    __device__ __forceinline__ Unit unit_at(const int *tab, int Hkv, int b, int pos) {
-        while (tab[b + 1] <= pos) ++b;
-        Unit u;
-        u.b = b, u.n = (tab[b + 1] - tab[b]) / Hkv;
-        u.hk  = (pos - tab[b]) / u.n;
-        u.off = tab[b] + u.hk * u.n;
-        return u;
+    template <typename T> __device__ __forceinline__ uint32_t pair16(float a, float b);
+    template <> __device__ __forceinline__ uint32_t pair16<__half>(float a, float b) { return f16x2(a, b); }
+    template <> __device__ __forceinline__ uint32_t pair16<__nv_bfloat16>(float a, float b) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
     }
+
+    // A position on the line: tile `tile` of the `n` tiles of the unit (b, hk).
+    struct At {
+        int b, hk, tile, n;
+    };
 
     template <typename T, int D, int NT, bool kE4m3>
     __global__ void __launch_bounds__(Stream<D, NT>::W * 32, 1)
@@ -182,13 +178,15 @@ namespace {
         const int      warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
         const int      Hkv = (int) p.q.Hkv;
 
-        if (threadIdx.x < W * S) ptx::mbar_init(base + L::oBar + 8u * threadIdx.x, 2); // the copies' arrival and the scales'
+        if (threadIdx.x < W * S) {
+            ptx::mbar_init(base + L::oBar + 8u * threadIdx.x, 2); // the copies' arrival and the scales'
+            ptx::fence_mbar_init();
+        }
         if (threadIdx.x == 0) {
             ctl[0] = 0;
             ptx::prefetch_tmap(&tmK);
             ptx::prefetch_tmap(&tmV);
         }
-        if (threadIdx.x < W * S) ptx::fence_mbar_init();
         vkc_grid_dep_wait();
         vkc_grid_dep_launch();
         // line positions: sequence b begins at tab[b] and has Hkv * ceil(len / 32) tiles
@@ -218,337 +216,343 @@ namespace {
             if (threadIdx.x == 0) tab[p.B] = run;
         }
         __syncthreads();
-        const int total = tab[p.B];
-        int       quota = (total + (int) gridDim.x - 1) / (int) gridDim.x;
-        if (quota < p.min_tiles) quota = p.min_tiles;
-        const int64_t c0 = (int64_t) blockIdx.x * quota;
-        const int     P0 = c0 < total ? (int) c0 : total, P1 = c0 + quota < total ? (int) (c0 + quota) : total;
         // sequences without a key: 0 / 0
         for (int b = blockIdx.x; b < p.B; b += gridDim.x)
             if (tab[b] == tab[b + 1])
                 for (int i = threadIdx.x; i < (int) p.q.Hq * D; i += W * 32) St<T>::st((T *) p.q.O + (int64_t) b * p.q.Hq * D + i, q8::nan_value());
-        if (threadIdx.x == 0) p.cut[blockIdx.x * 4 + 2] = -1; // (overwritten below by the same thread where a unit is cut)
-        if (P0 >= P1) return;
-
-        int b_first = 0; // sequence that holds P0
-        {
-            int lo = 0, hi = p.B;
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (tab[mid] <= P0) lo = mid;
-                else hi = mid;
+        // This warp's run [P0, P1) of the line. Neighbouring runs go to different SMs, so that a short line still uses all of them.
+        const int total = tab[p.B], runs = (int) gridDim.x * W, run = warp * (int) gridDim.x + (int) blockIdx.x;
+        int       quota = (total + runs - 1) / runs;
+        if (quota < kMinTiles) quota = kMinTiles;
+        const int64_t c0 = (int64_t) run * quota;
+        const int     P0 = c0 < total ? (int) c0 : total, P1 = c0 + quota < total ? (int) (c0 + quota) : total;
+        int4          cut = make_int4(0, 0, -1, 0);
+        bool          ok  = true;
+        if (P0 < P1) {
+            At at; // of P0
+            {
+                int lo = 0, hi = p.B;
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1;
+                    if (tab[mid] <= P0) lo = mid;
+                    else hi = mid;
+                }
+                at.b = lo, at.n = (tab[lo + 1] - tab[lo]) / Hkv;
+                at.hk = (P0 - tab[lo]) / at.n, at.tile = P0 - tab[lo] - at.hk * at.n;
             }
-            b_first = lo;
-        }
-        const int      rows_per_tile = kTile * D / 128, rows_per_unit = (int) (p.q.Lmax * D / 128);
-        const int      nb            = (int) (p.q.Lmax >> p.block_log2);
-        const uint32_t ring = base + L::oRing + (uint32_t) warp * S * 2 * L::TILE, bars = base + L::oBar + 8u * (uint32_t) (warp * S);
-        float         *sc   = (float *) (gb + L::oSc) + warp * S * 2;
-        const uint32_t sc_a = base + L::oSc + (uint32_t) warp * S * 8;
-
-        // ---- producer (lane 0 of the warp): the tile at line position `pp` into stage `ps`
-        int  pp = P0 + warp, ps = 0;
-        Unit pu;
-        pu.b = b_first, pu.off = 0, pu.n = 0, pu.hk = 0;
-        auto fetch = [&]() {
-            if (pp >= P1) return;
-            if (pp >= pu.off + pu.n) pu = unit_at(tab, Hkv, pu.b, pp);
-            const int      tile = pp - pu.off;
-            const int64_t  unit = (int64_t) pu.b * Hkv + pu.hk;
-            const uint32_t bar = bars + 8u * ps, dst = ring + (uint32_t) ps * 2 * L::TILE;
-            const int      row  = (int) (unit * rows_per_unit) + tile * rows_per_tile;
-            ptx::mbar_expect_tx(bar, 2 * L::TILE);
-            ptx::tma_load_2d(dst, &tmK, 0, row, bar);
-            ptx::tma_load_2d(dst + L::TILE, &tmV, 0, row, bar);
-            const int64_t si = unit * nb + ((tile * kTile) >> p.block_log2);
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sc_a + 8u * ps), "l"(p.q.ks + si) : "memory");
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sc_a + 8u * ps + 4u), "l"(p.q.vs + si) : "memory");
-            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-            pp += W;
-            ps = ps + 1 == S ? 0 : ps + 1;
-        };
-        if (lane == 0)
-            for (int i = 0; i < S; ++i) fetch();
-        __syncwarp();
-
-        int      stage = 0, items = 0;
-        uint32_t phase = 0;
-        bool     ok    = true;
-        int      pos = P0 + warp; // this warp's next tile
-        Unit     u;
-        u.b = b_first;
-        for (int at = P0; at < P1; ++items) { // one item: the part of a unit in this CTA's run
-            u               = unit_at(tab, Hkv, u.b, at);
-            const int end   = u.off + u.n < P1 ? u.off + u.n : P1;
-            const int len   = (int) q8_len(p.q, u.b);
-            const int hq0   = u.hk * p.G;
-            float     o[NT][MT][4], m[NT], l[NT], fac[NT];
-            uint32_t  qa[NT][D / 16][2];
-            // Q of this kv head's group: row g (and g + 8) of the A fragments, dims in the order the key chunks are read in
-#pragma unroll
-            for (int h = 0; h < NT; ++h) {
-                m[h] = -INFINITY, l[h] = 0.f, fac[h] = p.q.scale_log2;
-                const bool have = h * 8 + g < p.G;
-                const T   *qr   = (const T *) p.q.Q + ((int64_t) u.b * p.q.Hq + hq0 + (have ? h * 8 + g : 0)) * D;
-#pragma unroll
-                for (int c = 0; c < CH; ++c) {
-                    const int chunk = D == 256 ? (c >> 1) * 8 + (t & 1) + (t >> 1) * 4 + 2 * (c & 1) : t * CH + c;
-                    uint4     v[2]; // 16 dims
-                    v[0] = have ? __ldg(reinterpret_cast<const uint4 *>(qr + chunk * 16)) : make_uint4(0, 0, 0, 0);
-                    v[1] = have ? __ldg(reinterpret_cast<const uint4 *>(qr + chunk * 16) + 1) : make_uint4(0, 0, 0, 0);
-                    const uint32_t *w = reinterpret_cast<const uint32_t *>(v);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) qa[h][c * 4 + k][0] = w[2 * k], qa[h][c * 4 + k][1] = w[2 * k + 1];
+            auto next_unit = [&](At &x) { // to the beginning of the next unit (there is one)
+                x.tile = 0;
+                if (++x.hk == Hkv) {
+                    x.hk = 0;
+                    do ++x.b;
+                    while (tab[x.b + 1] == tab[x.b]);
+                    x.n = (tab[x.b + 1] - tab[x.b]) / Hkv;
                 }
-                if (!std::is_same<T, __half>::value) {
-                    // bf16: times the power of two that brings the row's largest value to [2^14, 2^15), exact in f16 for everything down
-                    // to 2^-29 of it; the score takes the inverse. A row of zeros, or with infinities, stays as it is.
-                    uint32_t top = 0;
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const uint32_t x = qa[h][k][e], a = (x << 16) & 0x7fffffffu, c = x & 0x7fff0000u;
-                            top              = a > top ? a : top;
-                            top              = c > top ? c : top;
-                        }
-                    uint32_t other = __shfl_xor_sync(0xffffffffu, top, 1);
-                    top            = other > top ? other : top;
-                    other          = __shfl_xor_sync(0xffffffffu, top, 2);
-                    top            = other > top ? other : top;
-                    const int e  = (int) (top >> 23) - 127;                                   // top in [2^e, 2^(e+1))
-                    const int up = top == 0 || top >= 0x7f800000u ? 0 : (14 - e > 126 ? 126 : 14 - e);
-                    const float mul = __uint_as_float((uint32_t) (127 + up) << 23);
-                    fac[h] *= __uint_as_float((uint32_t) (127 - up) << 23);
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k)
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) qa[h][k][i] = f16x2(__uint_as_float(qa[h][k][i] << 16) * mul, __uint_as_float(qa[h][k][i] & 0xffff0000u) * mul);
-                }
-#pragma unroll
-                for (int i = 0; i < MT; ++i) o[h][i][0] = o[h][i][1] = o[h][i][2] = o[h][i][3] = 0.f;
-            }
+            };
+            const int      rows_per_tile = kTile * D / 128, rows_per_unit = (int) (p.q.Lmax * D / 128);
+            const int      nb = (int) (p.q.Lmax >> p.block_log2);
+            const uint32_t ring = base + L::oRing + (uint32_t) warp * S * 2 * L::TILE, bars = base + L::oBar + 8u * (uint32_t) (warp * S);
+            float         *sc   = (float *) (gb + L::oSc) + warp * S * 2;
+            const uint32_t sc_a = base + L::oSc + (uint32_t) warp * S * 8;
 
-            for (; pos < end && ok; pos += W) {
-                ok = ptx::mbar_wait(bars + 8u * stage, phase, ctl, p.dev_err);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                const uint32_t sK = ring + (uint32_t) stage * 2 * L::TILE, sV = sK + L::TILE;
-                const float    ks = sc[2 * stage], vs = sc[2 * stage + 1];
-                const int      nv = len - (pos - u.off) * kTile; // valid keys of the tile
-                // scores: four groups of eight keys
-                float s[4][4];
-#pragma unroll
-                for (int n = 0; n < 4; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-#pragma unroll
-                for (int c = 0; c < CH; ++c) {
-                    const int chunk = D == 256 ? (c >> 1) * 8 + (t & 1) + (t >> 1) * 4 + 2 * (c & 1) : t * CH + c;
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        const uint32_t byte = (uint32_t) (n * 8 + g) * D + chunk * 16;
-                        const uint4    kv   = ptx::ld_shared_v4(sK + (byte ^ (((byte >> 7) & 7u) << 4)));
-                        const uint32_t w[4] = {kv.x, kv.y, kv.z, kv.w};
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            uint32_t b0, b1;
-                            codes_to_f16<kE4m3>(w[k], b0, b1);
-                            if (NT == 1) mma16816(s[n], qa[0][c * 4 + k][0], 0u, qa[0][c * 4 + k][1], 0u, b0, b1);
-                            else mma16816(s[n], qa[0][c * 4 + k][0], qa[NT - 1][c * 4 + k][0], qa[0][c * 4 + k][1], qa[NT - 1][c * 4 + k][1], b0, b1);
-                        }
-                    }
-                }
-                uint32_t pb[NT][4]; // P^T as B fragments: keys n * 8 + 2t, + 1 of head g (+ 8)
+            // ---- producer (lane 0): the tile at `pa` into stage `ps`
+            At   pa = at;
+            int  ps = 0, left = P1 - P0; // tiles not yet fetched
+            auto fetch = [&]() {
+                if (left == 0) return;
+                const int      unit = pa.b * Hkv + pa.hk, row = unit * rows_per_unit + pa.tile * rows_per_tile;
+                const uint32_t bar = bars + 8u * ps, dst = ring + (uint32_t) ps * 2 * L::TILE;
+                ptx::mbar_expect_tx(bar, 2 * L::TILE);
+                ptx::tma_load_2d(dst, &tmK, 0, row, bar);
+                ptx::tma_load_2d(dst + L::TILE, &tmV, 0, row, bar);
+                const int64_t si = (int64_t) unit * nb + ((pa.tile * kTile) >> p.block_log2);
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sc_a + 8u * ps), "l"(p.q.ks + si) : "memory");
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sc_a + 8u * ps + 4u), "l"(p.q.vs + si) : "memory");
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+                ps = ps + 1 == S ? 0 : ps + 1;
+                if (--left > 0 && ++pa.tile == pa.n) next_unit(pa);
+            };
+            if (lane == 0)
+                for (int i = 0; i < S; ++i) fetch();
+            __syncwarp();
+
+            int      stage = 0;
+            uint32_t phase = 0;
+            for (int todo = P1 - P0; todo > 0 && ok;) { // one item: the part of a unit in this run
+                const int len = (int) q8_len(p.q, at.b), hq0 = at.hk * p.G, first = at.tile;
+                const int end = at.n - first < todo ? at.n : first + todo; // its tiles: [first, end)
+                float     o[NT][MT][4], m[NT], l[NT], fac[NT];
+                uint32_t  qa[NT][D / 16][2];
+                // Q of this kv head's group: row g (and g + 8) of the A fragments, dims in the order the key chunks are read in
 #pragma unroll
                 for (int h = 0; h < NT; ++h) {
-                    const float f = fac[h] * ks;
-                    float       x[8], mx = -INFINITY;
+                    m[h] = -INFINITY, l[h] = 0.f, fac[h] = p.q.scale_log2;
+                    const bool have = h * 8 + g < p.G;
+                    const T   *qr   = (const T *) p.q.Q + ((int64_t) at.b * p.q.Hq + hq0 + (have ? h * 8 + g : 0)) * D;
 #pragma unroll
-                    for (int n = 0; n < 4; ++n)
+                    for (int c = 0; c < CH; ++c) {
+                        const int chunk = D == 256 ? (c >> 1) * 8 + (t & 1) + (t >> 1) * 4 + 2 * (c & 1) : t * CH + c;
+                        uint4     v[2]; // 16 dims
+                        v[0] = have ? __ldg(reinterpret_cast<const uint4 *>(qr + chunk * 16)) : make_uint4(0, 0, 0, 0);
+                        v[1] = have ? __ldg(reinterpret_cast<const uint4 *>(qr + chunk * 16) + 1) : make_uint4(0, 0, 0, 0);
+                        const uint32_t *w = reinterpret_cast<const uint32_t *>(v);
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const float v = s[n][h * 2 + e] * f;
-                            x[n * 2 + e]  = n * 8 + 2 * t + e < nv ? v : -INFINITY;
-                            mx            = fmaxf(mx, x[n * 2 + e]);
-                        }
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                    // the maximum is raised only when it grows by more than 2^8: P stays below 2^15 in f16
-                    const bool raise = mx > m[h] + 8.f || (m[h] == -INFINITY && mx > m[h]);
-                    if (__any_sync(0xffffffffu, raise)) {
-                        const float a = raise ? ex2(m[h] - mx) : 1.f; // (0 for the first tile)
-                        if (raise) m[h] = mx;
-                        l[h] *= a;
-                        const float a0 = __shfl_sync(0xffffffffu, a, t * 8), a1 = __shfl_sync(0xffffffffu, a, t * 8 + 4); // heads 2t, 2t + 1
-#pragma unroll
-                        for (int i = 0; i < MT; ++i) o[h][i][0] *= a0, o[h][i][1] *= a1, o[h][i][2] *= a0, o[h][i][3] *= a1;
+                        for (int k = 0; k < 4; ++k) qa[h][c * 4 + k][0] = w[2 * k], qa[h][c * 4 + k][1] = w[2 * k + 1];
                     }
-                    const float up = 7.f - m[h];
+                    if (!std::is_same<T, __half>::value) {
+                        // bf16: times the power of two that brings the row's largest value to [2^14, 2^15), exact in f16 for everything down
+                        // to 2^-29 of it; the score takes the inverse. A row of zeros, or with infinities, stays as it is.
+                        uint32_t top = 0;
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        const float e0 = ex2(x[n * 2] + up), e1 = ex2(x[n * 2 + 1] + up);
-                        l[h] += e0 + e1;
-                        pb[h][n] = f16x2(e0, e1);
+                        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const uint32_t x = qa[h][k][e], a = (x << 16) & 0x7fffffffu, c = x & 0x7fff0000u;
+                                top              = a > top ? a : top;
+                                top              = c > top ? c : top;
+                            }
+                        uint32_t other = __shfl_xor_sync(0xffffffffu, top, 1);
+                        top            = other > top ? other : top;
+                        other          = __shfl_xor_sync(0xffffffffu, top, 2);
+                        top            = other > top ? other : top;
+                        const int e  = (int) (top >> 23) - 127;                                   // top in [2^e, 2^(e+1))
+                        const int up = top == 0 || top >= 0x7f800000u ? 0 : (14 - e > 126 ? 126 : 14 - e);
+                        const float mul = __uint_as_float((uint32_t) (127 + up) << 23);
+                        fac[h] *= __uint_as_float((uint32_t) (127 - up) << 23);
+#pragma unroll
+                        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) qa[h][k][i] = f16x2(__uint_as_float(qa[h][k][i] << 16) * mul, __uint_as_float(qa[h][k][i] & 0xffff0000u) * mul);
+                    }
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) o[h][i][0] = o[h][i][1] = o[h][i][2] = o[h][i][3] = 0.f;
+                }
+                for (int tile = first; tile < end; ++tile) {
+                    ok = ptx::mbar_wait(bars + 8u * stage, phase, ctl, p.dev_err);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    const uint32_t sK = ring + (uint32_t) stage * 2 * L::TILE, sV = sK + L::TILE;
+                    const float    ks = sc[2 * stage], vs = sc[2 * stage + 1];
+                    const int      nv = len - tile * kTile; // valid keys of the tile
+                    // scores: four groups of eight keys
+                    float s[4][4];
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+                    for (int c = 0; c < CH; ++c) {
+                        const int chunk = D == 256 ? (c >> 1) * 8 + (t & 1) + (t >> 1) * 4 + 2 * (c & 1) : t * CH + c;
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) {
+                            const uint32_t byte = (uint32_t) (n * 8 + g) * D + chunk * 16;
+                            const uint4    kv   = ptx::ld_shared_v4(sK + (byte ^ (((byte >> 7) & 7u) << 4)));
+                            const uint32_t w[4] = {kv.x, kv.y, kv.z, kv.w};
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                uint32_t b0, b1;
+                                codes_to_f16<kE4m3>(w[k], b0, b1);
+                                if (NT == 1) mma16816(s[n], qa[0][c * 4 + k][0], 0u, qa[0][c * 4 + k][1], 0u, b0, b1);
+                                else mma16816(s[n], qa[0][c * 4 + k][0], qa[NT - 1][c * 4 + k][0], qa[0][c * 4 + k][1], qa[NT - 1][c * 4 + k][1], b0, b1);
+                            }
+                        }
+                    }
+                    uint32_t pb[NT][4]; // P^T as B fragments: keys n * 8 + 2t, + 1 of head g (+ 8)
+#pragma unroll
+                    for (int h = 0; h < NT; ++h) {
+                        const float f = fac[h] * ks;
+                        float       x[8], mx = -INFINITY;
+#pragma unroll
+                        for (int n = 0; n < 4; ++n)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const float v = s[n][h * 2 + e] * f;
+                                x[n * 2 + e]  = n * 8 + 2 * t + e < nv ? v : -INFINITY;
+                                mx            = fmaxf(mx, x[n * 2 + e]);
+                            }
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                        // the maximum is raised only when it grows by more than 2^8: P stays below 2^15 in f16
+                        const bool raise = mx > m[h] + 8.f || (m[h] == -INFINITY && mx > m[h]);
+                        if (__any_sync(0xffffffffu, raise)) {
+                            const float a = raise ? ex2(m[h] - mx) : 1.f; // (0 for the first tile)
+                            if (raise) m[h] = mx;
+                            l[h] *= a;
+                            const float a0 = __shfl_sync(0xffffffffu, a, t * 8), a1 = __shfl_sync(0xffffffffu, a, t * 8 + 4); // heads 2t, 2t + 1
+#pragma unroll
+                            for (int i = 0; i < MT; ++i) o[h][i][0] *= a0, o[h][i][1] *= a1, o[h][i][2] *= a0, o[h][i][3] *= a1;
+                        }
+                        const float up = 7.f - m[h];
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) {
+                            const float e0 = ex2(x[n * 2] + up), e1 = ex2(x[n * 2 + 1] + up);
+                            l[h] += e0 + e1;
+                            pb[h][n] = f16x2(e0, e1);
+                        }
+                    }
+                    // O^T += V^T . P^T, 16 keys a step; word w of a thread's bytes holds the dims of two row tiles
+                    constexpr int WPT = D / 32; // 4-byte words of a key per thread
+#pragma unroll
+                    for (int q4 = 0; q4 < (WPT + 3) / 4; ++q4) {
+                        constexpr int NW = WPT < 4 ? WPT : 4;
+                        uint32_t      x[2][4][NW]; // [step][key][word]
+#pragma unroll
+                        for (int st = 0; st < 2; ++st)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const int      key  = st * 16 + 2 * t + (k & 1) + (k >> 1) * 8;
+                                const uint32_t byte = (uint32_t) key * D + g * (D / 8) + q4 * 16, a = sV + (byte ^ (((byte >> 7) & 7u) << 4));
+                                if (NW == 4) {
+                                    const uint4 v = ptx::ld_shared_v4(a);
+                                    x[st][k][0] = v.x, x[st][k][1] = v.y, x[st][k][NW - 2] = v.z, x[st][k][NW - 1] = v.w;
+                                } else {
+                                    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(x[st][k][0]), "=r"(x[st][k][1]) : "r"(a));
+                                }
+                                if (key >= nv) // the cache behind the last key may hold any bits
+#pragma unroll
+                                    for (int w = 0; w < NW; ++w) x[st][k][w] = 0u;
+                            }
+#pragma unroll
+                        for (int w = 0; w < NW; ++w)
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) {
+                                float d[NT][4];
+#pragma unroll
+                                for (int h = 0; h < NT; ++h) d[h][0] = d[h][1] = d[h][2] = d[h][3] = 0.f;
+#pragma unroll
+                                for (int st = 0; st < 2; ++st) {
+                                    uint32_t a0, a1, a2, a3;
+                                    codes_to_f16<kE4m3>(__byte_perm(x[st][0][w], x[st][1][w], half ? 0x7362 : 0x5140), a0, a1);
+                                    codes_to_f16<kE4m3>(__byte_perm(x[st][2][w], x[st][3][w], half ? 0x7362 : 0x5140), a2, a3);
+#pragma unroll
+                                    for (int h = 0; h < NT; ++h) mma16816(d[h], a0, a1, a2, a3, pb[h][2 * st], pb[h][2 * st + 1]);
+                                }
+                                const int i = (q4 * 4 + w) * 2 + half;
+#pragma unroll
+                                for (int h = 0; h < NT; ++h)
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) o[h][i][e] = fmaf(vs, d[h][e], o[h][i][e]);
+                            }
+                    }
+                    __syncwarp(); // every lane has read the stage
+                    if (lane == 0) fetch();
+                    if (++stage == S) stage = 0, phase ^= 1;
+                }
+                if (!ok) break;
+                // ---- the item's rows: a thread holds D / 8 consecutive dims, from g * D / 8 on, of the heads 2t and 2t + 1
+                const bool whole = first == 0 && end == at.n;
+                const int  slot  = first == 0 ? 1 : 0; // (of a cut unit)
+#pragma unroll
+                for (int h = 0; h < NT; ++h) {
+                    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+                    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+                    const int64_t prow = ((int64_t) run * 2 + slot) * p.G + h * 8;
+                    if (!whole && t == 0 && h * 8 + g < p.G) p.part_ml[(prow + g) * 2] = m[h], p.part_ml[(prow + g) * 2 + 1] = l[h];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float inv = 1.0f / __shfl_sync(0xffffffffu, l[h], t * 8 + e * 4);
+                        const int   hd  = h * 8 + 2 * t + e;
+                        if (hd >= p.G) continue;
+                        if (whole) {
+                            uint4 *to = reinterpret_cast<uint4 *>((T *) p.q.O + ((int64_t) at.b * p.q.Hq + hq0 + hd) * D + g * (D / 8));
+#pragma unroll
+                            for (int i = 0; i < MT / 4; ++i) {
+                                uint32_t w[4];
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) w[k] = pair16<T>(o[h][i * 4 + k][e] * inv, o[h][i * 4 + k][2 + e] * inv);
+                                to[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                            }
+                        } else {
+                            float4 *to = reinterpret_cast<float4 *>(p.part_o + (prow + 2 * t + e) * D + g * (D / 8));
+#pragma unroll
+                            for (int i = 0; i < MT / 2; ++i) to[i] = make_float4(o[h][2 * i][e], o[h][2 * i][2 + e], o[h][2 * i + 1][e], o[h][2 * i + 1][2 + e]);
+                        }
                     }
                 }
-                // O^T += V^T . P^T, 16 keys a step; word w of a thread's bytes holds the dims of two row tiles
-                constexpr int WPT = D / 32; // 4-byte words of a key per thread
-#pragma unroll
-                for (int q4 = 0; q4 < (WPT + 3) / 4; ++q4) {
-                    constexpr int NW = WPT < 4 ? WPT : 4;
-                    uint32_t      x[2][4][NW]; // [step][key][word]
-#pragma unroll
-                    for (int st = 0; st < 2; ++st)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const int      key  = st * 16 + 2 * t + (k & 1) + (k >> 1) * 8;
-                            const uint32_t byte = (uint32_t) key * D + g * (D / 8) + q4 * 16, a = sV + (byte ^ (((byte >> 7) & 7u) << 4));
-                            if (NW == 4) {
-                                const uint4 v = ptx::ld_shared_v4(a);
-                                x[st][k][0] = v.x, x[st][k][1] = v.y, x[st][k][NW - 2] = v.z, x[st][k][NW - 1] = v.w;
-                            } else {
-                                asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(x[st][k][0]), "=r"(x[st][k][1]) : "r"(a));
-                            }
-                            if (key >= nv) // the cache behind the last key may hold any bits
-#pragma unroll
-                                for (int w = 0; w < NW; ++w) x[st][k][w] = 0u;
-                        }
-#pragma unroll
-                    for (int w = 0; w < NW; ++w)
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            float d[NT][4];
-#pragma unroll
-                            for (int h = 0; h < NT; ++h) d[h][0] = d[h][1] = d[h][2] = d[h][3] = 0.f;
-#pragma unroll
-                            for (int st = 0; st < 2; ++st) {
-                                uint32_t a0, a1, a2, a3;
-                                codes_to_f16<kE4m3>(__byte_perm(x[st][0][w], x[st][1][w], half ? 0x7362 : 0x5140), a0, a1);
-                                codes_to_f16<kE4m3>(__byte_perm(x[st][2][w], x[st][3][w], half ? 0x7362 : 0x5140), a2, a3);
-#pragma unroll
-                                for (int h = 0; h < NT; ++h) mma16816(d[h], a0, a1, a2, a3, pb[h][2 * st], pb[h][2 * st + 1]);
-                            }
-                            const int i = (q4 * 4 + w) * 2 + half;
-#pragma unroll
-                            for (int h = 0; h < NT; ++h)
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) o[h][i][e] = fmaf(vs, d[h][e], o[h][i][e]);
-                        }
-                }
-                __syncwarp(); // every lane has read the stage
-                if (lane == 0) fetch();
-                if (++stage == S) stage = 0, phase ^= 1;
+                todo -= end - first;
+                if (!whole && slot == 1) cut = make_int4(at.b, at.hk, (P0 + (P1 - P0 - todo) - (end - first) + at.n - 1) / quota, 0);
+                if (todo > 0) next_unit(at);
             }
-
-            // ---- end of the item: the warps' (m, l, O) become one
-            float(*ml)[NT * 8][2] = reinterpret_cast<float(*)[NT * 8][2]>(gb + L::oMl + (items & 1) * (W * NT * 8 * 8));
-#pragma unroll
-            for (int h = 0; h < NT; ++h) {
-                l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-                l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-                if (t == 0) ml[warp][h * 8 + g][0] = m[h], ml[warp][h * 8 + g][1] = l[h];
-            }
-            __syncthreads();
-            // weight of warp w for head `hd`, against the largest maximum
-            auto top_of = [&](int hd) {
-                float r = -INFINITY;
-#pragma unroll
-                for (int w = 0; w < W; ++w) r = fmaxf(r, ml[w][hd][0]);
-                return r;
-            };
-            auto weight = [&](int w, int hd, float top) { return ml[w][hd][0] == -INFINITY && ml[w][hd][1] == 0.f ? 0.f : ex2(ml[w][hd][0] - top); };
-            float *buf = (float *) (gb + L::oBuf) + (warp % (W / 2)) * L::R * 33 + lane;
-#pragma unroll
-            for (int h = 0; h < NT; ++h) {
-                const int   h0 = h * 8 + 2 * t;
-                const float f0 = weight(warp, h0, top_of(h0)), f1 = weight(warp, h0 + 1, top_of(h0 + 1));
-#pragma unroll
-                for (int i = 0; i < MT; ++i) o[h][i][0] *= f0, o[h][i][1] *= f1, o[h][i][2] *= f0, o[h][i][3] *= f1;
-            }
-            if (warp >= W / 2) {
-#pragma unroll
-                for (int h = 0; h < NT; ++h)
-#pragma unroll
-                    for (int i = 0; i < MT; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) buf[((h * MT + i) * 4 + e) * 33] = o[h][i][e];
-            }
-            __syncthreads();
-            if (warp < W / 2) {
-#pragma unroll
-                for (int h = 0; h < NT; ++h)
-#pragma unroll
-                    for (int i = 0; i < MT; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) buf[((h * MT + i) * 4 + e) * 33] += o[h][i][e];
-            }
-            __syncthreads();
-            const bool whole = at == u.off && end == u.off + u.n;
-            const int  slot  = at == u.off ? 1 : 0; // (of a cut unit)
-            for (int i = threadIdx.x; i < p.G * D; i += W * 32) {
-                const int    hd = i / D, d = i % D, r = ((hd >> 3) * MT + ((d % (D / 8)) >> 1)) * 4 + (d & 1) * 2 + (hd & 1);
-                const float *x  = (const float *) (gb + L::oBuf) + r * 33 + (d / (D / 8)) * 4 + ((hd & 7) >> 1);
-                float        ov = 0.f;
-#pragma unroll
-                for (int w = 0; w < W / 2; ++w) ov += x[w * L::R * 33];
-                const float top = top_of(hd);
-                float       lv  = 0.f;
-#pragma unroll
-                for (int w = 0; w < W; ++w) lv += ml[w][hd][1] * weight(w, hd, top);
-                if (whole) {
-                    St<T>::st((T *) p.q.O + ((int64_t) u.b * p.q.Hq + hq0 + hd) * D + d, ov / lv);
-                } else {
-                    const int64_t row       = ((int64_t) blockIdx.x * 2 + slot) * p.G + hd;
-                    p.part_o[row * D + d] = ov;
-                    if (d == 0) p.part_ml[row * 2] = top, p.part_ml[row * 2 + 1] = lv;
-                }
-            }
-            if (!whole && slot == 1 && threadIdx.x == 0) {
-                int *cut = p.cut + blockIdx.x * 4;
-                cut[0] = u.b, cut[1] = u.hk, cut[2] = (u.off + u.n - 1) / quota;
-            }
-            at = end;
         }
+        if (lane == 0) p.cut[run] = cut;
         if (ctl[0])
             for (int i = 0; i < 50; ++i) __nanosleep(20000); // aborted: let copies in flight land
     }
 
-    // Joins the partials of the cut unit that begins in CTA blockIdx.x's run: its slot 1, then slot 0 of the CTAs behind it.
-    template <typename T> __global__ void __launch_bounds__(256) attn_decode_q8_join_kernel(const StreamParams p, int D) {
+    // Joins the partials of the cut unit that begins in run blockIdx.x: its slot 1, then slot 0 of the runs behind it. A thread
+    // takes four dims of one head over every `groups`-th run; the groups meet in shared memory, in order.
+    constexpr int kJoinThreads = 512;
+    template <typename T> __global__ void __launch_bounds__(kJoinThreads) attn_decode_q8_join_kernel(const StreamParams p, int D) {
+        __shared__ float4 so[kJoinThreads];
+        __shared__ float  sl[kJoinThreads], st[kJoinThreads];
         vkc_grid_dep_wait();
         vkc_grid_dep_launch();
-        const int c = blockIdx.x, last = p.cut[c * 4 + 2];
+        const int  c = blockIdx.x;
+        const int4 cut = p.cut[c];
+        const int  last = cut.z;
         if (last < 0) return;
-        const int64_t b = p.cut[c * 4], hk = p.cut[c * 4 + 1];
-        auto          row = [&](int cc, int hd) { return ((int64_t) cc * 2 + (cc == c ? 1 : 0)) * p.G + hd; };
-        for (int i = threadIdx.x; i < p.G * D; i += blockDim.x) {
-            const int hd = i / D, d = i % D;
-            float     top = -INFINITY, lt = 0.f, ot = 0.f;
-            for (int cc = c; cc <= last; ++cc) top = fmaxf(top, p.part_ml[row(cc, hd) * 2]);
-            for (int cc = c; cc <= last; ++cc) {
-                const float a = ex2(p.part_ml[row(cc, hd) * 2] - top);
-                lt += p.part_ml[row(cc, hd) * 2 + 1] * a;
-                ot += p.part_o[row(cc, hd) * D + d] * a;
+        const int lanes  = p.G * D / 4 < kJoinThreads ? p.G * D / 4 : kJoinThreads; // threads that cover the unit's rows
+        const int groups = kJoinThreads / lanes, grp = threadIdx.x / lanes, ln = threadIdx.x - grp * lanes;
+        for (int i0 = 0; i0 < p.G * D / 4; i0 += lanes) {
+            const int  i = i0 + ln, hd = i * 4 / D, d = i * 4 - hd * D;
+            const bool in = grp < groups && i < p.G * D / 4;
+            float      top = -INFINITY, lt = 0.f;
+            float4     ot = make_float4(0.f, 0.f, 0.f, 0.f);
+            auto       row = [&](int r) { return ((int64_t) r * 2 + (r == c ? 1 : 0)) * p.G + hd; };
+            if (in) {
+                for (int r = c + grp; r <= last; r += groups) top = fmaxf(top, p.part_ml[row(r) * 2]);
+#pragma unroll 4
+                for (int r = c + grp; r <= last; r += groups) {
+                    const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + row(r) * 2);
+                    const float4 v  = *reinterpret_cast<const float4 *>(p.part_o + row(r) * D + d);
+                    const float  a  = ml.x == -INFINITY && ml.y == 0.f ? 0.f : ex2(ml.x - top);
+                    lt += ml.y * a;
+                    ot.x += v.x * a, ot.y += v.y * a, ot.z += v.z * a, ot.w += v.w * a;
+                }
             }
-            St<T>::st((T *) p.q.O + (b * p.q.Hq + hk * p.G + hd) * D + d, ot / lt);
+            so[threadIdx.x] = ot, sl[threadIdx.x] = lt, st[threadIdx.x] = top;
+            __syncthreads();
+            if (grp == 0 && in) {
+                float all = top;
+                for (int k = 1; k < groups; ++k) all = fmaxf(all, st[k * lanes + ln]);
+                float  ls = 0.f;
+                float4 os = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int k = 0; k < groups; ++k) {
+                    const int   x = k * lanes + ln;
+                    const float a = st[x] == -INFINITY && sl[x] == 0.f ? 0.f : ex2(st[x] - all);
+                    ls += sl[x] * a;
+                    os.x += so[x].x * a, os.y += so[x].y * a, os.z += so[x].z * a, os.w += so[x].w * a;
+                }
+                T *to = (T *) p.q.O + ((int64_t) cut.x * p.q.Hq + (int64_t) cut.y * p.G + hd) * D + d;
+                const uint2 w = make_uint2(pair16<T>(os.x / ls, os.y / ls), pair16<T>(os.z / ls, os.w / ls));
+                *reinterpret_cast<uint2 *>(to) = w;
+            }
+            __syncthreads();
         }
     }
 
-    // Bytes of the workspace: partials of two cut units per CTA, and what was cut.
-    size_t stream_ws(int64_t G, int64_t D) { return (size_t) kMaxCtas * 2 * (size_t) G * (size_t) (D + 2) * 4 + (size_t) kMaxCtas * 16; }
+    // Runs of a launch that can have tiles, and bytes of the workspace: partials of two cut units for each of them, and what was
+    // cut (an entry for every warp).
+    int64_t stream_runs(int64_t B, int64_t Hkv, int64_t Lmax, int64_t D) {
+        const int64_t most = kMaxCtas * (D == 256 ? 4 : 8), b = B < kSliceB ? B : kSliceB;
+        const int64_t need = (b * Hkv * ((Lmax + kTile - 1) / kTile) + kMinTiles - 1) / kMinTiles;
+        return need < most ? need : most;
+    }
+    size_t stream_ws(int64_t B, int64_t Hq, int64_t Hkv, int64_t Lmax, int64_t D) {
+        return (size_t) stream_runs(B, Hkv, Lmax, D) * 2 * (size_t) (Hq / Hkv) * (size_t) (D + 2) * 4 + (size_t) kMaxCtas * 8 * 16;
+    }
 
     template <typename T, int D, int NT, bool kE4m3>
-    int launch_stream(vkc_ctx *ctx, const StreamParams &p, int grid, const CUtensorMap &tk, const CUtensorMap &tv, cudaStream_t st) {
+    int launch_stream(vkc_ctx *ctx, const StreamParams &p, int grid, int runs, const CUtensorMap &tk, const CUtensorMap &tv, cudaStream_t st) {
         auto          kern = attn_decode_q8_kernel<T, D, NT, kE4m3>;
         constexpr int smem = (int) Stream<D, NT>::total;
         if (int rc = vkc_configure_smem(ctx, kern, smem)) return rc;
         vkc_launch(ctx, kern, dim3((unsigned) grid), dim3(Stream<D, NT>::W * 32), smem, st, tk, tv, p);
         if (int rc = vkc_post_launch(ctx, "attn_decode_q8")) return rc;
-        vkc_launch(ctx, attn_decode_q8_join_kernel<T>, dim3((unsigned) grid), dim3(256), 0, st, p, D);
+        vkc_launch(ctx, attn_decode_q8_join_kernel<T>, dim3((unsigned) (runs < grid * Stream<D, NT>::W ? runs : grid * Stream<D, NT>::W)), dim3(kJoinThreads), 0, st, p, D);
         return vkc_post_launch(ctx, "attn_decode_q8_join");
     }
-    template <typename T, int D> int pick_stream_form(vkc_ctx *ctx, const StreamParams &p, bool e4m3, int grid, const CUtensorMap &tk, const CUtensorMap &tv, cudaStream_t st) {
-        if (p.G <= 8) return e4m3 ? launch_stream<T, D, 1, true>(ctx, p, grid, tk, tv, st) : launch_stream<T, D, 1, false>(ctx, p, grid, tk, tv, st);
-        return e4m3 ? launch_stream<T, D, 2, true>(ctx, p, grid, tk, tv, st) : launch_stream<T, D, 2, false>(ctx, p, grid, tk, tv, st);
+    template <typename T, int D> int pick_stream_form(vkc_ctx *ctx, const StreamParams &p, bool e4m3, int grid, int runs, const CUtensorMap &tk, const CUtensorMap &tv, cudaStream_t st) {
+        if (p.G <= 8) return e4m3 ? launch_stream<T, D, 1, true>(ctx, p, grid, runs, tk, tv, st) : launch_stream<T, D, 1, false>(ctx, p, grid, runs, tk, tv, st);
+        return e4m3 ? launch_stream<T, D, 2, true>(ctx, p, grid, runs, tk, tv, st) : launch_stream<T, D, 2, false>(ctx, p, grid, runs, tk, tv, st);
     }
 
     // The streaming form for the whole call, kSliceB sequences per launch.
@@ -561,14 +565,15 @@ namespace {
             p.q.Q = (const char *) q.Q + b0 * q.Hq * D * 2, p.q.O = (char *) q.O + b0 * q.Hq * D * 2;
             p.q.Kc += cache0, p.q.Vc += cache0, p.q.ks += scale0, p.q.vs += scale0;
             if (q.kv_len) p.q.kv_len += b0;
-            p.min_tiles = 8;
-            p.dev_err   = ctx->dev_err;
-            const int64_t tiles = p.B * q.Hkv * ((q.Lmax + kTile - 1) / kTile);
-            int           grid  = ctx->sm_count < kMaxCtas ? ctx->sm_count : kMaxCtas;
-            if ((tiles + p.min_tiles - 1) / p.min_tiles < grid) grid = (int) ((tiles + p.min_tiles - 1) / p.min_tiles);
+            p.dev_err = ctx->dev_err;
+            // one CTA per SM, or one for each run where there are fewer (a CTA's runs are spread over the line, so that the others
+            // of its warps are then idle)
+            const int64_t runs = stream_runs(B, q.Hkv, q.Lmax, D), here = stream_runs(p.B, q.Hkv, q.Lmax, D);
+            int64_t       grid = ctx->sm_count < kMaxCtas ? ctx->sm_count : kMaxCtas;
+            if (grid > here) grid = here;
             p.part_o  = (float *) ws;
-            p.part_ml = p.part_o + (size_t) kMaxCtas * 2 * G * D;
-            p.cut     = (int *) (p.part_ml + (size_t) kMaxCtas * 2 * G * 2);
+            p.part_ml = p.part_o + runs * 2 * G * D;
+            p.cut     = (int4 *) (p.part_ml + runs * 2 * G * 2);
             // both caches as rows of 128 bytes, whatever D is
             CUtensorMap    tk, tv;
             const uint64_t dims[2] = {64, (uint64_t) (p.B * per * D / 128)}, stride[1] = {128};
@@ -577,12 +582,12 @@ namespace {
             if (int rc = vkc_make_tmap(ctx, &tv, VKC_F16, p.q.Vc, 2, dims, stride, box)) return rc;
             int rc;
             if (dtype == VKC_F16)
-                rc = D == 64 ? pick_stream_form<__half, 64>(ctx, p, e4m3, grid, tk, tv, st) : D == 128 ? pick_stream_form<__half, 128>(ctx, p, e4m3, grid, tk, tv, st)
-                                                                                                       : pick_stream_form<__half, 256>(ctx, p, e4m3, grid, tk, tv, st);
+                rc = D == 64 ? pick_stream_form<__half, 64>(ctx, p, e4m3, (int) grid, (int) here, tk, tv, st) : D == 128 ? pick_stream_form<__half, 128>(ctx, p, e4m3, (int) grid, (int) here, tk, tv, st)
+                                                                                                       : pick_stream_form<__half, 256>(ctx, p, e4m3, (int) grid, (int) here, tk, tv, st);
             else
-                rc = D == 64 ? pick_stream_form<__nv_bfloat16, 64>(ctx, p, e4m3, grid, tk, tv, st)
-                             : D == 128 ? pick_stream_form<__nv_bfloat16, 128>(ctx, p, e4m3, grid, tk, tv, st)
-                                        : pick_stream_form<__nv_bfloat16, 256>(ctx, p, e4m3, grid, tk, tv, st);
+                rc = D == 64 ? pick_stream_form<__nv_bfloat16, 64>(ctx, p, e4m3, (int) grid, (int) here, tk, tv, st)
+                             : D == 128 ? pick_stream_form<__nv_bfloat16, 128>(ctx, p, e4m3, (int) grid, (int) here, tk, tv, st)
+                                        : pick_stream_form<__nv_bfloat16, 256>(ctx, p, e4m3, (int) grid, (int) here, tk, tv, st);
             if (rc) return rc;
         }
         return VKC_OK;
@@ -597,7 +602,7 @@ namespace {
 
 extern "C" size_t vkc_attn_decode_q8_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Lmax, int64_t D) {
     if (B <= 0 || Hq <= 0 || Hkv <= 0 || Lmax <= 0 || D <= 0) return 0;
-    return stream_ws(Hq / Hkv, D);
+    return stream_ws(B, Hq, Hkv, Lmax, D);
 }
 
 extern "C" int vkc_attn_decode_q8(vkc_ctx *ctx, const void *Q, const void *Kc, const void *Vc, const float *k_scale, const float *v_scale, void *O,
@@ -611,7 +616,7 @@ extern "C" int vkc_attn_decode_q8(vkc_ctx *ctx, const void *Q, const void *Kc, c
     VKC_REQUIRE(ctx, Hq <= 65535 * 16, "attn_decode_q8: extents too large");
     if (B == 0) return VKC_OK;
     VKC_REQUIRE(ctx, Q && Kc && Vc && k_scale && v_scale && O, "attn_decode_q8: null tensor");
-    VKC_REQUIRE(ctx, !(((uintptr_t) Q | (uintptr_t) Kc | (uintptr_t) Vc) & 15), "attn_decode_q8: Q and the cache must be 16-byte aligned");
+    VKC_REQUIRE(ctx, !(((uintptr_t) Q | (uintptr_t) O | (uintptr_t) Kc | (uintptr_t) Vc) & 15), "attn_decode_q8: Q, O and the cache must be 16-byte aligned");
     const size_t need = vkc_attn_decode_q8_workspace_bytes(B, Hq, Hkv, Lmax, D);
     VKC_REQUIRE(ctx, !workspace || (workspace_bytes >= need && !((uintptr_t) workspace & 15)),
                 "attn_decode_q8: workspace of %zu bytes is smaller than the %zu required, or not 16-byte aligned", workspace_bytes, need);
