@@ -22,6 +22,7 @@
 // columns.
 // A unit that lies in one run is finished there; one that is cut leaves a partial (maximum, sum, O) per run in the workspace
 // (slot 0: the unit began in an earlier run, slot 1: in this one) and a second kernel joins them in the order of the runs.
+// (Joined by the warp whose partial arrives last instead, the batch took 73 us, not 67: the fences hold up the stream.)
 #include "kv_q8.cuh"
 #include "ptx.cuh"
 #include "tensormap.cuh"
@@ -104,7 +105,7 @@ namespace {
         int         block_log2;
         float      *part_o;  // [runs][2][G][D]
         float      *part_ml; // [runs][2][G][2]
-        int4       *cut;     // [runs]: sequence, kv head, last run of the cut unit that begins in this run (-1: none)
+        int        *line;    // [B + 1] first line position of each sequence, then the tiles of a run: written for the join
         int        *dev_err;
     };
 
@@ -167,7 +168,7 @@ namespace {
 
     template <typename T, int D, int NT, bool kE4m3>
     __global__ void __launch_bounds__(Stream<D, NT>::W * 32, 1)
-        attn_decode_q8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const StreamParams p) {
+        attn_decode_q8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ StreamParams p) {
         using L          = Stream<D, NT>;
         constexpr int W = L::W, S = L::S, CH = L::CH, MT = L::MT;
         extern __shared__ uint8_t smem_raw[];
@@ -224,9 +225,10 @@ namespace {
         const int total = tab[p.B], runs = (int) gridDim.x * W, run = warp * (int) gridDim.x + (int) blockIdx.x;
         int       quota = (total + runs - 1) / runs;
         if (quota < kMinTiles) quota = kMinTiles;
+        if (blockIdx.x == 0)
+            for (int i = threadIdx.x; i <= p.B + 1; i += W * 32) p.line[i] = i <= p.B ? tab[i] : quota;
         const int64_t c0 = (int64_t) run * quota;
         const int     P0 = c0 < total ? (int) c0 : total, P1 = c0 + quota < total ? (int) (c0 + quota) : total;
-        int4          cut = make_int4(0, 0, -1, 0);
         bool          ok  = true;
         if (P0 < P1) {
             At at; // of P0
@@ -254,6 +256,14 @@ namespace {
             const uint32_t ring = base + L::oRing + (uint32_t) warp * S * 2 * L::TILE, bars = base + L::oBar + 8u * (uint32_t) (warp * S);
             float         *sc   = (float *) (gb + L::oSc) + warp * S * 2;
             const uint32_t sc_a = base + L::oSc + (uint32_t) warp * S * 8;
+
+            // Where in a swizzled tile this lane's chunks of the keys g, g + 8, ... (K) and 2t, 2t + 8, ... and 2t + 1, ... (V) begin. Eight
+            // keys further the swizzle is the same again, except that for D = 64 (eight keys are four rows of 128 bytes) bit 6 flips.
+            auto     swz = [](uint32_t byte) { return byte ^ (((byte >> 7) & 7u) << 4); };
+            uint32_t k_at[CH], v_at[2];
+#pragma unroll
+            for (int c = 0; c < CH; ++c) k_at[c] = swz((uint32_t) g * D + (D == 256 ? (c >> 1) * 8 + (t & 1) + (t >> 1) * 4 + 2 * (c & 1) : t * CH + c) * 16u);
+            v_at[0] = swz((uint32_t) (2 * t) * D + g * (D / 8)), v_at[1] = swz((uint32_t) (2 * t + 1) * D + g * (D / 8));
 
             // ---- producer (lane 0): the tile at `pa` into stage `ps`
             At   pa = at;
@@ -340,11 +350,9 @@ namespace {
                     for (int n = 0; n < 4; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
                     for (int c = 0; c < CH; ++c) {
-                        const int chunk = D == 256 ? (c >> 1) * 8 + (t & 1) + (t >> 1) * 4 + 2 * (c & 1) : t * CH + c;
 #pragma unroll
                         for (int n = 0; n < 4; ++n) {
-                            const uint32_t byte = (uint32_t) (n * 8 + g) * D + chunk * 16;
-                            const uint4    kv   = ptx::ld_shared_v4(sK + (byte ^ (((byte >> 7) & 7u) << 4)));
+                            const uint4    kv   = ptx::ld_shared_v4(sK + n * 8 * D + (D == 64 && (n & 1) ? k_at[c] ^ 64u : k_at[c]));
                             const uint32_t w[4] = {kv.x, kv.y, kv.z, kv.w};
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
@@ -361,13 +369,14 @@ namespace {
                         const float f = fac[h] * ks;
                         float       x[8], mx = -INFINITY;
 #pragma unroll
-                        for (int n = 0; n < 4; ++n)
+                        for (int n = 0; n < 4; ++n) x[2 * n] = s[n][h * 2] * f, x[2 * n + 1] = s[n][h * 2 + 1] * f;
+                        if (nv < kTile) {
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const float v = s[n][h * 2 + e] * f;
-                                x[n * 2 + e]  = n * 8 + 2 * t + e < nv ? v : -INFINITY;
-                                mx            = fmaxf(mx, x[n * 2 + e]);
-                            }
+                            for (int i = 0; i < 8; ++i)
+                                if ((i >> 1) * 8 + 2 * t + (i & 1) >= nv) x[i] = -INFINITY;
+                        }
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) mx = fmaxf(mx, x[i]);
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                         // the maximum is raised only when it grows by more than 2^8: P stays below 2^15 in f16
@@ -398,18 +407,23 @@ namespace {
                         for (int st = 0; st < 2; ++st)
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
-                                const int      key  = st * 16 + 2 * t + (k & 1) + (k >> 1) * 8;
-                                const uint32_t byte = (uint32_t) key * D + g * (D / 8) + q4 * 16, a = sV + (byte ^ (((byte >> 7) & 7u) << 4));
+                                const uint32_t a = sV + (st * 2 + (k >> 1)) * 8 * D + ((D == 64 && (k >> 1) ? v_at[k & 1] ^ 64u : v_at[k & 1]) ^ (q4 * 16u));
                                 if (NW == 4) {
                                     const uint4 v = ptx::ld_shared_v4(a);
                                     x[st][k][0] = v.x, x[st][k][1] = v.y, x[st][k][NW - 2] = v.z, x[st][k][NW - 1] = v.w;
                                 } else {
                                     asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(x[st][k][0]), "=r"(x[st][k][1]) : "r"(a));
                                 }
-                                if (key >= nv) // the cache behind the last key may hold any bits
-#pragma unroll
-                                    for (int w = 0; w < NW; ++w) x[st][k][w] = 0u;
                             }
+                        if (nv < kTile) { // the cache behind the last key may hold any bits
+#pragma unroll
+                            for (int st = 0; st < 2; ++st)
+#pragma unroll
+                                for (int k = 0; k < 4; ++k)
+                                    if (st * 16 + 2 * t + (k & 1) + (k >> 1) * 8 >= nv)
+#pragma unroll
+                                        for (int w = 0; w < NW; ++w) x[st][k][w] = 0u;
+                        }
 #pragma unroll
                         for (int w = 0; w < NW; ++w)
 #pragma unroll
@@ -468,91 +482,108 @@ namespace {
                     }
                 }
                 todo -= end - first;
-                if (!whole && slot == 1) cut = make_int4(at.b, at.hk, (P0 + (P1 - P0 - todo) - (end - first) + at.n - 1) / quota, 0);
                 if (todo > 0) next_unit(at);
             }
         }
-        if (lane == 0) p.cut[run] = cut;
         if (ctl[0])
             for (int i = 0; i < 50; ++i) __nanosleep(20000); // aborted: let copies in flight land
     }
 
-    // Joins the partials of the cut unit that begins in run blockIdx.x: its slot 1, then slot 0 of the runs behind it. A thread
-    // takes four dims of one head over every `groups`-th run; the groups meet in shared memory, in order.
-    constexpr int kJoinThreads = 512;
-    template <typename T> __global__ void __launch_bounds__(kJoinThreads) attn_decode_q8_join_kernel(const StreamParams p, int D) {
-        __shared__ float4 so[kJoinThreads];
-        __shared__ float  sl[kJoinThreads], st[kJoinThreads];
+    // Joins the partials of unit (sequence blockIdx.y, kv head blockIdx.x) if it was cut: slot 1 of the run it begins in, slot 0 of the
+    // runs behind it. A thread takes four dims of one head over every `groups`-th partial, eight of them on their way at a time;
+    // the groups meet in shared memory, in order.
+    template <typename T, int D> __global__ void __launch_bounds__(1024) attn_decode_q8_join_kernel(const StreamParams p, int lanes) {
+        constexpr int U = 8;
+        extern __shared__ float4 sm4[]; // [threads] O, then [threads] (maximum, sum)
+        float2        *sml = reinterpret_cast<float2 *>(sm4 + blockDim.x);
+        const int      b = blockIdx.y, hk = blockIdx.x, grp = threadIdx.x / lanes, ln = threadIdx.x - grp * lanes, groups = blockDim.x / lanes;
         vkc_grid_dep_wait();
         vkc_grid_dep_launch();
-        const int  c = blockIdx.x;
-        const int4 cut = p.cut[c];
-        const int  last = cut.z;
-        if (last < 0) return;
-        const int lanes  = p.G * D / 4 < kJoinThreads ? p.G * D / 4 : kJoinThreads; // threads that cover the unit's rows
-        const int groups = kJoinThreads / lanes, grp = threadIdx.x / lanes, ln = threadIdx.x - grp * lanes;
-        for (int i0 = 0; i0 < p.G * D / 4; i0 += lanes) {
-            const int  i = i0 + ln, hd = i * 4 / D, d = i * 4 - hd * D;
-            const bool in = grp < groups && i < p.G * D / 4;
-            float      top = -INFINITY, lt = 0.f;
-            float4     ot = make_float4(0.f, 0.f, 0.f, 0.f);
-            auto       row = [&](int r) { return ((int64_t) r * 2 + (r == c ? 1 : 0)) * p.G + hd; };
-            if (in) {
-                for (int r = c + grp; r <= last; r += groups) top = fmaxf(top, p.part_ml[row(r) * 2]);
-#pragma unroll 4
-                for (int r = c + grp; r <= last; r += groups) {
-                    const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + row(r) * 2);
-                    const float4 v  = *reinterpret_cast<const float4 *>(p.part_o + row(r) * D + d);
-                    const float  a  = ml.x == -INFINITY && ml.y == 0.f ? 0.f : ex2(ml.x - top);
-                    lt += ml.y * a;
-                    ot.x += v.x * a, ot.y += v.y * a, ot.z += v.z * a, ot.w += v.w * a;
-                }
+        const int t0 = p.line[b], t1 = p.line[b + 1], quota = p.line[p.B + 1];
+        const int n = (t1 - t0) / (int) p.q.Hkv, off = t0 + hk * n;
+        const int r0 = off / quota, parts = n > 0 ? (off + n - 1) / quota - r0 + 1 : 0;
+        if (parts < 2) return;
+        const int  hd = ln * 4 / D, d = ln * 4 - hd * D;
+        const bool in = hd < p.G;
+        auto       row = [&](int k) { return ((int64_t) (r0 + k) * 2 + (k ? 0 : 1)) * p.G + hd; };
+        float      top = -INFINITY, ls = 0.f;
+        float4     acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto       merge = [&](const float2 (&ml)[U], const float4 (&v)[U]) {
+            float now = top;
+#pragma unroll
+            for (int u = 0; u < U; ++u) now = fmaxf(now, ml[u].x);
+            // (a part whose scores were all NaN has the maximum -inf and the sum NaN, which must stay)
+            const float keep = top == -INFINITY && ls == 0.f ? 0.f : ex2(top - now);
+            ls *= keep, acc.x *= keep, acc.y *= keep, acc.z *= keep, acc.w *= keep;
+            top = now;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float a = ml[u].x == -INFINITY && ml[u].y == 0.f ? 0.f : ex2(ml[u].x - now);
+                ls            = fmaf(ml[u].y, a, ls);
+                acc.x = fmaf(v[u].x, a, acc.x), acc.y = fmaf(v[u].y, a, acc.y), acc.z = fmaf(v[u].z, a, acc.z), acc.w = fmaf(v[u].w, a, acc.w);
             }
-            so[threadIdx.x] = ot, sl[threadIdx.x] = lt, st[threadIdx.x] = top;
-            __syncthreads();
-            if (grp == 0 && in) {
-                float all = top;
-                for (int k = 1; k < groups; ++k) all = fmaxf(all, st[k * lanes + ln]);
-                float  ls = 0.f;
-                float4 os = make_float4(0.f, 0.f, 0.f, 0.f);
-                for (int k = 0; k < groups; ++k) {
-                    const int   x = k * lanes + ln;
-                    const float a = st[x] == -INFINITY && sl[x] == 0.f ? 0.f : ex2(st[x] - all);
-                    ls += sl[x] * a;
-                    os.x += so[x].x * a, os.y += so[x].y * a, os.z += so[x].z * a, os.w += so[x].w * a;
-                }
-                T *to = (T *) p.q.O + ((int64_t) cut.x * p.q.Hq + (int64_t) cut.y * p.G + hd) * D + d;
-                const uint2 w = make_uint2(pair16<T>(os.x / ls, os.y / ls), pair16<T>(os.z / ls, os.w / ls));
-                *reinterpret_cast<uint2 *>(to) = w;
+        };
+        float2 ml[U];
+        float4 v[U];
+        for (int k0 = grp; k0 < parts && in; k0 += U * groups) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int  k    = k0 + u * groups;
+                const bool have = k < parts;
+                ml[u]           = have ? *reinterpret_cast<const float2 *>(p.part_ml + row(k) * 2) : make_float2(-INFINITY, 0.f);
+                v[u]            = have ? *reinterpret_cast<const float4 *>(p.part_o + row(k) * D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
+            merge(ml, v);
+        }
+        if (groups > 1) {
+            sm4[threadIdx.x] = acc, sml[threadIdx.x] = make_float2(top, ls);
             __syncthreads();
+            if (grp != 0) return;
+            top = -INFINITY, ls = 0.f, acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                ml[u] = u < groups ? sml[u * lanes + ln] : make_float2(-INFINITY, 0.f);
+                v[u]  = u < groups ? sm4[u * lanes + ln] : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            merge(ml, v);
+        }
+        if (in) {
+            const float inv = 1.0f / ls;
+            T          *to  = (T *) p.q.O + ((int64_t) b * p.q.Hq + (int64_t) hk * p.G + hd) * D + d;
+            *reinterpret_cast<uint2 *>(to) = make_uint2(pair16<T>(acc.x * inv, acc.y * inv), pair16<T>(acc.z * inv, acc.w * inv));
         }
     }
 
-    // Runs of a launch that can have tiles, and bytes of the workspace: partials of two cut units for each of them, and what was
-    // cut (an entry for every warp).
+    // Runs of a launch that can have tiles, and bytes of the workspace: partials of two cut units for each of them, and the line.
     int64_t stream_runs(int64_t B, int64_t Hkv, int64_t Lmax, int64_t D) {
         const int64_t most = kMaxCtas * (D == 256 ? 4 : 8), b = B < kSliceB ? B : kSliceB;
         const int64_t need = (b * Hkv * ((Lmax + kTile - 1) / kTile) + kMinTiles - 1) / kMinTiles;
         return need < most ? need : most;
     }
     size_t stream_ws(int64_t B, int64_t Hq, int64_t Hkv, int64_t Lmax, int64_t D) {
-        return (size_t) stream_runs(B, Hkv, Lmax, D) * 2 * (size_t) (Hq / Hkv) * (size_t) (D + 2) * 4 + (size_t) kMaxCtas * 8 * 16;
+        return (size_t) stream_runs(B, Hkv, Lmax, D) * 2 * (size_t) (Hq / Hkv) * (size_t) (D + 2) * 4 + (kSliceB + 4) * 4;
     }
 
     template <typename T, int D, int NT, bool kE4m3>
-    int launch_stream(vkc_ctx *ctx, const StreamParams &p, int grid, int runs, const CUtensorMap &tk, const CUtensorMap &tv, cudaStream_t st) {
+    int launch_stream(vkc_ctx *ctx, const StreamParams &p, int grid, const CUtensorMap &tk, const CUtensorMap &tv, cudaStream_t st) {
         auto          kern = attn_decode_q8_kernel<T, D, NT, kE4m3>;
         constexpr int smem = (int) Stream<D, NT>::total;
         if (int rc = vkc_configure_smem(ctx, kern, smem)) return rc;
         vkc_launch(ctx, kern, dim3((unsigned) grid), dim3(Stream<D, NT>::W * 32), smem, st, tk, tv, p);
         if (int rc = vkc_post_launch(ctx, "attn_decode_q8")) return rc;
-        vkc_launch(ctx, attn_decode_q8_join_kernel<T>, dim3((unsigned) (runs < grid * Stream<D, NT>::W ? runs : grid * Stream<D, NT>::W)), dim3(kJoinThreads), 0, st, p, D);
+        // threads of the join: the rows of a unit, times up to eight groups where a unit is cut into many parts (as many as it would
+        // be with sequences of full length)
+        const int     lanes = (p.G * D / 4 + 31) / 32 * 32;
+        const int64_t parts = (int64_t) grid * Stream<D, NT>::W / ((int64_t) p.B * p.q.Hkv);
+        int           groups = 1;
+        while (groups < 8 && parts > 8 * groups && lanes * groups * 2 <= 1024) groups *= 2;
+        const int threads = lanes * groups;
+        vkc_launch(ctx, attn_decode_q8_join_kernel<T, D>, dim3((unsigned) p.q.Hkv, (unsigned) p.B), dim3((unsigned) threads), (size_t) threads * 24, st, p, lanes);
         return vkc_post_launch(ctx, "attn_decode_q8_join");
     }
-    template <typename T, int D> int pick_stream_form(vkc_ctx *ctx, const StreamParams &p, bool e4m3, int grid, int runs, const CUtensorMap &tk, const CUtensorMap &tv, cudaStream_t st) {
-        if (p.G <= 8) return e4m3 ? launch_stream<T, D, 1, true>(ctx, p, grid, runs, tk, tv, st) : launch_stream<T, D, 1, false>(ctx, p, grid, runs, tk, tv, st);
-        return e4m3 ? launch_stream<T, D, 2, true>(ctx, p, grid, runs, tk, tv, st) : launch_stream<T, D, 2, false>(ctx, p, grid, runs, tk, tv, st);
+    template <typename T, int D> int pick_stream_form(vkc_ctx *ctx, const StreamParams &p, bool e4m3, int grid, const CUtensorMap &tk, const CUtensorMap &tv, cudaStream_t st) {
+        if (p.G <= 8) return e4m3 ? launch_stream<T, D, 1, true>(ctx, p, grid, tk, tv, st) : launch_stream<T, D, 1, false>(ctx, p, grid, tk, tv, st);
+        return e4m3 ? launch_stream<T, D, 2, true>(ctx, p, grid, tk, tv, st) : launch_stream<T, D, 2, false>(ctx, p, grid, tk, tv, st);
     }
 
     // The streaming form for the whole call, kSliceB sequences per launch.
@@ -573,7 +604,7 @@ namespace {
             if (grid > here) grid = here;
             p.part_o  = (float *) ws;
             p.part_ml = p.part_o + runs * 2 * G * D;
-            p.cut     = (int4 *) (p.part_ml + runs * 2 * G * 2);
+            p.line    = (int *) (p.part_ml + runs * 2 * G * 2);
             // both caches as rows of 128 bytes, whatever D is
             CUtensorMap    tk, tv;
             const uint64_t dims[2] = {64, (uint64_t) (p.B * per * D / 128)}, stride[1] = {128};
@@ -582,12 +613,12 @@ namespace {
             if (int rc = vkc_make_tmap(ctx, &tv, VKC_F16, p.q.Vc, 2, dims, stride, box)) return rc;
             int rc;
             if (dtype == VKC_F16)
-                rc = D == 64 ? pick_stream_form<__half, 64>(ctx, p, e4m3, (int) grid, (int) here, tk, tv, st) : D == 128 ? pick_stream_form<__half, 128>(ctx, p, e4m3, (int) grid, (int) here, tk, tv, st)
-                                                                                                       : pick_stream_form<__half, 256>(ctx, p, e4m3, (int) grid, (int) here, tk, tv, st);
+                rc = D == 64 ? pick_stream_form<__half, 64>(ctx, p, e4m3, (int) grid, tk, tv, st) : D == 128 ? pick_stream_form<__half, 128>(ctx, p, e4m3, (int) grid, tk, tv, st)
+                                                                                                       : pick_stream_form<__half, 256>(ctx, p, e4m3, (int) grid, tk, tv, st);
             else
-                rc = D == 64 ? pick_stream_form<__nv_bfloat16, 64>(ctx, p, e4m3, (int) grid, (int) here, tk, tv, st)
-                             : D == 128 ? pick_stream_form<__nv_bfloat16, 128>(ctx, p, e4m3, (int) grid, (int) here, tk, tv, st)
-                                        : pick_stream_form<__nv_bfloat16, 256>(ctx, p, e4m3, (int) grid, (int) here, tk, tv, st);
+                rc = D == 64 ? pick_stream_form<__nv_bfloat16, 64>(ctx, p, e4m3, (int) grid, tk, tv, st)
+                             : D == 128 ? pick_stream_form<__nv_bfloat16, 128>(ctx, p, e4m3, (int) grid, tk, tv, st)
+                                        : pick_stream_form<__nv_bfloat16, 256>(ctx, p, e4m3, (int) grid, tk, tv, st);
             if (rc) return rc;
         }
         return VKC_OK;
