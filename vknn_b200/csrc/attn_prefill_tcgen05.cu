@@ -87,6 +87,10 @@ namespace {
         // stored (of the merge kernel in the balanced form), flag[d] (a word in destination d's memory) receives this rank's
         // count of completed fan-outs
         FanOut fan;
+        // Packed sequences (kPacked): unit `u` of a head is a group of query tiles of the sequence that vkc_packed_find names; Sq and
+        // Skv above are the totals, O's rows follow os[2] from the first row of the first sequence.
+        const int32_t *cu_q, *cu_k;
+        int64_t        nseq;
     };
 
     // Key tiles the 128-row query tile that starts at row `first` needs when `len` keys are visible to the sequence.
@@ -122,6 +126,7 @@ namespace {
         int     adv;      // how far the item moves the CTA along the line
         int64_t m0, len;  // first query row of the unit, visible key length
         int     n_t[QT], n_max;
+        int     q0, k0, sq; // packed: first query and key row of the sequence, its query length (m0 and len count within it)
     };
     // Which CTA of which grid (the kernel passes blockIdx / gridDim.x; the host walks the same arithmetic for its plan report).
     struct CtaId {
@@ -205,6 +210,36 @@ namespace {
         }
         return w;
     }
+
+#ifdef __CUDACC__
+    // The same for packed sequences: CTA c.x of head c.y is one unit.
+    template <int QT> __device__ __forceinline__ Work<QT> packed_work(const AttnParams &p, int pos, const CtaId c) {
+        Work<QT> w;
+        w.valid = pos < 1;
+        if (!w.valid) return w;
+        int64_t       first;
+        const int64_t b = vkc_packed_find(p.cu_q, p.nseq, p.Sq, c.x, QT * BM, 1, &first);
+        const int64_t q0 = vkc_packed_clamp(p.cu_q[b], p.Sq), sq = vkc_packed_clamp(p.cu_q[b + 1], p.Sq) - q0;
+        const int64_t k0 = vkc_packed_clamp(p.cu_k[b], p.Skv), sk = vkc_packed_clamp(p.cu_k[b + 1], p.Skv) - k0;
+        // (a sequence of n rows has at most as many units as lie between its first and the next sequence's; the rest are empty)
+        const int64_t groups = (sq + QT * BM - 1) / (QT * BM), qg = c.x - first;
+        w.valid              = qg >= 0 && qg < groups;
+        if (!w.valid) return w;
+        w.b = 0, w.h = c.y, w.qg = (int) (p.causal ? groups - 1 - qg : qg); // heavy (late) query tiles first when causal
+        w.j0 = 0, w.slot = -1, w.adv = 1, w.last = true;
+        w.m0  = (int64_t) w.qg * (QT * BM);
+        w.len = sk < 0 ? 0 : sk;
+        w.q0 = (int) q0, w.k0 = (int) k0, w.sq = (int) sq;
+        w.n_max = 0;
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            const int n = tile_steps(sq, w.len, p.causal, w.m0 + (int64_t) t * BM, w.len);
+            w.n_t[t]    = n;
+            w.n_max     = n > w.n_max ? n : w.n_max;
+        }
+        return w;
+    }
+#endif
 
     template <int D, int KS, int VS, int QT> struct Smem {
         static constexpr uint32_t Q_BYTES  = BM * D * 2; // per query tile
@@ -290,7 +325,7 @@ namespace {
         return d;
     }
 
-    template <typename T, int D, int kMode, int QT>
+    template <typename T, int D, int kMode, int QT, bool kPacked>
     __global__ void __launch_bounds__(threads_for(QT), QT == 1 ? 2 : 1)
         attn_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                             AttnParams p) {
@@ -340,10 +375,15 @@ namespace {
             ptx::tmem_alloc(base + L::oCtl, kTmemCols);
             ptx::tmem_relinquish();
         }
-        const Work<QT> w_first = work_at<QT>(p, 0, cta); // the first item, looked up while the barriers are being set up
+        auto look_up = [&](int pos) {
+            if constexpr (kPacked) return packed_work<QT>(p, pos, cta);
+            else return work_at<QT>(p, pos, cta);
+        };
+        if constexpr (kPacked) vkc_grid_dep_wait(); // the offsets may be the previous kernel's
+        const Work<QT> w_first = look_up(0); // the first item, looked up while the barriers are being set up
         // the item after `cur` (which began at step `pos` minus its length); none behind the CTA's last
         auto next_work = [&](const Work<QT> &cur, int pos) {
-            if (!cur.last) return work_at<QT>(p, pos, cta);
+            if (!cur.last) return look_up(pos);
             Work<QT> none;
             none.valid = false;
             return none;
@@ -352,7 +392,7 @@ namespace {
         __syncthreads();
         ptx::tc_fence_after();
         const uint32_t tmem = (uint32_t) ctl[0];
-        vkc_grid_dep_wait(); // set-up above overlaps the previous kernel's tail; global memory from here on
+        if constexpr (!kPacked) vkc_grid_dep_wait(); // set-up above overlaps the previous kernel's tail; global memory from here on
         vkc_grid_dep_launch();
 
         if (warp >= kWarpTma) {
@@ -372,13 +412,14 @@ namespace {
                     if (!w.valid) break;
                     pos += w.adv;
                     const int hk = w.h / hq_per_kv;
+                    const int q0 = kPacked ? w.q0 : 0, k0 = kPacked ? w.k0 : 0; // the sequence's first rows
                     for (int j = 0; j < w.n_max; ++j, ++g) {
                         const int      st = g & 1;
                         const uint32_t ph = (uint32_t) ((g >> 1) & 1);
                         if (!(ok = ptx::mbar_wait(bar(bKE + st), ph ^ 1, ctl + 1, p.dev_err))) break;
                         ptx::mbar_expect_tx(bar(bKF + st), L::KV_BYTES);
 #pragma unroll
-                        for (int c = 0; c < DCH; ++c) ptx::tma_load_4d(sK + st * L::KV_BYTES + c * (BN * 128), &tmK, c * 64, (w.j0 + j) * BN, hk, w.b, bar(bKF + st));
+                        for (int c = 0; c < DCH; ++c) ptx::tma_load_4d(sK + st * L::KV_BYTES + c * (BN * 128), &tmK, c * 64, k0 + (w.j0 + j) * BN, hk, w.b, bar(bKF + st));
                         if (j == 0) {
                             if (cq > 0) {
                                 const uint32_t pq = (uint32_t) ((cq - 1) & 1);
@@ -389,13 +430,13 @@ namespace {
                             for (int t = 0; t < kQTiles; ++t)
 #pragma unroll
                                 for (int c = 0; c < DCH; ++c)
-                                    ptx::tma_load_4d(sQ + t * L::Q_BYTES + c * (BM * 128), &tmQ, c * 64, (int) (w.m0 + t * BM), w.h, w.b, bar(bQ));
+                                    ptx::tma_load_4d(sQ + t * L::Q_BYTES + c * (BM * 128), &tmQ, c * 64, q0 + (int) (w.m0 + t * BM), w.h, w.b, bar(bQ));
                             ++cq;
                         }
                         if (!(ok = ptx::mbar_wait(bar(bVE + st), ph ^ 1, ctl + 1, p.dev_err))) break;
                         ptx::mbar_expect_tx(bar(bVF + st), L::KV_BYTES);
 #pragma unroll
-                        for (int c = 0; c < DCH; ++c) ptx::tma_load_4d(sV + st * L::KV_BYTES + c * (BN * 128), &tmV, c * 64, (w.j0 + j) * BN, hk, w.b, bar(bVF + st));
+                        for (int c = 0; c < DCH; ++c) ptx::tma_load_4d(sV + st * L::KV_BYTES + c * (BN * 128), &tmV, c * 64, k0 + (w.j0 + j) * BN, hk, w.b, bar(bVF + st));
                     }
                 }
             }
@@ -422,13 +463,28 @@ namespace {
                     }
                     if (leader) ptx::tc_commit(bar(bSF + t));
                 };
+                int  ksteps   = 8; // 16-key steps of the current key tile that hold keys of the sequence
                 auto issue_pv = [&](int t, int j, int g, int part) { // j: key tile within the item (0 starts a new O_t)
                     // V tile: D/64 spans of [128 keys x 128 B]; 16 keys per MMA step = 2048 B; `part` selects BN / kPParts keys
                     const uint64_t bv = (g & 1) ? dV1 : dV0;
                     const uint32_t d = tmem + kColO + t * D, a = tmem + kColS + t * BN;
 #pragma unroll
                     for (int k = part * (8 / kPParts); k < (part + 1) * (8 / kPParts); ++k)
-                        if (leader) ptx::mma_f16_ts(d, a + k * 8, bv + (uint64_t) (k * 128), kIdescPV, (j | k) != 0 ? 1u : 0u);
+                        if (leader && (!kPacked || k < ksteps)) ptx::mma_f16_ts(d, a + k * 8, bv + (uint64_t) (k * 128), kIdescPV, (j | k) != 0 ? 1u : 0u);
+                };
+                // Packed: behind the sequence's last key its V tile holds the next sequence's rows, whose values may be infinite or
+                // NaN, which a probability of 0 would not silence. Steps without a key are left out; the rest of the last step's rows
+                // (fewer than 16) is set to zero.
+                auto clear_tail = [&](const Work<QT> &w, int j, int g) {
+                    const int nv = (int) (w.len - (int64_t) j * BN);
+                    ksteps       = nv >= BN ? 8 : (nv + 15) / 16;
+                    if (nv >= BN || nv % 16 == 0) return;
+                    const uint32_t v = sV + (uint32_t) (g & 1) * L::KV_BYTES;
+                    const int      rows = ksteps * 16 - nv;
+                    for (int i = threadIdx.x & 31; i < rows * DCH * 8; i += 32)
+                        ptx::st_shared_v4(v + (uint32_t) (i / (rows * 8)) * (BN * 128) + (uint32_t) (nv * 128 + i % (rows * 8) * 16), 0u, 0u, 0u, 0u);
+                    ptx::fence_proxy_async();
+                    __syncwarp();
                 };
                 int  cq = 0;      // items with work so far (phase of the Q barriers)
                 int  cs[kQTiles]; // key tiles each query tile has been through (phase of its S and P barriers)
@@ -457,6 +513,9 @@ namespace {
                     for (int j = 0; j < n_max && ok; ++j) {
                         const int g = g0 + j, vs = g & 1;
                         ok = wait(bVF + vs, (uint32_t) ((g >> 1) & 1));
+                        if constexpr (kPacked) {
+                            if (ok) clear_tail(w, j, g);
+                        }
                         const bool more = j + 1 < n_max;
 #pragma unroll
                         for (int t = 0; t < kQTiles && ok; ++t) {
@@ -514,14 +573,16 @@ namespace {
             // occupy registers next to a whole row of scores; the epilogue looks the item up again.
             int  n = 0, kbase = 0, jm = 0, lim_row = 0;
             int  iadv = 0, ib = 0, ih = 0, imisc = 0; // the item's length along the line and what the epilogue needs: batch, head, and group | (slot + 1) << 26 | last << 28 | (n_max > 0) << 29
+            int  isq = 0; // packed: the sequence's query length (and ib its first row)
             bool have = false;
             auto prepare = [&](const Work<QT> &w) {
                 have = w.valid;
                 if (!have) return;
-                iadv = w.adv, ib = w.b, ih = w.h, imisc = w.qg | ((w.slot + 1) << 26) | (w.last ? 1 << 28 : 0) | (w.n_max > 0 ? 1 << 29 : 0);
+                if constexpr (kPacked) isq = w.sq;
+                iadv = w.adv, ib = kPacked ? w.q0 : w.b, ih = w.h, imisc = w.qg | ((w.slot + 1) << 26) | (w.last ? 1 << 28 : 0) | (w.n_max > 0 ? 1 << 29 : 0);
                 n     = t ? w.n_t[QT - 1] : w.n_t[0]; // (a run-time index would put the whole description into local memory)
                 kbase = w.j0 * BN; // first key of the item
-                const int64_t first = w.m0 + (int64_t) t * BM, off = p.Skv - p.Sq;
+                const int64_t first = w.m0 + (int64_t) t * BM, off = kPacked ? w.len - w.sq : p.Skv - p.Sq;
                 // keys < lim_row are visible to this thread's row
                 int64_t lim = w.len;
                 if (p.causal && first + r + off + 1 < lim) lim = first + r + off + 1;
@@ -541,6 +602,8 @@ namespace {
             // straddle kv_len or the causal diagonal take it, every other tile runs free of any mask arithmetic).
             auto tile = [&](auto mask_tag, int j) -> bool {
                 constexpr bool kMask = decltype(mask_tag)::value;
+                // packed: hidden keys get exactly 0 (the polynomial would make it 2^-125, which a huge V could lift)
+                constexpr int kExp = kPacked && kMask ? 1 : kMode;
                 ok = ptx::mbar_wait(bar(bSF + t), (uint32_t) (cs & 1), ctl + 1, p.dev_err);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) return false;
@@ -599,7 +662,9 @@ namespace {
                         ptx::tmem_st_x32(tO + c * 32, v);
                     }
                 }
-                const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
+                // packed, f16: P times 2^7, so that probabilities down to 2^-21 of the largest keep all bits of f16
+                constexpr float kLift = kPacked && !kBf16 ? 7.f : 0.f;
+                const float neg_m = m_used == -INFINITY ? 0.f : kLift - m_used;
                 const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), nm2 = make_float2(neg_m, neg_m);
                 float2       ls  = make_float2(0.f, 0.f);
                 // P for column group `part` of this row is in TMEM: one arrival per warp on that group's barrier
@@ -609,7 +674,7 @@ namespace {
                     __syncwarp();
                     if (lane == 0) ptx::mbar_arrive(bar(bPF + kPParts * t + part));
                 };
-                if (kMode == 0) {
+                if (kExp == 0) {
 #pragma unroll
                     for (int c = 0; c < 4; c += 2) {
                         uint32_t pk[32];
@@ -664,25 +729,25 @@ namespace {
                         const int m0 = 4 * i, m1 = m0 + 1, m2 = m0 + 2, q = m0 + 3;
                         v_ex2(X(m0));
                         S0(m0 + 4);
-                        if (kMode == 2) v_max(X(q), -125.0f), v_max(Y(q), -125.0f);
+                        if (kExp == 2) v_max(X(q), -125.0f), v_max(Y(q), -125.0f);
                         v_ex2(Y(m0));
-                        if (kMode == 2) {
+                        if (kExp == 2) {
                             v_fadd2to(tx, ty, X(q), Y(q), kMagic);
                             v_fadd2to(nx, ny, tx, ty, kNegMagic);
                         }
                         S2(m0 - 4);
                         v_ex2(X(m1));
                         S0(m1 + 4);
-                        if (kMode == 2) {
+                        if (kExp == 2) {
                             v_ffma2(nx, ny, nx, ny, kNegOne, make_float2(__uint_as_float(X(q)), __uint_as_float(Y(q)))); // f = x - n
                             v_ffma2to(px, py, kC3, nx, ny, kC2);
                         }
                         v_ex2(Y(m1));
-                        if (kMode == 2) v_ffma2acc(px, py, nx, ny, kC1);
+                        if (kExp == 2) v_ffma2acc(px, py, nx, ny, kC1);
                         S2(m1 - 4);
                         v_ex2(X(m2));
                         S0(m2 + 4);
-                        if (kMode == 2) {
+                        if (kExp == 2) {
                             v_ffma2acc(px, py, nx, ny, kC0);
                             v_expo(X(q), px, tx);
                         } else {
@@ -690,7 +755,7 @@ namespace {
                         }
                         v_ex2(Y(m2));
                         S0(q + 4);
-                        if (kMode == 2) {
+                        if (kExp == 2) {
                             v_expo(Y(q), py, ty);
                         } else {
                             v_ex2(Y(q));
@@ -711,7 +776,8 @@ namespace {
             struct { int slot; bool last; int n_max; } w; // (n_max: only whether the item had work)
             w.slot = ((imisc >> 26) & 3) - 1, w.last = (imisc >> 28) & 1, w.n_max = (imisc >> 29) & 1;
             pos += iadv;
-            const int      b = ib, h = ih;
+            const int      b = kPacked ? 0 : ib, h = ih;
+            const int64_t  Sq = kPacked ? (int64_t) isq : p.Sq, rows0 = kPacked ? (int64_t) ib * p.os[2] : 0; // the sequence's rows of O
             const int64_t  m0 = (int64_t) (imisc & ((1 << 26) - 1)) * (QT * BM), row = m0 + (int64_t) t * BM + r;
             const int      ndest  = w.slot >= 0 ? 0 : p.fan.n_dest; // fan-out of final rows only (the launcher checked alignment)
             // epilogue of the item
@@ -725,7 +791,7 @@ namespace {
                 ptx::tc_fence_after();
                 // a row with no visible key stores NaN like the reference's 0/0
                 float       inv    = (n > 0 && m_used == -INFINITY) ? __int_as_float(0x7fc00000) : 1.0f / l;
-                const int64_t ooff  = (int64_t) b * p.os[0] + (int64_t) h * p.os[1] + row * p.os[2];
+                const int64_t ooff  = (int64_t) b * p.os[0] + (int64_t) h * p.os[1] + row * p.os[2] + rows0;
                 T          *orow   = (T *) p.O + ooff;
                 bool        vec_ok = (p.os[0] % 8 == 0) && (p.os[1] % 8 == 0) && (p.os[2] % 8 == 0) && (((uintptr_t) p.O & 15) == 0);
                 const bool  partial = w.slot >= 0;
@@ -752,7 +818,7 @@ namespace {
                     const uint32_t sStage = base + L::oStage + (uint32_t) (t * 4 + q) * 4096;
                     // partial rows are dense [.., QT * BM, D]; final rows follow the caller's output strides
                     const int64_t row_stride = partial ? (int64_t) D : p.os[2];
-                    const int64_t base_off   = partial ? (prow0 - (m0 + (int64_t) t * BM)) * D : (int64_t) b * p.os[0] + (int64_t) h * p.os[1];
+                    const int64_t base_off   = partial ? (prow0 - (m0 + (int64_t) t * BM)) * D : (int64_t) b * p.os[0] + (int64_t) h * p.os[1] + rows0;
                     T *const      obase      = partial ? (T *) p.part_o : (T *) p.O;
 #pragma unroll 1
                     for (int c = 0; c < D / 64; ++c) {
@@ -779,7 +845,7 @@ namespace {
                             const int     rr   = i * 4 + (lane >> 3), ch = lane & 7;
                             const int64_t grow = m0 + (int64_t) t * BM + q * 32 + rr;
                             const uint4   o4   = ptx::ld_shared_v4(sStage + (uint32_t) rr * 128 + (uint32_t) ((ch ^ (rr & 7)) << 4));
-                            if (grow < p.Sq) {
+                            if (grow < Sq) {
                                 const int64_t off = base_off + grow * row_stride + c * 64 + ch * 8;
                                 if (ndest == 0) *reinterpret_cast<uint4 *>(obase + off) = o4;
                                 else vkc_fanout_store16<T>(p.fan, off, o4);
@@ -798,7 +864,7 @@ namespace {
 #pragma unroll
                             for (int i = 0; i < 32; ++i) v[i] = 0u;
                         }
-                        if (row < p.Sq) {
+                        if (row < Sq) {
 #pragma unroll
                             for (int i = 0; i < 32; ++i) St<T>::st(orow + c * 32 + i, __uint_as_float(v[i]) * inv);
                         }
@@ -809,7 +875,7 @@ namespace {
                 ptx::tc_fence_before();
             }
             if (w.last) break;
-            prepare(work_at<QT>(p, pos, cta));
+            prepare(look_up(pos));
           }
         }
         if (ctl[1]) {
@@ -988,7 +1054,7 @@ namespace {
     template <typename T, int D, int QT>
     int launch_attn_qt(vkc_ctx *ctx, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, AttnParams &p, int64_t B, Distribution d,
                        cudaStream_t st) {
-        auto          kern = attn_prefill_kernel<T, D, 2, QT>;
+        auto          kern = attn_prefill_kernel<T, D, 2, QT, false>;
         constexpr int smem = (int) Smem<D, 2, 2, QT>::total;
         static_assert(smem * (QT == 1 && D == 64 ? 2 : 1) <= 227 * 1024, "shared memory budget");
         if (int rc = vkc_configure_smem(ctx, kern, smem)) return rc;
@@ -1019,6 +1085,24 @@ namespace {
         const Distribution d = distribute(p, B, D, ctx->sm_count);
         if (D == 64 && d.qt == 1) return launch_attn_qt<T, 64, 1>(ctx, tq, tk, tv, p, B, d, st);
         return launch_attn_qt<T, D, 2>(ctx, tq, tk, tv, p, B, d, st);
+    }
+
+    template <typename T, int D, int QT>
+    int launch_packed_qt(vkc_ctx *ctx, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, AttnParams &p, cudaStream_t st) {
+        auto          kern = attn_prefill_kernel<T, D, 2, QT, true>;
+        constexpr int smem = (int) Smem<D, 2, 2, QT>::total;
+        if (int rc = vkc_configure_smem(ctx, kern, smem)) return rc;
+        const dim3 grid((unsigned) (p.Sq / (QT * BM) + p.nseq), (unsigned) p.Hq, 1);
+        vkc_launch(ctx, kern, grid, dim3(threads_for(QT)), smem, st, tq, tk, tv, p);
+        return vkc_post_launch(ctx, "attn_prefill_packed_tcgen05");
+    }
+    template <typename T, int D>
+    int launch_packed(vkc_ctx *ctx, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, AttnParams &p, cudaStream_t st) {
+        // the same choice as for one sequence length (distribute)
+        const bool one_tile = D == 64 && (p.Sq / (2 * BM) + p.nseq) * p.Hq < 6 * ctx->sm_count;
+        if constexpr (D == 64)
+            if (one_tile) return launch_packed_qt<T, 64, 1>(ctx, tq, tk, tv, p, st);
+        return launch_packed_qt<T, D, 2>(ctx, tq, tk, tv, p, st);
     }
 
     int make_qkv_map(vkc_ctx *ctx, CUtensorMap *map, int dtype, const void *base, int64_t B, int64_t H, int64_t S, int64_t D, const int64_t *str) {
@@ -1070,6 +1154,36 @@ int vkc_attn_prefill_tcgen05(vkc_ctx *ctx, const void *Q, const void *K, const v
     p.part_ml    = nullptr;
     if (dtype == VKC_F16) return D == 64 ? launch_attn<__half, 64>(ctx, tq, tk, tv, p, B, st) : launch_attn<__half, 128>(ctx, tq, tk, tv, p, B, st);
     return D == 64 ? launch_attn<__nv_bfloat16, 64>(ctx, tq, tk, tv, p, B, st) : launch_attn<__nv_bfloat16, 128>(ctx, tq, tk, tv, p, B, st);
+}
+
+// Packed sequences; strides {unused, head, token}. VKC_ERR_UNSUPPORTED: the SIMT kernel's case.
+int vkc_attn_prefill_packed_tcgen05(vkc_ctx *ctx, const void *Q, const void *K, const void *V, void *O, int64_t nseq, int64_t Hq, int64_t Hkv,
+                                    int64_t total_q, int64_t total_k, int64_t D, const int64_t *qs, const int64_t *ks, const int64_t *vs,
+                                    const int64_t *os, float scale, int causal, const int32_t *cu_q, const int32_t *cu_k, int dtype, cudaStream_t st) {
+    if (dtype != VKC_F16 && dtype != VKC_BF16) return vkc_fail(ctx, VKC_ERR_UNSUPPORTED, "attn_prefill_packed: the tensor-core kernel takes 16-bit storage only");
+    if (D != 64 && D != 128) return vkc_fail(ctx, VKC_ERR_UNSUPPORTED, "attn_prefill_packed: the tensor-core kernel takes head dims 64 and 128");
+    if (!(scale > 0.f)) return vkc_fail(ctx, VKC_ERR_UNSUPPORTED, "attn_prefill_packed: the tensor-core kernel takes a positive scale");
+    for (int i = 1; i < 3; ++i)
+        if ((qs[i] % 8) || (ks[i] % 8) || (vs[i] % 8) || qs[i] <= 0 || ks[i] <= 0 || vs[i] <= 0)
+            return vkc_fail(ctx, VKC_ERR_UNSUPPORTED, "attn_prefill_packed: the tensor-core kernel takes Q/K/V strides that are positive multiples of 16 bytes");
+    if (((uintptr_t) Q | (uintptr_t) K | (uintptr_t) V) & 15) return vkc_fail(ctx, VKC_ERR_UNSUPPORTED, "attn_prefill_packed: the tensor-core kernel takes 16-byte aligned Q/K/V");
+    if (total_k == 0) return vkc_fail(ctx, VKC_ERR_UNSUPPORTED, "attn_prefill_packed: no keys");
+    CUtensorMap   tq, tk, tv;
+    int           rc;
+    const int64_t q3[3] = {0, qs[1], qs[2]}, k3[3] = {0, ks[1], ks[2]}, v3[3] = {0, vs[1], vs[2]};
+    if ((rc = make_qkv_map(ctx, &tq, dtype, Q, 1, Hq, total_q, D, q3))) return rc;
+    if ((rc = make_qkv_map(ctx, &tk, dtype, K, 1, Hkv, total_k, D, k3))) return rc;
+    if ((rc = make_qkv_map(ctx, &tv, dtype, V, 1, Hkv, total_k, D, v3))) return rc;
+    AttnParams p = {};
+    p.O          = O;
+    p.os[1] = os[1], p.os[2] = os[2];
+    p.Sq = total_q, p.Skv = total_k, p.Hq = Hq, p.Hkv = Hkv;
+    p.scale_log2 = scale * 1.4426950408889634f;
+    p.causal     = causal;
+    p.dev_err    = ctx->dev_err;
+    p.cu_q = cu_q, p.cu_k = cu_k, p.nseq = nseq;
+    if (dtype == VKC_F16) return D == 64 ? launch_packed<__half, 64>(ctx, tq, tk, tv, p, st) : launch_packed<__half, 128>(ctx, tq, tk, tv, p, st);
+    return D == 64 ? launch_packed<__nv_bfloat16, 64>(ctx, tq, tk, tv, p, st) : launch_packed<__nv_bfloat16, 128>(ctx, tq, tk, tv, p, st);
 }
 
 // ---- introspection of the work distribution (host arithmetic only: no device, no context) -------------------------------

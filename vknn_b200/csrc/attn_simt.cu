@@ -9,6 +9,10 @@ int vkc_attn_prefill_tcgen05(vkc_ctx *ctx, const void *Q, const void *K, const v
                              int64_t Skv, int64_t D, const int64_t *qs, const int64_t *ks, const int64_t *vs, const int64_t *os, float scale,
                              int causal, const int32_t *kv_len, int dtype, const vkc_fanout *fan, cudaStream_t st);
 
+int vkc_attn_prefill_packed_tcgen05(vkc_ctx *ctx, const void *Q, const void *K, const void *V, void *O, int64_t nseq, int64_t Hq, int64_t Hkv,
+                                    int64_t total_q, int64_t total_k, int64_t D, const int64_t *qs, const int64_t *ks, const int64_t *vs,
+                                    const int64_t *os, float scale, int causal, const int32_t *cu_q, const int32_t *cu_k, int dtype, cudaStream_t st);
+
 namespace {
 
     constexpr int kRows = 8;  // query rows (= warps) per CTA
@@ -234,7 +238,10 @@ extern "C" int vkc_attn_prefill_packed(vkc_ctx *ctx, const void *Q, const void *
     set(p.qs, q_strides, dq), set(p.ks, k_strides, dk), set(p.vs, v_strides, dk), set(p.os, o_strides, dq);
     p.scale = scale, p.causal = causal ? 1 : 0, p.mask = nullptr, p.kv_len = nullptr;
     p.cu_q = cu_q, p.cu_k = cu_k ? cu_k : cu_q;
-    if (ctx->impl == VKC_IMPL_TCGEN05) return vkc_fail(ctx, VKC_ERR_UNSUPPORTED, "attn_prefill_packed: no tensor-core kernel");
+    if (ctx->impl != VKC_IMPL_SIMT) {
+        const int rc = vkc_attn_prefill_packed_tcgen05(ctx, Q, K, V, O, nseq, Hq, Hkv, total_q, total_k, D, p.qs, p.ks, p.vs, p.os, scale, p.causal, p.cu_q, p.cu_k, dtype, st);
+        if (rc != VKC_ERR_UNSUPPORTED || ctx->impl == VKC_IMPL_TCGEN05) return rc;
+    }
     switch (dtype) {
         case VKC_F32: return launch_attn_simt<float>(ctx, Q, K, V, O, p, st);
         case VKC_F16: return launch_attn_simt<__half>(ctx, Q, K, V, O, p, st);
