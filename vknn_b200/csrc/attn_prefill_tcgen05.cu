@@ -91,6 +91,16 @@ namespace {
         // Skv above are the totals, O's rows follow os[2] from the first row of the first sequence.
         const int32_t *cu_q, *cu_k;
         int64_t        nseq;
+        int            ranked; // units to rank (at most kRanked), or 0: one CTA per unit
+    };
+    // Packed sequences, more units than SMs: persistent CTAs take them longest first. Every CTA ranks the units by itself (their
+    // number is small, the lengths are on the device only, and a list in global memory would need a kernel of its own and memory
+    // that outlives it); round r of CTA c is the unit and head number r * CTAs + c, and c counted from the other end in odd
+    // rounds, which evens out the lengths.
+    constexpr int kRanked = 512;
+    constexpr int kCached = 24; // rounds whose units are looked up in advance
+    struct PackedUnit {
+        int q0, k0, sq, sk, qg;
     };
 
     // Key tiles the 128-row query tile that starts at row `first` needs when `len` keys are visible to the sequence.
@@ -126,7 +136,9 @@ namespace {
         int     adv;      // how far the item moves the CTA along the line
         int64_t m0, len;  // first query row of the unit, visible key length
         int     n_t[QT], n_max;
-        int     q0, k0, sq; // packed: first query and key row of the sequence, its query length (m0 and len count within it)
+    };
+    template <int QT> struct PackedWork : Work<QT> {
+        int q0, k0, sq; // first query and key row of the sequence, its query length (m0 and len count within it)
     };
     // Which CTA of which grid (the kernel passes blockIdx / gridDim.x; the host walks the same arithmetic for its plan report).
     struct CtaId {
@@ -212,32 +224,82 @@ namespace {
     }
 
 #ifdef __CUDACC__
-    // The same for packed sequences: CTA c.x of head c.y is one unit.
-    template <int QT> __device__ __forceinline__ Work<QT> packed_work(const AttnParams &p, int pos, const CtaId c) {
-        Work<QT> w;
-        w.valid = pos < 1;
-        if (!w.valid) return w;
+    // Unit `u` of the packed sequences (vkc_packed_find's numbers); sq < 0: there is none with this number.
+    template <int QT> __device__ __forceinline__ PackedUnit packed_unit(const AttnParams &p, const int32_t *cu_q, const int32_t *cu_k, int u) {
+        PackedUnit    x;
         int64_t       first;
-        const int64_t b = vkc_packed_find(p.cu_q, p.nseq, p.Sq, c.x, QT * BM, 1, &first);
-        const int64_t q0 = vkc_packed_clamp(p.cu_q[b], p.Sq), sq = vkc_packed_clamp(p.cu_q[b + 1], p.Sq) - q0;
-        const int64_t k0 = vkc_packed_clamp(p.cu_k[b], p.Skv), sk = vkc_packed_clamp(p.cu_k[b + 1], p.Skv) - k0;
+        const int64_t b = vkc_packed_find(cu_q, p.nseq, p.Sq, u, QT * BM, 1, &first);
+        x.q0 = (int) vkc_packed_clamp(cu_q[b], p.Sq), x.sq = (int) vkc_packed_clamp(cu_q[b + 1], p.Sq) - x.q0;
+        x.k0 = (int) vkc_packed_clamp(cu_k[b], p.Skv), x.sk = (int) vkc_packed_clamp(cu_k[b + 1], p.Skv) - x.k0;
+        if (x.sk < 0) x.sk = 0;
         // (a sequence of n rows has at most as many units as lie between its first and the next sequence's; the rest are empty)
-        const int64_t groups = (sq + QT * BM - 1) / (QT * BM), qg = c.x - first;
-        w.valid              = qg >= 0 && qg < groups;
-        if (!w.valid) return w;
-        w.b = 0, w.h = c.y, w.qg = (int) (p.causal ? groups - 1 - qg : qg); // heavy (late) query tiles first when causal
-        w.j0 = 0, w.slot = -1, w.adv = 1, w.last = true;
-        w.m0  = (int64_t) w.qg * (QT * BM);
-        w.len = sk < 0 ? 0 : sk;
-        w.q0 = (int) q0, w.k0 = (int) k0, w.sq = (int) sq;
+        const int groups = (x.sq + QT * BM - 1) / (QT * BM), qg = u - (int) first;
+        x.qg             = p.causal ? groups - 1 - qg : qg; // heavy (late) query tiles first when causal
+        if (qg < 0 || qg >= groups) x.sq = -1;
+        return x;
+    }
+    template <int QT> __device__ __forceinline__ void packed_tiles(PackedWork<QT> &w, int causal) {
         w.n_max = 0;
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
-            const int n = tile_steps(sq, w.len, p.causal, w.m0 + (int64_t) t * BM, w.len);
+            const int n = tile_steps(w.sq, w.len, causal, w.m0 + (int64_t) t * BM, w.len);
             w.n_t[t]    = n;
             w.n_max     = n > w.n_max ? n : w.n_max;
         }
+    }
+    template <int QT> __device__ __forceinline__ PackedWork<QT> packed_item(const AttnParams &p, const PackedUnit &x, int h, bool last) {
+        PackedWork<QT> w;
+        w.valid = x.sq >= 0;
+        if (!w.valid) return w;
+        w.b = 0, w.h = h, w.qg = x.qg;
+        w.j0 = 0, w.slot = -1, w.adv = 1, w.last = last;
+        w.m0  = (int64_t) w.qg * (QT * BM);
+        w.len = x.sk;
+        w.q0 = x.q0, w.k0 = x.k0, w.sq = x.sq;
+        packed_tiles<QT>(w, p.causal);
         return w;
+    }
+    // Number of the unit-and-head of a CTA's round.
+    __device__ __forceinline__ int packed_turn(int round, const CtaId c) { return round * c.nx + (round & 1 ? c.nx - 1 - c.x : c.x); }
+    // Ranks the units by their key tiles, longest first (ties: lower number), with the whole CTA; `tmp` is shared memory that nothing
+    // uses yet. order[i] becomes the i-th unit, cached[r] the unit of round r. Returns how many units there are.
+    template <int QT> __device__ __forceinline__ int packed_rank(const AttnParams &p, const CtaId c, int *tmp, uint16_t *order, PackedUnit *cached) {
+        int32_t *cq = tmp, *ck = cq + kRanked + 1, *key = tmp + 2 * kRanked + 4;
+        for (int i = threadIdx.x; i <= (int) p.nseq; i += blockDim.x) cq[i] = p.cu_q[i], ck[i] = p.cu_k[i];
+        __syncthreads();
+        const int pad = (p.ranked + 3) / 4 * 4;
+        int       n   = 0;
+        for (int u0 = 0; u0 < pad; u0 += blockDim.x) {
+            const int u = u0 + threadIdx.x;
+            int       k = -1;
+            if (u < p.ranked) {
+                const PackedUnit x = packed_unit<QT>(p, cq, ck, u);
+                if (x.sq >= 0) {
+                    k = 0;
+#pragma unroll
+                    for (int t = 0; t < QT; ++t) k += tile_steps(x.sq, x.sk, p.causal, (int64_t) x.qg * (QT * BM) + t * BM, x.sk);
+                }
+            }
+            if (u < pad) key[u] = k;
+            n += __syncthreads_count(k >= 0);
+        }
+        for (int u = threadIdx.x; u < p.ranked; u += blockDim.x) {
+            const int k = key[u];
+            if (k < 0) continue;
+            int rank = 0;
+            for (int v = 0; v < pad; v += 4) {
+                const int4 o = *reinterpret_cast<const int4 *>(key + v);
+                rank += (o.x > k || (o.x == k && v < u)) + (o.y > k || (o.y == k && v + 1 < u)) + (o.z > k || (o.z == k && v + 2 < u)) +
+                        (o.w > k || (o.w == k && v + 3 < u));
+            }
+            order[rank] = (uint16_t) u;
+        }
+        __syncthreads();
+        for (int r = threadIdx.x; r < kCached; r += blockDim.x) {
+            const int i = packed_turn(r, c);
+            if (i < n * (int) p.Hq) cached[r] = packed_unit<QT>(p, cq, ck, order[i / (int) p.Hq]);
+        }
+        return n; // (the caller's barrier)
     }
 #endif
 
@@ -252,7 +314,8 @@ namespace {
         // barriers: q_full, q_read, k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full[QT], p_full[QT][kPParts], o_final[QT]
         static constexpr int nBar = 2 + 2 * KS + 2 * VS + QT * (2 + kPParts);
         static constexpr uint32_t oCtl  = oBar + 8 * nBar;
-        static constexpr uint32_t total = oCtl + 16 + 1024;
+        static constexpr uint32_t oCached = oCtl + 16, oOrder = oCached + kCached * sizeof(PackedUnit); // packed sequences only
+        static constexpr uint32_t total = oCtl + 16 + 1024, total_packed = oOrder + kRanked * 2 + 1024;
     };
 
     __device__ __forceinline__ float fast_exp2(float x) {
@@ -375,16 +438,33 @@ namespace {
             ptx::tmem_alloc(base + L::oCtl, kTmemCols);
             ptx::tmem_relinquish();
         }
+        using Item = std::conditional_t<kPacked, PackedWork<QT>, Work<QT>>;
+        int units = 0; // packed, ranked: their number
+        if constexpr (kPacked) {
+            vkc_grid_dep_wait(); // the offsets may be the previous kernel's
+            if (p.ranked) {
+                units = packed_rank<QT>(p, cta, (int *) (gbase + L::oQ), (uint16_t *) (gbase + L::oOrder), (PackedUnit *) (gbase + L::oCached));
+                ptx::fence_proxy_async(); // the scratch of the ranking lies where the Q tiles will be copied to
+                __syncthreads();
+            }
+        }
         auto look_up = [&](int pos) {
-            if constexpr (kPacked) return packed_work<QT>(p, pos, cta);
-            else return work_at<QT>(p, pos, cta);
+            if constexpr (kPacked) {
+                if (!p.ranked) return packed_item<QT>(p, packed_unit<QT>(p, p.cu_q, p.cu_k, cta.x), cta.y, true);
+                const int  Hq = (int) p.Hq, i = packed_turn(pos, cta);
+                PackedUnit x;
+                x.sq = -1;
+                if (i < units * Hq) x = pos < kCached ? ((const PackedUnit *) (gbase + L::oCached))[pos] : packed_unit<QT>(p, p.cu_q, p.cu_k, ((const uint16_t *) (gbase + L::oOrder))[i / Hq]);
+                return packed_item<QT>(p, x, i % Hq, packed_turn(pos + 1, cta) >= units * Hq);
+            } else {
+                return work_at<QT>(p, pos, cta);
+            }
         };
-        if constexpr (kPacked) vkc_grid_dep_wait(); // the offsets may be the previous kernel's
-        const Work<QT> w_first = look_up(0); // the first item, looked up while the barriers are being set up
+        const Item w_first = look_up(0); // the first item, looked up while the barriers are being set up
         // the item after `cur` (which began at step `pos` minus its length); none behind the CTA's last
-        auto next_work = [&](const Work<QT> &cur, int pos) {
+        auto next_work = [&](const Item &cur, int pos) {
             if (!cur.last) return look_up(pos);
-            Work<QT> none;
+            Item none;
             none.valid = false;
             return none;
         };
@@ -407,12 +487,13 @@ namespace {
                 int  g  = 0;
                 bool ok = true;
                 const int hq_per_kv = (int) (p.Hq / p.Hkv);
-                Work<QT>  w = w_first;
+                Item  w = w_first;
                 for (int pos = 0; ok; w = next_work(w, pos)) {
                     if (!w.valid) break;
                     pos += w.adv;
                     const int hk = w.h / hq_per_kv;
-                    const int q0 = kPacked ? w.q0 : 0, k0 = kPacked ? w.k0 : 0; // the sequence's first rows
+                    int       q0 = 0, k0 = 0; // packed: the sequence's first rows
+                    if constexpr (kPacked) q0 = w.q0, k0 = w.k0;
                     for (int j = 0; j < w.n_max; ++j, ++g) {
                         const int      st = g & 1;
                         const uint32_t ph = (uint32_t) ((g >> 1) & 1);
@@ -475,7 +556,7 @@ namespace {
                 // Packed: behind the sequence's last key its V tile holds the next sequence's rows, whose values may be infinite or
                 // NaN, which a probability of 0 would not silence. Steps without a key are left out; the rest of the last step's rows
                 // (fewer than 16) is set to zero.
-                auto clear_tail = [&](const Work<QT> &w, int j, int g) {
+                auto clear_tail = [&](const Item &w, int j, int g) {
                     const int nv = (int) (w.len - (int64_t) j * BN);
                     ksteps       = nv >= BN ? 8 : (nv + 15) / 16;
                     if (nv >= BN || nv % 16 == 0) return;
@@ -492,7 +573,7 @@ namespace {
                 bool ok = true;
 #pragma unroll
                 for (int t = 0; t < kQTiles; ++t) cs[t] = 0;
-                Work<QT> w = w_first;
+                Item w = w_first;
                 for (int pos = 0; ok; w = next_work(w, pos)) {
                     if (!w.valid) break;
                     pos += w.adv;
@@ -575,14 +656,15 @@ namespace {
             int  iadv = 0, ib = 0, ih = 0, imisc = 0; // the item's length along the line and what the epilogue needs: batch, head, and group | (slot + 1) << 26 | last << 28 | (n_max > 0) << 29
             int  isq = 0; // packed: the sequence's query length (and ib its first row)
             bool have = false;
-            auto prepare = [&](const Work<QT> &w) {
+            auto prepare = [&](const Item &w) {
                 have = w.valid;
                 if (!have) return;
-                if constexpr (kPacked) isq = w.sq;
-                iadv = w.adv, ib = kPacked ? w.q0 : w.b, ih = w.h, imisc = w.qg | ((w.slot + 1) << 26) | (w.last ? 1 << 28 : 0) | (w.n_max > 0 ? 1 << 29 : 0);
+                int first_row = w.b;
+                if constexpr (kPacked) isq = w.sq, first_row = w.q0;
+                iadv = w.adv, ib = first_row, ih = w.h, imisc = w.qg | ((w.slot + 1) << 26) | (w.last ? 1 << 28 : 0) | (w.n_max > 0 ? 1 << 29 : 0);
                 n     = t ? w.n_t[QT - 1] : w.n_t[0]; // (a run-time index would put the whole description into local memory)
                 kbase = w.j0 * BN; // first key of the item
-                const int64_t first = w.m0 + (int64_t) t * BM, off = kPacked ? w.len - w.sq : p.Skv - p.Sq;
+                const int64_t first = w.m0 + (int64_t) t * BM, off = kPacked ? w.len - isq : p.Skv - p.Sq;
                 // keys < lim_row are visible to this thread's row
                 int64_t lim = w.len;
                 if (p.causal && first + r + off + 1 < lim) lim = first + r + off + 1;
@@ -777,7 +859,11 @@ namespace {
             w.slot = ((imisc >> 26) & 3) - 1, w.last = (imisc >> 28) & 1, w.n_max = (imisc >> 29) & 1;
             pos += iadv;
             const int      b = kPacked ? 0 : ib, h = ih;
-            const int64_t  Sq = kPacked ? (int64_t) isq : p.Sq, rows0 = kPacked ? (int64_t) ib * p.os[2] : 0; // the sequence's rows of O
+            const int64_t  rows0 = kPacked ? (int64_t) ib * p.os[2] : 0; // the sequence's first row of O
+            auto           in_seq = [&](int64_t r) {
+                if constexpr (kPacked) return r < isq;
+                else return r < p.Sq;
+            };
             const int64_t  m0 = (int64_t) (imisc & ((1 << 26) - 1)) * (QT * BM), row = m0 + (int64_t) t * BM + r;
             const int      ndest  = w.slot >= 0 ? 0 : p.fan.n_dest; // fan-out of final rows only (the launcher checked alignment)
             // epilogue of the item
@@ -845,7 +931,7 @@ namespace {
                             const int     rr   = i * 4 + (lane >> 3), ch = lane & 7;
                             const int64_t grow = m0 + (int64_t) t * BM + q * 32 + rr;
                             const uint4   o4   = ptx::ld_shared_v4(sStage + (uint32_t) rr * 128 + (uint32_t) ((ch ^ (rr & 7)) << 4));
-                            if (grow < Sq) {
+                            if (in_seq(grow)) {
                                 const int64_t off = base_off + grow * row_stride + c * 64 + ch * 8;
                                 if (ndest == 0) *reinterpret_cast<uint4 *>(obase + off) = o4;
                                 else vkc_fanout_store16<T>(p.fan, off, o4);
@@ -864,7 +950,7 @@ namespace {
 #pragma unroll
                             for (int i = 0; i < 32; ++i) v[i] = 0u;
                         }
-                        if (row < Sq) {
+                        if (in_seq(row)) {
 #pragma unroll
                             for (int i = 0; i < 32; ++i) St<T>::st(orow + c * 32 + i, __uint_as_float(v[i]) * inv);
                         }
@@ -1090,9 +1176,13 @@ namespace {
     template <typename T, int D, int QT>
     int launch_packed_qt(vkc_ctx *ctx, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, AttnParams &p, cudaStream_t st) {
         auto          kern = attn_prefill_kernel<T, D, 2, QT, true>;
-        constexpr int smem = (int) Smem<D, 2, 2, QT>::total;
+        constexpr int smem = (int) Smem<D, 2, 2, QT>::total_packed;
+        static_assert(smem * (QT == 1 && D == 64 ? 2 : 1) <= 227 * 1024, "shared memory budget");
         if (int rc = vkc_configure_smem(ctx, kern, smem)) return rc;
-        const dim3 grid((unsigned) (p.Sq / (QT * BM) + p.nseq), (unsigned) p.Hq, 1);
+        // unit numbers of a head (a few of them empty); persistent CTAs when they are more than fit the SMs at once
+        const int64_t units = p.Sq / (QT * BM) + p.nseq, slots = (int64_t) ctx->sm_count * (QT == 1 ? 2 : 1);
+        dim3          grid((unsigned) units, (unsigned) p.Hq, 1);
+        if (units * p.Hq > slots && units <= kRanked) p.ranked = (int) units, grid = dim3((unsigned) slots, 1, 1);
         vkc_launch(ctx, kern, grid, dim3(threads_for(QT)), smem, st, tq, tk, tv, p);
         return vkc_post_launch(ctx, "attn_prefill_packed_tcgen05");
     }
