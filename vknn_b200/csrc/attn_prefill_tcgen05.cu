@@ -92,6 +92,7 @@ namespace {
         const int32_t *cu_q, *cu_k;
         int64_t        nseq;
         int            ranked; // units to rank (at most kRanked), or 0: one CTA per unit
+        int            turns;  // query heads, or pairs of them (kPack == 2): a unit's rows come once for each
     };
     // Packed sequences, more units than SMs: persistent CTAs take them longest first. Every CTA ranks the units by itself (their
     // number is small, the lengths are on the device only, and a list in global memory would need a kernel of its own and memory
@@ -225,45 +226,42 @@ namespace {
 
 #ifdef __CUDACC__
     // Unit `u` of the packed sequences (vkc_packed_find's numbers); sq < 0: there is none with this number.
-    template <int QT> __device__ __forceinline__ PackedUnit packed_unit(const AttnParams &p, const int32_t *cu_q, const int32_t *cu_k, int u) {
+    template <int kRows> __device__ __forceinline__ PackedUnit packed_unit(const AttnParams &p, const int32_t *cu_q, const int32_t *cu_k, int u) {
         PackedUnit    x;
         int64_t       first;
-        const int64_t b = vkc_packed_find(cu_q, p.nseq, p.Sq, u, QT * BM, 1, &first);
+        const int64_t b = vkc_packed_find(cu_q, p.nseq, p.Sq, u, kRows, 1, &first);
         x.q0 = (int) vkc_packed_clamp(cu_q[b], p.Sq), x.sq = (int) vkc_packed_clamp(cu_q[b + 1], p.Sq) - x.q0;
         x.k0 = (int) vkc_packed_clamp(cu_k[b], p.Skv), x.sk = (int) vkc_packed_clamp(cu_k[b + 1], p.Skv) - x.k0;
         if (x.sk < 0) x.sk = 0;
         // (a sequence of n rows has at most as many units as lie between its first and the next sequence's; the rest are empty)
-        const int groups = (x.sq + QT * BM - 1) / (QT * BM), qg = u - (int) first;
+        const int groups = (x.sq + kRows - 1) / kRows, qg = u - (int) first;
         x.qg             = p.causal ? groups - 1 - qg : qg; // heavy (late) query tiles first when causal
         if (qg < 0 || qg >= groups) x.sq = -1;
         return x;
     }
-    template <int QT> __device__ __forceinline__ void packed_tiles(PackedWork<QT> &w, int causal) {
-        w.n_max = 0;
-#pragma unroll
-        for (int t = 0; t < QT; ++t) {
-            const int n = tile_steps(w.sq, w.len, causal, w.m0 + (int64_t) t * BM, w.len);
-            w.n_t[t]    = n;
-            w.n_max     = n > w.n_max ? n : w.n_max;
-        }
-    }
-    template <int QT> __device__ __forceinline__ PackedWork<QT> packed_item(const AttnParams &p, const PackedUnit &x, int h, bool last) {
+    template <int QT, int kRows> __device__ __forceinline__ PackedWork<QT> packed_item(const AttnParams &p, const PackedUnit &x, int h, bool last) {
         PackedWork<QT> w;
         w.valid = x.sq >= 0;
         if (!w.valid) return w;
         w.b = 0, w.h = h, w.qg = x.qg;
         w.j0 = 0, w.slot = -1, w.adv = 1, w.last = last;
-        w.m0  = (int64_t) w.qg * (QT * BM);
+        w.m0  = (int64_t) w.qg * kRows;
         w.len = x.sk;
         w.q0 = x.q0, w.k0 = x.k0, w.sq = x.sq;
-        packed_tiles<QT>(w, p.causal);
+        w.n_max = 0;
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            const int n = tile_steps(w.sq, w.len, p.causal, w.m0 + (int64_t) (t * (kRows / QT / BM)) * BM, w.len);
+            w.n_t[t]    = n;
+            w.n_max     = n > w.n_max ? n : w.n_max;
+        }
         return w;
     }
     // Number of the unit-and-head of a CTA's round.
     __device__ __forceinline__ int packed_turn(int round, const CtaId c) { return round * c.nx + (round & 1 ? c.nx - 1 - c.x : c.x); }
     // Ranks the units by their key tiles, longest first (ties: lower number), with the whole CTA; `tmp` is shared memory that nothing
     // uses yet. order[i] becomes the i-th unit, cached[r] the unit of round r. Returns how many units there are.
-    template <int QT> __device__ __forceinline__ int packed_rank(const AttnParams &p, const CtaId c, int *tmp, uint16_t *order, PackedUnit *cached) {
+    template <int QT, int kRows> __device__ __forceinline__ int packed_rank(const AttnParams &p, const CtaId c, int *tmp, uint16_t *order, PackedUnit *cached) {
         int32_t *cq = tmp, *ck = cq + kRanked + 1, *key = tmp + 2 * kRanked + 4;
         for (int i = threadIdx.x; i <= (int) p.nseq; i += blockDim.x) cq[i] = p.cu_q[i], ck[i] = p.cu_k[i];
         __syncthreads();
@@ -273,11 +271,11 @@ namespace {
             const int u = u0 + threadIdx.x;
             int       k = -1;
             if (u < p.ranked) {
-                const PackedUnit x = packed_unit<QT>(p, cq, ck, u);
+                const PackedUnit x = packed_unit<kRows>(p, cq, ck, u);
                 if (x.sq >= 0) {
                     k = 0;
 #pragma unroll
-                    for (int t = 0; t < QT; ++t) k += tile_steps(x.sq, x.sk, p.causal, (int64_t) x.qg * (QT * BM) + t * BM, x.sk);
+                    for (int t = 0; t < QT; ++t) k += tile_steps(x.sq, x.sk, p.causal, (int64_t) x.qg * kRows + t * (kRows / QT / BM) * BM, x.sk);
                 }
             }
             if (u < pad) key[u] = k;
@@ -297,7 +295,7 @@ namespace {
         __syncthreads();
         for (int r = threadIdx.x; r < kCached; r += blockDim.x) {
             const int i = packed_turn(r, c);
-            if (i < n * (int) p.Hq) cached[r] = packed_unit<QT>(p, cq, ck, order[i / (int) p.Hq]);
+            if (i < n * p.turns) cached[r] = packed_unit<kRows>(p, cq, ck, order[i / p.turns]);
         }
         return n; // (the caller's barrier)
     }
@@ -388,10 +386,15 @@ namespace {
         return d;
     }
 
-    template <typename T, int D, int kMode, int QT, bool kPacked>
+    // kPack: 0 = one sequence length for all, 1 = packed sequences, 2 = packed sequences with the same rows of two neighbouring query heads of a
+    // group as the two query tiles (instead of 256 rows of one head): they see the same keys, share the K and V tiles and end
+    // together, also at the diagonal and at a sequence's end.
+    template <typename T, int D, int kMode, int QT, int kPack>
     __global__ void __launch_bounds__(threads_for(QT), QT == 1 ? 2 : 1)
         attn_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                             AttnParams p) {
+        constexpr bool kPacked = kPack != 0, kPair = kPack == 2;
+        constexpr int  kRows   = kPair ? BM : QT * BM; // query rows of a unit
         constexpr int KS = 2, VS = 2; // the MMA issuer selects ring stages by the parity of the key tile
         static_assert(KS == 2 && VS == 2, "stage selection assumes two-stage rings");
         using L               = Smem<D, KS, VS, QT>;
@@ -443,19 +446,20 @@ namespace {
         if constexpr (kPacked) {
             vkc_grid_dep_wait(); // the offsets may be the previous kernel's
             if (p.ranked) {
-                units = packed_rank<QT>(p, cta, (int *) (gbase + L::oQ), (uint16_t *) (gbase + L::oOrder), (PackedUnit *) (gbase + L::oCached));
+                units = packed_rank<QT, kRows>(p, cta, (int *) (gbase + L::oQ), (uint16_t *) (gbase + L::oOrder), (PackedUnit *) (gbase + L::oCached));
                 ptx::fence_proxy_async(); // the scratch of the ranking lies where the Q tiles will be copied to
                 __syncthreads();
             }
         }
         auto look_up = [&](int pos) {
             if constexpr (kPacked) {
-                if (!p.ranked) return packed_item<QT>(p, packed_unit<QT>(p, p.cu_q, p.cu_k, cta.x), cta.y, true);
-                const int  Hq = (int) p.Hq, i = packed_turn(pos, cta);
+                constexpr int kHeads = kPair ? 2 : 1; // query heads of a unit
+                if (!p.ranked) return packed_item<QT, kRows>(p, packed_unit<kRows>(p, p.cu_q, p.cu_k, cta.x), cta.y * kHeads, true);
+                const int  i = packed_turn(pos, cta);
                 PackedUnit x;
                 x.sq = -1;
-                if (i < units * Hq) x = pos < kCached ? ((const PackedUnit *) (gbase + L::oCached))[pos] : packed_unit<QT>(p, p.cu_q, p.cu_k, ((const uint16_t *) (gbase + L::oOrder))[i / Hq]);
-                return packed_item<QT>(p, x, i % Hq, packed_turn(pos + 1, cta) >= units * Hq);
+                if (i < units * p.turns) x = pos < kCached ? ((const PackedUnit *) (gbase + L::oCached))[pos] : packed_unit<kRows>(p, p.cu_q, p.cu_k, ((const uint16_t *) (gbase + L::oOrder))[i / p.turns]);
+                return packed_item<QT, kRows>(p, x, i % p.turns * kHeads, packed_turn(pos + 1, cta) >= units * p.turns);
             } else {
                 return work_at<QT>(p, pos, cta);
             }
@@ -511,7 +515,7 @@ namespace {
                             for (int t = 0; t < kQTiles; ++t)
 #pragma unroll
                                 for (int c = 0; c < DCH; ++c)
-                                    ptx::tma_load_4d(sQ + t * L::Q_BYTES + c * (BM * 128), &tmQ, c * 64, q0 + (int) (w.m0 + t * BM), w.h, w.b, bar(bQ));
+                                    ptx::tma_load_4d(sQ + t * L::Q_BYTES + c * (BM * 128), &tmQ, c * 64, q0 + (int) (w.m0 + (kPair ? 0 : t * BM)), kPair ? w.h + t : w.h, w.b, bar(bQ));
                             ++cq;
                         }
                         if (!(ok = ptx::mbar_wait(bar(bVE + st), ph ^ 1, ctl + 1, p.dev_err))) break;
@@ -574,6 +578,82 @@ namespace {
 #pragma unroll
                 for (int t = 0; t < kQTiles; ++t) cs[t] = 0;
                 Item w = w_first;
+              if constexpr (kPair) {
+                // Both query tiles have the same key tiles in every item, so the items form one stream of steps: behind P.V_t of an item's last
+                // key tile comes Q.K_t of the next item's first, while the softmax warps of tile t still store the rows. The two
+                // tiles stay half a step apart across items.
+                int  pos = 0;
+                auto to_work = [&](Item &x) { // on to the next item that has keys, if there is one
+                    while (x.valid && x.n_max == 0) {
+                        x = next_work(x, pos);
+                        if (x.valid) pos += x.adv;
+                    }
+                };
+                if (w.valid) pos += w.adv;
+                to_work(w);
+                if (w.valid) {
+                    ok = wait(bKF, 0u) && wait(bQ, 0u);
+                    if (ok) {
+                        ptx::tc_fence_after();
+                        issue_qk(0, 0);
+                        issue_qk(1, 0);
+                        if (leader) {
+                            ptx::tc_commit(bar(bKE));
+                            if (w.n_max == 1) ptx::tc_commit(bar(bQE));
+                        }
+                    }
+                }
+                while (ok && w.valid) {
+                    const int n_max = w.n_max;
+                    Item      nw; // the item behind this one
+                    nw.valid = false;
+                    for (int j = 0; j < n_max && ok; ++j) {
+                        const int  g = g0 + j, vs = g & 1;
+                        const bool last = j + 1 == n_max;
+                        if (last) {
+                            nw = next_work(w, pos);
+                            if (nw.valid) pos += nw.adv;
+                            to_work(nw);
+                        }
+                        const bool more = !last || nw.valid; // another Q.K^T follows
+                        ok = wait(bVF + vs, (uint32_t) ((g >> 1) & 1));
+                        if (!ok) break;
+                        clear_tail(w, j, g);
+#pragma unroll
+                        for (int t = 0; t < 2 && ok; ++t) {
+                            const uint32_t pp = (uint32_t) (g & 1);
+#pragma unroll
+                            for (int part = 0; part < kPParts && ok; ++part) {
+                                ok = wait(bPF + kPParts * t + part, pp);
+                                if (ok) {
+                                    ptx::tc_fence_after();
+                                    issue_pv(t, j, g, part);
+                                }
+                            }
+                            if (!ok) break;
+                            if (last && leader) ptx::tc_commit(bar(bOF + t)); // O_t complete
+                            if (more) {
+                                ok = wait(bKF + ((g + 1) & 1), (uint32_t) (((g + 1) >> 1) & 1)) && (!last || wait(bQ, (uint32_t) ((cq + 1) & 1)));
+                                if (!ok) break;
+                                ptx::tc_fence_after();
+                                issue_qk(t, g + 1);
+                            }
+                        }
+                        if (!ok) break;
+                        if (leader) {
+                            ptx::tc_commit(bar(bVE + vs));
+                            if (more) {
+                                ptx::tc_commit(bar(bKE + ((g + 1) & 1)));
+                                // the last Q.K^T MMAs of their item are issued: Q may be replaced
+                                if (last ? nw.n_max == 1 : j + 2 == n_max) ptx::tc_commit(bar(bQE));
+                            }
+                        }
+                    }
+                    g0 += n_max;
+                    ++cq;
+                    w = nw;
+                }
+              } else {
                 for (int pos = 0; ok; w = next_work(w, pos)) {
                     if (!w.valid) break;
                     pos += w.adv;
@@ -638,6 +718,7 @@ namespace {
                     g0 += n_max;
                     ++cq;
                 }
+              }
             }
           }
         } else {
@@ -661,10 +742,10 @@ namespace {
                 if (!have) return;
                 int first_row = w.b;
                 if constexpr (kPacked) isq = w.sq, first_row = w.q0;
-                iadv = w.adv, ib = first_row, ih = w.h, imisc = w.qg | ((w.slot + 1) << 26) | (w.last ? 1 << 28 : 0) | (w.n_max > 0 ? 1 << 29 : 0);
+                iadv = w.adv, ib = first_row, ih = kPair ? w.h + t : w.h, imisc = w.qg | ((w.slot + 1) << 26) | (w.last ? 1 << 28 : 0) | (w.n_max > 0 ? 1 << 29 : 0);
                 n     = t ? w.n_t[QT - 1] : w.n_t[0]; // (a run-time index would put the whole description into local memory)
                 kbase = w.j0 * BN; // first key of the item
-                const int64_t first = w.m0 + (int64_t) t * BM, off = kPacked ? w.len - isq : p.Skv - p.Sq;
+                const int64_t first = w.m0 + (int64_t) (kPair ? 0 : t) * BM, off = kPacked ? w.len - isq : p.Skv - p.Sq;
                 // keys < lim_row are visible to this thread's row
                 int64_t lim = w.len;
                 if (p.causal && first + r + off + 1 < lim) lim = first + r + off + 1;
@@ -864,7 +945,7 @@ namespace {
                 if constexpr (kPacked) return r < isq;
                 else return r < p.Sq;
             };
-            const int64_t  m0 = (int64_t) (imisc & ((1 << 26) - 1)) * (QT * BM), row = m0 + (int64_t) t * BM + r;
+            const int64_t  m0 = (int64_t) (imisc & ((1 << 26) - 1)) * kRows, tm = (kPair ? 0 : t) * BM, row = m0 + tm + r; // tm: the tile's first row in the unit
             const int      ndest  = w.slot >= 0 ? 0 : p.fan.n_dest; // fan-out of final rows only (the launcher checked alignment)
             // epilogue of the item
             if (n > 0) {
@@ -929,7 +1010,7 @@ namespace {
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             const int     rr   = i * 4 + (lane >> 3), ch = lane & 7;
-                            const int64_t grow = m0 + (int64_t) t * BM + q * 32 + rr;
+                            const int64_t grow = m0 + tm + q * 32 + rr;
                             const uint4   o4   = ptx::ld_shared_v4(sStage + (uint32_t) rr * 128 + (uint32_t) ((ch ^ (rr & 7)) << 4));
                             if (in_seq(grow)) {
                                 const int64_t off = base_off + grow * row_stride + c * 64 + ch * 8;
@@ -1140,7 +1221,7 @@ namespace {
     template <typename T, int D, int QT>
     int launch_attn_qt(vkc_ctx *ctx, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, AttnParams &p, int64_t B, Distribution d,
                        cudaStream_t st) {
-        auto          kern = attn_prefill_kernel<T, D, 2, QT, false>;
+        auto          kern = attn_prefill_kernel<T, D, 2, QT, 0>;
         constexpr int smem = (int) Smem<D, 2, 2, QT>::total;
         static_assert(smem * (QT == 1 && D == 64 ? 2 : 1) <= 227 * 1024, "shared memory budget");
         if (int rc = vkc_configure_smem(ctx, kern, smem)) return rc;
@@ -1173,26 +1254,29 @@ namespace {
         return launch_attn_qt<T, D, 2>(ctx, tq, tk, tv, p, B, d, st);
     }
 
-    template <typename T, int D, int QT>
+    template <typename T, int D, int QT, bool kPair>
     int launch_packed_qt(vkc_ctx *ctx, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, AttnParams &p, cudaStream_t st) {
-        auto          kern = attn_prefill_kernel<T, D, 2, QT, true>;
-        constexpr int smem = (int) Smem<D, 2, 2, QT>::total_packed;
+        auto          kern = attn_prefill_kernel<T, D, 2, QT, kPair ? 2 : 1>;
+        constexpr int smem = (int) Smem<D, 2, 2, QT>::total_packed, rows = kPair ? BM : QT * BM;
         static_assert(smem * (QT == 1 && D == 64 ? 2 : 1) <= 227 * 1024, "shared memory budget");
         if (int rc = vkc_configure_smem(ctx, kern, smem)) return rc;
-        // unit numbers of a head (a few of them empty); persistent CTAs when they are more than fit the SMs at once
-        const int64_t units = p.Sq / (QT * BM) + p.nseq, slots = (int64_t) ctx->sm_count * (QT == 1 ? 2 : 1);
-        dim3          grid((unsigned) units, (unsigned) p.Hq, 1);
-        if (units * p.Hq > slots && units <= kRanked) p.ranked = (int) units, grid = dim3((unsigned) slots, 1, 1);
+        // unit numbers of a head or pair of heads (a few of them empty); persistent CTAs when they are more than fit the SMs at once
+        const int64_t units = p.Sq / rows + p.nseq, slots = (int64_t) ctx->sm_count * (QT == 1 ? 2 : 1);
+        p.turns             = (int) (kPair ? p.Hq / 2 : p.Hq);
+        dim3 grid((unsigned) units, (unsigned) p.turns, 1);
+        if (units * p.turns > slots && units <= kRanked) p.ranked = (int) units, grid = dim3((unsigned) slots, 1, 1);
         vkc_launch(ctx, kern, grid, dim3(threads_for(QT)), smem, st, tq, tk, tv, p);
         return vkc_post_launch(ctx, "attn_prefill_packed_tcgen05");
     }
     template <typename T, int D>
     int launch_packed(vkc_ctx *ctx, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, AttnParams &p, cudaStream_t st) {
-        // the same choice as for one sequence length (distribute)
+        // Two query heads of a group in one CTA wherever there are two. Else 256 rows of a head, or one tile of 128 by the
+        // same rule as for one sequence length (distribute).
+        if (p.Hq / p.Hkv % 2 == 0) return launch_packed_qt<T, D, 2, true>(ctx, tq, tk, tv, p, st);
         const bool one_tile = D == 64 && (p.Sq / (2 * BM) + p.nseq) * p.Hq < 6 * ctx->sm_count;
         if constexpr (D == 64)
-            if (one_tile) return launch_packed_qt<T, 64, 1>(ctx, tq, tk, tv, p, st);
-        return launch_packed_qt<T, D, 2>(ctx, tq, tk, tv, p, st);
+            if (one_tile) return launch_packed_qt<T, 64, 1, false>(ctx, tq, tk, tv, p, st);
+        return launch_packed_qt<T, D, 2, false>(ctx, tq, tk, tv, p, st);
     }
 
     int make_qkv_map(vkc_ctx *ctx, CUtensorMap *map, int dtype, const void *base, int64_t B, int64_t H, int64_t S, int64_t D, const int64_t *str) {
