@@ -101,7 +101,8 @@ namespace {
     constexpr int kRanked = 512;
     constexpr int kCached = 24; // rounds whose units are looked up in advance
     struct PackedUnit {
-        int q0, k0, sq, sk, qg;
+        int q0, k0, sq, sk, qg; // the sequence's rows and lengths, the group of rows; sq < 0: nothing to do
+        int h, last;            // first query head; whether it is the CTA's last round
     };
 
     // Key tiles the 128-row query tile that starts at row `first` needs when `len` keys are visible to the sequence.
@@ -239,12 +240,12 @@ namespace {
         if (qg < 0 || qg >= groups) x.sq = -1;
         return x;
     }
-    template <int QT, int kRows> __device__ __forceinline__ PackedWork<QT> packed_item(const AttnParams &p, const PackedUnit &x, int h, bool last) {
+    template <int QT, int kRows> __device__ __forceinline__ PackedWork<QT> packed_item(const AttnParams &p, const PackedUnit &x) {
         PackedWork<QT> w;
         w.valid = x.sq >= 0;
         if (!w.valid) return w;
-        w.b = 0, w.h = h, w.qg = x.qg;
-        w.j0 = 0, w.slot = -1, w.adv = 1, w.last = last;
+        w.b = 0, w.h = x.h, w.qg = x.qg;
+        w.j0 = 0, w.slot = -1, w.adv = 1, w.last = x.last;
         w.m0  = (int64_t) w.qg * kRows;
         w.len = x.sk;
         w.q0 = x.q0, w.k0 = x.k0, w.sq = x.sq;
@@ -257,11 +258,22 @@ namespace {
         }
         return w;
     }
-    // Number of the unit-and-head of a CTA's round.
-    __device__ __forceinline__ int packed_turn(int round, const CtaId c) { return round * c.nx + (round & 1 ? c.nx - 1 - c.x : c.x); }
+    // What CTA c does in a round, when `n` units are ranked in `order`. cu_q, cu_k: the offsets, in global or shared memory.
+    template <int kRows> __device__ __forceinline__ PackedUnit packed_round(const AttnParams &p, const CtaId c, const int32_t *cu_q, const int32_t *cu_k,
+                                                                           const uint16_t *order, int n, int heads, int round) {
+        auto       turn = [&](int r) { return r * c.nx + (r & 1 ? c.nx - 1 - c.x : c.x); };
+        const int  i = turn(round);
+        PackedUnit x;
+        x.sq = -1;
+        if (i < n * p.turns) {
+            x   = packed_unit<kRows>(p, cu_q, cu_k, order[i / p.turns]);
+            x.h = i % p.turns * heads, x.last = turn(round + 1) >= n * p.turns;
+        }
+        return x;
+    }
     // Ranks the units by their key tiles, longest first (ties: lower number), with the whole CTA; `tmp` is shared memory that nothing
     // uses yet. order[i] becomes the i-th unit, cached[r] the unit of round r. Returns how many units there are.
-    template <int QT, int kRows> __device__ __forceinline__ int packed_rank(const AttnParams &p, const CtaId c, int *tmp, uint16_t *order, PackedUnit *cached) {
+    template <int QT, int kRows> __device__ __forceinline__ int packed_rank(const AttnParams &p, const CtaId c, int heads, int *tmp, uint16_t *order, PackedUnit *cached) {
         int32_t *cq = tmp, *ck = cq + kRanked + 1, *key = tmp + 2 * kRanked + 4;
         for (int i = threadIdx.x; i <= (int) p.nseq; i += blockDim.x) cq[i] = p.cu_q[i], ck[i] = p.cu_k[i];
         __syncthreads();
@@ -293,10 +305,7 @@ namespace {
             order[rank] = (uint16_t) u;
         }
         __syncthreads();
-        for (int r = threadIdx.x; r < kCached; r += blockDim.x) {
-            const int i = packed_turn(r, c);
-            if (i < n * p.turns) cached[r] = packed_unit<kRows>(p, cq, ck, order[i / p.turns]);
-        }
+        for (int r = threadIdx.x; r < kCached; r += blockDim.x) cached[r] = packed_round<kRows>(p, c, cq, ck, order, n, heads, r);
         return n; // (the caller's barrier)
     }
 #endif
@@ -442,29 +451,27 @@ namespace {
             ptx::tmem_relinquish();
         }
         using Item = std::conditional_t<kPacked, PackedWork<QT>, Work<QT>>;
-        int units = 0; // packed, ranked: their number
+        PackedUnit *const cached = (PackedUnit *) (gbase + L::oCached);
+        uint16_t *const   order  = (uint16_t *) (gbase + L::oOrder);
+        constexpr int     kHeads = kPair ? 2 : 1; // query heads of a unit
         if constexpr (kPacked) {
             vkc_grid_dep_wait(); // the offsets may be the previous kernel's
             if (p.ranked) {
-                units = packed_rank<QT, kRows>(p, cta, (int *) (gbase + L::oQ), (uint16_t *) (gbase + L::oOrder), (PackedUnit *) (gbase + L::oCached));
+                const int n = packed_rank<QT, kRows>(p, cta, kHeads, (int *) (gbase + L::oQ), order, cached);
+                if (threadIdx.x == 0) ctl[2] = n;
                 ptx::fence_proxy_async(); // the scratch of the ranking lies where the Q tiles will be copied to
-                __syncthreads();
+            } else if (threadIdx.x == (kWarpMma + 2) * 32) {
+                PackedUnit x = packed_unit<kRows>(p, p.cu_q, p.cu_k, cta.x);
+                x.h = cta.y * kHeads, x.last = 1;
+                cached[0] = x;
             }
         }
-        auto look_up = [&](int pos) {
-            if constexpr (kPacked) {
-                constexpr int kHeads = kPair ? 2 : 1; // query heads of a unit
-                if (!p.ranked) return packed_item<QT, kRows>(p, packed_unit<kRows>(p, p.cu_q, p.cu_k, cta.x), cta.y * kHeads, true);
-                const int  i = packed_turn(pos, cta);
-                PackedUnit x;
-                x.sq = -1;
-                if (i < units * p.turns) x = pos < kCached ? ((const PackedUnit *) (gbase + L::oCached))[pos] : packed_unit<kRows>(p, p.cu_q, p.cu_k, ((const uint16_t *) (gbase + L::oOrder))[i / p.turns]);
-                return packed_item<QT, kRows>(p, x, i % p.turns * kHeads, packed_turn(pos + 1, cta) >= units * p.turns);
-            } else {
-                return work_at<QT>(p, pos, cta);
-            }
+        auto look_up = [&](int pos) { // packed: behind the set-up barrier only
+            if constexpr (kPacked) return packed_item<QT, kRows>(p, pos < kCached ? cached[pos] : packed_round<kRows>(p, cta, p.cu_q, p.cu_k, order, ctl[2], kHeads, pos));
+            else return work_at<QT>(p, pos, cta);
         };
-        const Item w_first = look_up(0); // the first item, looked up while the barriers are being set up
+        Item w_first; // the first item, looked up while the barriers are being set up
+        if constexpr (!kPacked) w_first = look_up(0);
         // the item after `cur` (which began at step `pos` minus its length); none behind the CTA's last
         auto next_work = [&](const Item &cur, int pos) {
             if (!cur.last) return look_up(pos);
@@ -492,6 +499,7 @@ namespace {
                 bool ok = true;
                 const int hq_per_kv = (int) (p.Hq / p.Hkv);
                 Item  w = w_first;
+                if constexpr (kPacked) w = look_up(0);
                 for (int pos = 0; ok; w = next_work(w, pos)) {
                     if (!w.valid) break;
                     pos += w.adv;
@@ -578,6 +586,7 @@ namespace {
 #pragma unroll
                 for (int t = 0; t < kQTiles; ++t) cs[t] = 0;
                 Item w = w_first;
+                if constexpr (kPacked) w = look_up(0);
               if constexpr (kPair) {
                 // Both query tiles have the same key tiles in every item, so the items form one stream of steps: behind P.V_t of an item's last
                 // key tile comes Q.K_t of the next item's first, while the softmax warps of tile t still store the rows. The two
@@ -735,17 +744,17 @@ namespace {
             // occupy registers next to a whole row of scores; the epilogue looks the item up again.
             int  n = 0, kbase = 0, jm = 0, lim_row = 0;
             int  iadv = 0, ib = 0, ih = 0, imisc = 0; // the item's length along the line and what the epilogue needs: batch, head, and group | (slot + 1) << 26 | last << 28 | (n_max > 0) << 29
-            int  isq = 0; // packed: the sequence's query length (and ib its first row)
             bool have = false;
             auto prepare = [&](const Item &w) {
                 have = w.valid;
                 if (!have) return;
-                int first_row = w.b;
-                if constexpr (kPacked) isq = w.sq, first_row = w.q0;
-                iadv = w.adv, ib = first_row, ih = kPair ? w.h + t : w.h, imisc = w.qg | ((w.slot + 1) << 26) | (w.last ? 1 << 28 : 0) | (w.n_max > 0 ? 1 << 29 : 0);
+                if constexpr (!kPacked) iadv = w.adv, ib = w.b, ih = w.h, imisc = w.qg | ((w.slot + 1) << 26) | (w.last ? 1 << 28 : 0) | (w.n_max > 0 ? 1 << 29 : 0);
                 n     = t ? w.n_t[QT - 1] : w.n_t[0]; // (a run-time index would put the whole description into local memory)
-                kbase = w.j0 * BN; // first key of the item
-                const int64_t first = w.m0 + (int64_t) (kPair ? 0 : t) * BM, off = kPacked ? w.len - isq : p.Skv - p.Sq;
+                if constexpr (!kPacked) kbase = w.j0 * BN; // first key of the item
+                const int64_t first = w.m0 + (int64_t) (kPair ? 0 : t) * BM;
+                int64_t       off;
+                if constexpr (kPacked) off = w.len - w.sq;
+                else off = p.Skv - p.Sq;
                 // keys < lim_row are visible to this thread's row
                 int64_t lim = w.len;
                 if (p.causal && first + r + off + 1 < lim) lim = first + r + off + 1;
@@ -758,7 +767,8 @@ namespace {
                     jm = j2 < jm ? j2 : jm;
                 }
             };
-            prepare(w_first);
+            if constexpr (kPacked) prepare(look_up(0));
+            else prepare(w_first);
           for (int pos = 0; ok && have;) {
             float          m_used = -INFINITY, l = 0.f;
             // One key tile; kMask selects the body that replaces invisible scores by -inf (only the tiles that
@@ -938,14 +948,21 @@ namespace {
             if (!ok) break;
             struct { int slot; bool last; int n_max; } w; // (n_max: only whether the item had work)
             w.slot = ((imisc >> 26) & 3) - 1, w.last = (imisc >> 28) & 1, w.n_max = (imisc >> 29) & 1;
-            pos += iadv;
-            const int      b = kPacked ? 0 : ib, h = ih;
-            const int64_t  rows0 = kPacked ? (int64_t) ib * p.os[2] : 0; // the sequence's first row of O
-            auto           in_seq = [&](int64_t r) {
+            int     b = ib, h = ih, isq = 0; // isq: packed, the sequence's query length
+            int64_t rows0 = 0, m0 = (int64_t) (imisc & ((1 << 26) - 1)) * kRows; // rows0: packed, offset of the sequence's first row of O
+            if constexpr (kPacked) { // (what a packed item needs here lies in shared memory)
+                const Item x = look_up(pos);
+                b = 0, h = kPair ? x.h + t : x.h, isq = x.sq, rows0 = (int64_t) x.q0 * p.os[2], m0 = x.m0;
+                w.slot = -1, w.last = x.last, w.n_max = x.n_max > 0;
+                ++pos;
+            } else {
+                pos += iadv;
+            }
+            auto in_seq = [&](int64_t r) {
                 if constexpr (kPacked) return r < isq;
                 else return r < p.Sq;
             };
-            const int64_t  m0 = (int64_t) (imisc & ((1 << 26) - 1)) * kRows, tm = (kPair ? 0 : t) * BM, row = m0 + tm + r; // tm: the tile's first row in the unit
+            const int64_t  tm = (kPair ? 0 : t) * BM, row = m0 + tm + r; // tm: the tile's first row in the unit
             const int      ndest  = w.slot >= 0 ? 0 : p.fan.n_dest; // fan-out of final rows only (the launcher checked alignment)
             // epilogue of the item
             if (n > 0) {
