@@ -101,8 +101,11 @@ namespace {
     constexpr int kRanked = 512;
     constexpr int kCached = 24; // rounds whose units are looked up in advance
     struct PackedUnit {
-        int q0, k0, sq, sk, qg; // the sequence's rows and lengths, the group of rows; sq < 0: nothing to do
-        int h, last;            // first query head; whether it is the CTA's last round
+        int q0, k0;   // the unit's first query row, the sequence's first key row
+        int sq, sk;   // the sequence's query rows from q0 on (0: nothing to do) and its keys
+        int lim0;     // keys that the unit's first row sees (each row behind it one more, when causal); may be negative
+        int n[2];     // key tiles of the query tiles
+        int h, last;  // first query head; whether it is the CTA's last round
     };
 
     // Key tiles the 128-row query tile that starts at row `first` needs when `len` keys are visible to the sequence.
@@ -140,7 +143,7 @@ namespace {
         int     n_t[QT], n_max;
     };
     template <int QT> struct PackedWork : Work<QT> {
-        int q0, k0, sq; // first query and key row of the sequence, its query length (m0 and len count within it)
+        int q0, k0, sq, lim0; // of PackedUnit below (m0 is 0: rows are counted from the unit's first)
     };
     // Which CTA of which grid (the kernel passes blockIdx / gridDim.x; the host walks the same arithmetic for its plan report).
     struct CtaId {
@@ -226,47 +229,48 @@ namespace {
     }
 
 #ifdef __CUDACC__
-    // Unit `u` of the packed sequences (vkc_packed_find's numbers); sq < 0: there is none with this number.
-    template <int kRows> __device__ __forceinline__ PackedUnit packed_unit(const AttnParams &p, const int32_t *cu_q, const int32_t *cu_k, int u) {
+    // Unit `u` of the packed sequences (vkc_packed_find's numbers).
+    template <int QT, int kRows> __device__ __forceinline__ PackedUnit packed_unit(const AttnParams &p, const int32_t *cu_q, const int32_t *cu_k, int u) {
         PackedUnit    x;
         int64_t       first;
-        const int64_t b = vkc_packed_find(cu_q, p.nseq, p.Sq, u, kRows, 1, &first);
-        x.q0 = (int) vkc_packed_clamp(cu_q[b], p.Sq), x.sq = (int) vkc_packed_clamp(cu_q[b + 1], p.Sq) - x.q0;
+        const int64_t b  = vkc_packed_find(cu_q, p.nseq, p.Sq, u, kRows, 1, &first);
+        const int     q0 = (int) vkc_packed_clamp(cu_q[b], p.Sq), sq = (int) vkc_packed_clamp(cu_q[b + 1], p.Sq) - q0;
         x.k0 = (int) vkc_packed_clamp(cu_k[b], p.Skv), x.sk = (int) vkc_packed_clamp(cu_k[b + 1], p.Skv) - x.k0;
         if (x.sk < 0) x.sk = 0;
         // (a sequence of n rows has at most as many units as lie between its first and the next sequence's; the rest are empty)
-        const int groups = (x.sq + kRows - 1) / kRows, qg = u - (int) first;
-        x.qg             = p.causal ? groups - 1 - qg : qg; // heavy (late) query tiles first when causal
-        if (qg < 0 || qg >= groups) x.sq = -1;
+        const int groups = (sq + kRows - 1) / kRows, qg = u - (int) first;
+        const int m0     = (p.causal ? groups - 1 - qg : qg) * kRows; // heavy (late) query tiles first when causal
+        x.q0 = q0 + m0, x.sq = qg < 0 || qg >= groups ? 0 : sq - m0;
+        x.lim0 = m0 + x.sk - sq + 1;
+        x.n[1] = 0;
+#pragma unroll
+        for (int t = 0; t < QT; ++t) x.n[t] = tile_steps(sq, x.sk, p.causal, (int64_t) m0 + t * (kRows / QT / BM) * BM, x.sk);
         return x;
     }
-    template <int QT, int kRows> __device__ __forceinline__ PackedWork<QT> packed_item(const AttnParams &p, const PackedUnit &x) {
+    template <int QT> __device__ __forceinline__ PackedWork<QT> packed_item(const PackedUnit &x) {
         PackedWork<QT> w;
-        w.valid = x.sq >= 0;
+        w.valid = x.sq > 0;
         if (!w.valid) return w;
-        w.b = 0, w.h = x.h, w.qg = x.qg;
+        w.b = 0, w.h = x.h, w.qg = 0;
         w.j0 = 0, w.slot = -1, w.adv = 1, w.last = x.last;
-        w.m0  = (int64_t) w.qg * kRows;
-        w.len = x.sk;
-        w.q0 = x.q0, w.k0 = x.k0, w.sq = x.sq;
+        w.m0 = 0, w.len = x.sk, w.q0 = x.q0, w.k0 = x.k0, w.sq = x.sq, w.lim0 = x.lim0;
         w.n_max = 0;
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
-            const int n = tile_steps(w.sq, w.len, p.causal, w.m0 + (int64_t) (t * (kRows / QT / BM)) * BM, w.len);
-            w.n_t[t]    = n;
-            w.n_max     = n > w.n_max ? n : w.n_max;
+            w.n_t[t] = x.n[t];
+            w.n_max  = x.n[t] > w.n_max ? x.n[t] : w.n_max;
         }
         return w;
     }
     // What CTA c does in a round, when `n` units are ranked in `order`. cu_q, cu_k: the offsets, in global or shared memory.
-    template <int kRows> __device__ __forceinline__ PackedUnit packed_round(const AttnParams &p, const CtaId c, const int32_t *cu_q, const int32_t *cu_k,
+    template <int QT, int kRows> __device__ __forceinline__ PackedUnit packed_round(const AttnParams &p, const CtaId c, const int32_t *cu_q, const int32_t *cu_k,
                                                                            const uint16_t *order, int n, int heads, int round) {
         auto       turn = [&](int r) { return r * c.nx + (r & 1 ? c.nx - 1 - c.x : c.x); };
         const int  i = turn(round);
         PackedUnit x;
-        x.sq = -1;
+        x.sq = 0;
         if (i < n * p.turns) {
-            x   = packed_unit<kRows>(p, cu_q, cu_k, order[i / p.turns]);
+            x   = packed_unit<QT, kRows>(p, cu_q, cu_k, order[i / p.turns]);
             x.h = i % p.turns * heads, x.last = turn(round + 1) >= n * p.turns;
         }
         return x;
@@ -283,12 +287,8 @@ namespace {
             const int u = u0 + threadIdx.x;
             int       k = -1;
             if (u < p.ranked) {
-                const PackedUnit x = packed_unit<kRows>(p, cq, ck, u);
-                if (x.sq >= 0) {
-                    k = 0;
-#pragma unroll
-                    for (int t = 0; t < QT; ++t) k += tile_steps(x.sq, x.sk, p.causal, (int64_t) x.qg * kRows + t * (kRows / QT / BM) * BM, x.sk);
-                }
+                const PackedUnit x = packed_unit<QT, kRows>(p, cq, ck, u);
+                if (x.sq > 0) k = x.n[0] + x.n[1];
             }
             if (u < pad) key[u] = k;
             n += __syncthreads_count(k >= 0);
@@ -305,7 +305,7 @@ namespace {
             order[rank] = (uint16_t) u;
         }
         __syncthreads();
-        for (int r = threadIdx.x; r < kCached; r += blockDim.x) cached[r] = packed_round<kRows>(p, c, cq, ck, order, n, heads, r);
+        for (int r = threadIdx.x; r < kCached; r += blockDim.x) cached[r] = packed_round<QT, kRows>(p, c, cq, ck, order, n, heads, r);
         return n; // (the caller's barrier)
     }
 #endif
@@ -461,13 +461,13 @@ namespace {
                 if (threadIdx.x == 0) ctl[2] = n;
                 ptx::fence_proxy_async(); // the scratch of the ranking lies where the Q tiles will be copied to
             } else if (threadIdx.x == (kWarpMma + 2) * 32) {
-                PackedUnit x = packed_unit<kRows>(p, p.cu_q, p.cu_k, cta.x);
+                PackedUnit x = packed_unit<QT, kRows>(p, p.cu_q, p.cu_k, cta.x);
                 x.h = cta.y * kHeads, x.last = 1;
                 cached[0] = x;
             }
         }
         auto look_up = [&](int pos) { // packed: behind the set-up barrier only
-            if constexpr (kPacked) return packed_item<QT, kRows>(p, pos < kCached ? cached[pos] : packed_round<kRows>(p, cta, p.cu_q, p.cu_k, order, ctl[2], kHeads, pos));
+            if constexpr (kPacked) return packed_item<QT>(pos < kCached ? cached[pos] : packed_round<QT, kRows>(p, cta, p.cu_q, p.cu_k, order, ctl[2], kHeads, pos));
             else return work_at<QT>(p, pos, cta);
         };
         Item w_first; // the first item, looked up while the barriers are being set up
@@ -748,13 +748,16 @@ namespace {
             auto prepare = [&](const Item &w) {
                 have = w.valid;
                 if (!have) return;
-                if constexpr (!kPacked) iadv = w.adv, ib = w.b, ih = w.h, imisc = w.qg | ((w.slot + 1) << 26) | (w.last ? 1 << 28 : 0) | (w.n_max > 0 ? 1 << 29 : 0);
-                n     = t ? w.n_t[QT - 1] : w.n_t[0]; // (a run-time index would put the whole description into local memory)
-                if constexpr (!kPacked) kbase = w.j0 * BN; // first key of the item
-                const int64_t first = w.m0 + (int64_t) (kPair ? 0 : t) * BM;
-                int64_t       off;
-                if constexpr (kPacked) off = w.len - w.sq;
-                else off = p.Skv - p.Sq;
+                n = t ? w.n_t[QT - 1] : w.n_t[0]; // (a run-time index would put the whole description into local memory)
+                if constexpr (kPacked) {
+                    const int len = (int) w.len, lim = w.lim0 + (kPair ? 0 : t) * BM; // keys that the tile's first row sees
+                    lim_row = !p.causal ? len : lim + r < 0 ? 0 : lim + r < len ? lim + r : len;
+                    jm      = (!p.causal ? len : lim < 0 ? 0 : lim < len ? lim : len) / BN;
+                    return;
+                }
+                iadv = w.adv, ib = w.b, ih = w.h, imisc = w.qg | ((w.slot + 1) << 26) | (w.last ? 1 << 28 : 0) | (w.n_max > 0 ? 1 << 29 : 0);
+                kbase = w.j0 * BN; // first key of the item
+                const int64_t first = w.m0 + (int64_t) t * BM, off = p.Skv - p.Sq;
                 // keys < lim_row are visible to this thread's row
                 int64_t lim = w.len;
                 if (p.causal && first + r + off + 1 < lim) lim = first + r + off + 1;
@@ -1024,6 +1027,25 @@ namespace {
                             ptx::st_shared_v4(sStage + (uint32_t) lane * 128 + (uint32_t) ((g ^ (lane & 7)) << 4), o32[0], o32[1], o32[2], o32[3]);
                         }
                         __syncwarp();
+                        if constexpr (kPacked) {
+                            // the eight lines of the warp are read before the first is stored, the addresses step from one to the next
+                            // (taken one by one, with an address each, the stores held the warps for 2000 to 3000 cycles per item)
+                            uint4 o4[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const int rr = i * 4 + (lane >> 3), ch = lane & 7;
+                                o4[i]        = ptx::ld_shared_v4(sStage + (uint32_t) rr * 128 + (uint32_t) ((ch ^ (rr & 7)) << 4));
+                            }
+                            const int from = (int) tm + q * 32 + (lane >> 3); // this lane's first row
+                            T        *at   = (T *) p.O + base_off + from * p.os[2] + c * 64 + (lane & 7) * 8;
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                if (from + 4 * i < isq) ptx::st_global_v4(at, o4[i]);
+                                at += 4 * p.os[2];
+                            }
+                            __syncwarp(); // the staging lines are rewritten by the next 64 columns
+                            continue;
+                        }
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             const int     rr   = i * 4 + (lane >> 3), ch = lane & 7;

@@ -228,6 +228,9 @@ namespace ptx {
     __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
     }
+    __device__ __forceinline__ void st_global_v4(void *at, const uint4 &v) {
+        asm volatile("st.global.v4.b32 [%0], {%1, %2, %3, %4};" ::"l"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+    }
     __device__ __forceinline__ void fence_acq_rel_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
     __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar_cluster_addr) {
         asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
