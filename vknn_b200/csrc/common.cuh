@@ -154,6 +154,31 @@ __device__ __forceinline__ int vkc_packed_find(const int32_t *cu, int64_t nseq, 
     *first = at;
     return (int) lo;
 }
+// The same by a whole warp, one load latency for up to 32 sequences and one more for every further factor of 32: also returns
+// the sequence's rows [x0, x1) and held[b] (0 if held is null).
+__device__ __forceinline__ int vkc_packed_find_warp(const int32_t *cu, const int32_t *held, int64_t nseq, int64_t total, int64_t u, int step, int extra,
+                                                    int64_t *first, int64_t *x0, int64_t *x1, int *held_b) {
+    const int lane = threadIdx.x & 31;
+    int64_t   lo = 0, hi = nseq;
+    while (hi - lo > 32) { // 32 samples of [lo, hi)
+        const int64_t stride = (hi - lo + 31) >> 5, b = lo + lane * stride;
+        const bool    le     = b < hi && (b == lo || vkc_packed_clamp(cu[b], total) / step + extra * b <= u);
+        const int     k      = 31 - __clz(__ballot_sync(0xffffffffu, le));
+        lo += k * stride;
+        hi = lo + stride < hi ? lo + stride : hi;
+    }
+    const int64_t b    = lo + lane;
+    const bool    in   = b < hi;
+    const int64_t mine = in ? vkc_packed_clamp(cu[b], total) : 0, next = in ? vkc_packed_clamp(cu[b + 1], total) : 0;
+    const int     h    = in && held ? held[b] : 0;
+    const int64_t f    = mine / step + extra * b;
+    const int     k    = 31 - __clz(__ballot_sync(0xffffffffu, in && (b == lo || f <= u)));
+    *first  = __shfl_sync(0xffffffffu, f, k);
+    *x0     = __shfl_sync(0xffffffffu, mine, k);
+    *x1     = __shfl_sync(0xffffffffu, next, k);
+    *held_b = __shfl_sync(0xffffffffu, h, k);
+    return (int) (lo + k);
+}
 #endif
 
 int vkc_ensure_scratch(vkc_ctx *ctx, size_t bytes, cudaStream_t st);

@@ -27,8 +27,6 @@ namespace {
         int            vec_ok; // bases and strides of K and V allow 16-byte loads
     };
 
-    __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-
     // Eight values as fp32, from one 16-byte vector of a 16-bit type or two of fp32.
     template <typename T> struct Row8 {
         uint4 v[sizeof(T) == 4 ? 2 : 1];
@@ -46,6 +44,23 @@ namespace {
 #pragma unroll
             for (int i = 0; i < (int) (sizeof(v) / 16); ++i) v[i] = make_uint4(0, 0, 0, 0);
         }
+        // The larger of `m` and the magnitudes, as ordered bits: for the 16-bit types two at a time, in the two halves of m.
+        __device__ __forceinline__ uint32_t top(uint32_t m) const {
+            const uint32_t *w = reinterpret_cast<const uint32_t *>(v);
+#pragma unroll
+            for (int i = 0; i < (int) (sizeof(v) / 4); ++i) {
+                if (sizeof(T) == 4) m = m > (w[i] & 0x7fffffffu) ? m : w[i] & 0x7fffffffu;
+                else m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+            }
+            return m;
+        }
+        // ... and its fp32 bits.
+        static __device__ __forceinline__ uint32_t top_bits(uint32_t m) {
+            if (sizeof(T) == 4) return m;
+            const uint32_t h = m >> 16 > (m & 0xffffu) ? m >> 16 : m & 0xffffu;
+            if (std::is_same<T, __nv_bfloat16>::value) return h << 16;
+            return __float_as_uint(__half2float(__ushort_as_half((unsigned short) h)));
+        }
         __device__ __forceinline__ float get(int i) const { return St<T>::ld(reinterpret_cast<const T *>(v) + i); }
     };
 
@@ -56,16 +71,16 @@ namespace {
         vkc_grid_dep_launch();
         // the (sequence, block) of this CTA
         int64_t b, x0, n, blk;
+        int     start = 0; // tokens the sequence holds
         if (p.cu) {
-            int64_t first;
-            b  = vkc_packed_find(p.cu, p.B, p.total, blockIdx.x, block, 2, &first);
-            x0 = vkc_packed_clamp(p.cu[b], p.total);
-            n  = vkc_packed_clamp(p.cu[b + 1], p.total) - x0;
+            int64_t first, x1;
+            b   = vkc_packed_find_warp(p.cu, p.kv_len, p.B, p.total, blockIdx.x, block, 2, &first, &x0, &x1, &start);
+            n   = x1 - x0;
             blk = blockIdx.x - first;
         } else {
             b = blockIdx.x, x0 = b, n = 1, blk = 0;
+            if (p.kv_len) start = p.kv_len[b];
         }
-        const int64_t start = p.kv_len ? (int64_t) p.kv_len[b] : 0;
         if (blk < 0 || start < 0 || start >= p.Lmax) return;
         blk += start / block;
         const int64_t lo   = blk * block;
@@ -91,12 +106,8 @@ namespace {
             else rows[i].zero();
         }
 #pragma unroll
-        for (int i = 0; i < kVec; ++i)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t a = abs_bits(rows[i].get(e));
-                top              = a > top ? a : top;
-            }
+        for (int i = 0; i < kVec; ++i) top = rows[i].top(top);
+        top = Row8<T>::top_bits(top);
         __shared__ uint32_t part[16];
         top = __reduce_max_sync(0xffffffffu, top);
         if ((tid & 31) == 0) part[tid >> 5] = top;
@@ -125,9 +136,10 @@ namespace {
         for (int i = 0; i < kVec; ++i) {
             const int v = i * nt + tid, r = v >> sh;
             if (r >= r0 && r < r1) {
-                uint2 c;
-                c.x = quant.four(rows[i].get(0), rows[i].get(1), rows[i].get(2), rows[i].get(3));
-                c.y = quant.four(rows[i].get(4), rows[i].get(5), rows[i].get(6), rows[i].get(7));
+                float f[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = rows[i].get(e);
+                const uint2 c = quant.eight(f);
                 *reinterpret_cast<uint2 *>(codes + (int64_t) v * 8) = c;
             }
         }

@@ -58,7 +58,7 @@ namespace q8 {
             exact               = (bits & 0x7fffffu) == 0 && (bits >> 23) >= 1 && (bits >> 23) <= 253;
             inv                 = kE4m3 && exact ? __uint_as_float(0x7f000000u - bits) : __fdiv_rn(1.0f, scale);
         }
-        __device__ __forceinline__ int near_middle(float x) const {
+        static __device__ __noinline__ int near_middle(float x, float s) {
             const float y = __fdiv_rn(x, s);
             float       r = rintf(y);
             if (fabsf(y - truncf(y)) == 0.5f) {
@@ -68,18 +68,33 @@ namespace q8 {
             }
             return clamp127((int) r);
         }
-        __device__ __forceinline__ int one(float x) const {
-            const float y = x * inv, r = rintf(y);
-            if (fabsf(fabsf(y - r) - 0.5f) < 3.0517578125e-5f) return near_middle(x);
-            return clamp127((int) r);
-        }
-        __device__ __forceinline__ uint32_t four(float a, float b, float c, float d) const {
-            if (none) return 0u;
+        // Eight values. int8: adding 1.5 * 2^23 leaves the nearest integer in the low bits of the sum; what the values are off
+        // their codes says whether one of them is close to the middle.
+        __device__ __forceinline__ uint2 eight(const float (&x)[8]) const {
+            if (none) return make_uint2(0u, 0u);
             if (kE4m3) {
-                if (exact) return e4m3x4(a * inv, b * inv, c * inv, d * inv);
-                return e4m3x4(__fdiv_rn(a, s), __fdiv_rn(b, s), __fdiv_rn(c, s), __fdiv_rn(d, s));
+                if (exact)
+                    return make_uint2(e4m3x4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv), e4m3x4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv));
+                return make_uint2(e4m3x4(__fdiv_rn(x[0], s), __fdiv_rn(x[1], s), __fdiv_rn(x[2], s), __fdiv_rn(x[3], s)),
+                                  e4m3x4(__fdiv_rn(x[4], s), __fdiv_rn(x[5], s), __fdiv_rn(x[6], s), __fdiv_rn(x[7], s)));
             }
-            return pack4(one(a), one(b), one(c), one(d));
+            constexpr float kMagic = 12582912.0f;
+            uint32_t        z[8];
+            float           off = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float f = fmaf(x[e], inv, kMagic);
+                z[e]          = __float_as_uint(f);
+                off           = fmaxf(off, fabsf(fmaf(x[e], inv, kMagic - f)));
+            }
+            if (off > 0.5f - 3.0517578125e-5f) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) z[e] = (uint32_t) near_middle(x[e], s);
+            }
+            return make_uint2(bytes(z[0], z[1], z[2], z[3]), bytes(z[4], z[5], z[6], z[7]));
+        }
+        static __device__ __forceinline__ uint32_t bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { // the low byte of each
+            return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
         }
     };
 
