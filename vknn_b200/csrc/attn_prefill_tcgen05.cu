@@ -233,7 +233,8 @@ namespace {
     template <int QT, int kRows> __device__ __forceinline__ PackedUnit packed_unit(const AttnParams &p, const int32_t *cu_q, const int32_t *cu_k, int u) {
         PackedUnit    x;
         int64_t       first;
-        const int64_t b  = vkc_packed_find(cu_q, p.nseq, p.Sq, u, kRows, 1, &first);
+        static_assert(kRows == 128 || kRows == 256, "a power of two");
+        const int64_t b  = vkc_packed_find(cu_q, p.nseq, p.Sq, u, kRows == 256 ? 8 : 7, 1, &first);
         const int     q0 = (int) vkc_packed_clamp(cu_q[b], p.Sq), sq = (int) vkc_packed_clamp(cu_q[b + 1], p.Sq) - q0;
         x.k0 = (int) vkc_packed_clamp(cu_k[b], p.Skv), x.sk = (int) vkc_packed_clamp(cu_k[b + 1], p.Skv) - x.k0;
         if (x.sk < 0) x.sk = 0;

@@ -15,7 +15,7 @@ int vkc_attn_prefill_packed_tcgen05(vkc_ctx *ctx, const void *Q, const void *K, 
 
 namespace {
 
-    constexpr int kRows = 8;  // query rows (= warps) per CTA
+    constexpr int kRows = 8;  // query rows (= warps) per CTA (packed sequences: 1 << 3)
     constexpr int kKeys = 32; // keys per shared-memory block
     constexpr int kMaxD = 256;
 
@@ -44,7 +44,7 @@ namespace {
         int64_t       Sq = p.Sq, Skv = p.Skv, q0 = 0, k0 = 0; // the sequence's lengths and first rows
         if (p.cu_q) {
             int64_t first;
-            b   = vkc_packed_find(p.cu_q, p.B, p.Sq, blockIdx.x, kRows, 1, &first);
+            b   = vkc_packed_find(p.cu_q, p.B, p.Sq, blockIdx.x, 3, 1, &first);
             i0  = (blockIdx.x - first) * kRows;
             q0  = vkc_packed_clamp(p.cu_q[b], p.Sq);
             k0  = vkc_packed_clamp(p.cu_k[b], p.Skv);

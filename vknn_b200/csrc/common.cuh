@@ -138,16 +138,16 @@ struct VkcDeviceGuard {
 
 #ifdef __CUDACC__
 // Packed sequences: which sequence the work unit `u` belongs to when the units of sequence b begin at
-// first(b) = cu[b] / step + extra * b (integer division, cu clamped to [0, total]). A sequence of n rows that is cut into
+// first(b) = cu[b] / step + extra * b (integer division by step = 1 << log2, cu clamped to [0, total]). A sequence of n rows that is cut into
 // pieces of `step` rows counted from its own beginning has at most n / step + 1 of them, and from any other beginning one more:
 // with extra = 1 or 2 that many units always lie between first(b) and first(b + 1), and there are
 // total / step + extra * nseq units in all. No list of the units is needed, only this search. One thread, log2(nseq) loads.
 __device__ __forceinline__ int64_t vkc_packed_clamp(int32_t v, int64_t total) { return v < 0 ? 0 : ((int64_t) v > total ? total : (int64_t) v); }
-__device__ __forceinline__ int vkc_packed_find(const int32_t *cu, int64_t nseq, int64_t total, int64_t u, int step, int extra, int64_t *first) {
+__device__ __forceinline__ int vkc_packed_find(const int32_t *cu, int64_t nseq, int64_t total, int64_t u, int log2, int extra, int64_t *first) {
     int64_t lo = 0, hi = nseq; // first(lo) <= u < first(hi)
-    int64_t at = vkc_packed_clamp(cu[0], total) / step;
+    int64_t at = vkc_packed_clamp(cu[0], total) >> log2;
     while (hi - lo > 1) {
-        const int64_t mid = (lo + hi) >> 1, f = vkc_packed_clamp(cu[mid], total) / step + extra * mid;
+        const int64_t mid = (lo + hi) >> 1, f = (vkc_packed_clamp(cu[mid], total) >> log2) + extra * mid;
         if (f <= u) lo = mid, at = f;
         else hi = mid;
     }
@@ -156,13 +156,13 @@ __device__ __forceinline__ int vkc_packed_find(const int32_t *cu, int64_t nseq, 
 }
 // The same by a whole warp, one load latency for up to 32 sequences and one more for every further factor of 32: also returns
 // the sequence's rows [x0, x1) and held[b] (0 if held is null).
-__device__ __forceinline__ int vkc_packed_find_warp(const int32_t *cu, const int32_t *held, int64_t nseq, int64_t total, int64_t u, int step, int extra,
+__device__ __forceinline__ int vkc_packed_find_warp(const int32_t *cu, const int32_t *held, int64_t nseq, int64_t total, int64_t u, int log2, int extra,
                                                     int64_t *first, int64_t *x0, int64_t *x1, int *held_b) {
     const int lane = threadIdx.x & 31;
     int64_t   lo = 0, hi = nseq;
     while (hi - lo > 32) { // 32 samples of [lo, hi)
         const int64_t stride = (hi - lo + 31) >> 5, b = lo + lane * stride;
-        const bool    le     = b < hi && (b == lo || vkc_packed_clamp(cu[b], total) / step + extra * b <= u);
+        const bool    le     = b < hi && (b == lo || (vkc_packed_clamp(cu[b], total) >> log2) + extra * b <= u);
         const int     k      = 31 - __clz(__ballot_sync(0xffffffffu, le));
         lo += k * stride;
         hi = lo + stride < hi ? lo + stride : hi;
@@ -171,7 +171,7 @@ __device__ __forceinline__ int vkc_packed_find_warp(const int32_t *cu, const int
     const bool    in   = b < hi;
     const int64_t mine = in ? vkc_packed_clamp(cu[b], total) : 0, next = in ? vkc_packed_clamp(cu[b + 1], total) : 0;
     const int     h    = in && held ? held[b] : 0;
-    const int64_t f    = mine / step + extra * b;
+    const int64_t f    = (mine >> log2) + extra * b;
     const int     k    = 31 - __clz(__ballot_sync(0xffffffffu, in && (b == lo || f <= u)));
     *first  = __shfl_sync(0xffffffffu, f, k);
     *x0     = __shfl_sync(0xffffffffu, mine, k);

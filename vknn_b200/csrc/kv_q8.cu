@@ -22,7 +22,7 @@ namespace {
         float         *scales[2];
         int64_t        xs[2][2]; // element strides {token, head}
         int64_t        B, Hkv, Lmax, total;
-        int            D, block, vshift; // D = 8 << vshift
+        int            D, block, vshift, bshift; // D = 8 << vshift, block = 1 << bshift
         const int32_t *cu, *kv_len;
         int            vec_ok; // bases and strides of K and V allow 16-byte loads
     };
@@ -74,7 +74,7 @@ namespace {
         int     start = 0; // tokens the sequence holds
         if (p.cu) {
             int64_t first, x1;
-            b   = vkc_packed_find_warp(p.cu, p.kv_len, p.B, p.total, blockIdx.x, block, 2, &first, &x0, &x1, &start);
+            b   = vkc_packed_find_warp(p.cu, p.kv_len, p.B, p.total, blockIdx.x, p.bshift, 2, &first, &x0, &x1, &start);
             n   = x1 - x0;
             blk = blockIdx.x - first;
         } else {
@@ -82,8 +82,8 @@ namespace {
             if (p.kv_len) start = p.kv_len[b];
         }
         if (blk < 0 || start < 0 || start >= p.Lmax) return;
-        blk += start / block;
-        const int64_t lo   = blk * block;
+        blk += start >> p.bshift;
+        const int64_t lo   = blk << p.bshift;
         const int64_t from = start > lo ? start : lo; // new rows of this block: positions [from, to)
         int64_t       to   = start + n < lo + block ? start + n : lo + block;
         if (to > p.Lmax) to = p.Lmax;
@@ -93,17 +93,23 @@ namespace {
 
         const int64_t row0  = (b * p.Hkv + hk) * p.Lmax + lo;
         uint8_t      *codes = p.codes[which] + row0 * D;
-        float        *scale = p.scales[which] + (b * p.Hkv + hk) * (p.Lmax / block) + blk;
+        float        *scale = p.scales[which] + (b * p.Hkv + hk) * (p.Lmax >> p.bshift) + blk;
         const T      *x     = (const T *) p.X[which] + (x0 + from - start) * p.xs[which][0] + hk * p.xs[which][1];
         const float   s_old = held ? *scale : 0.f;
 
+        // vector i of this thread: row first + i * step of the block, always the same dims
+        const int     first = tid >> sh, step = block >> 3;
+        const int64_t leap = step * p.xs[which][0];
+        x += (int64_t) (first - r0) * p.xs[which][0] + (tid - (first << sh)) * 8;
+        uint2   *at = reinterpret_cast<uint2 *>(codes) + tid;
         Row8<T>  rows[kVec];
         uint32_t top = 0; // bits of |x| order like the values, infinities and NaN above all
 #pragma unroll
         for (int i = 0; i < kVec; ++i) {
-            const int v = i * nt + tid, r = v >> sh, c = (v - (r << sh)) * 8;
-            if (r >= r0 && r < r1) rows[i].load(x + (int64_t) (r - r0) * p.xs[which][0] + c, p.vec_ok);
+            const int r = first + i * step;
+            if (r >= r0 && r < r1) rows[i].load(x, p.vec_ok);
             else rows[i].zero();
+            x += leap;
         }
 #pragma unroll
         for (int i = 0; i < kVec; ++i) top = rows[i].top(top);
@@ -123,24 +129,21 @@ namespace {
             const q8::Requant<kE4m3> re(s_old, s);
 #pragma unroll
             for (int i = 0; i < kVec; ++i) {
-                const int v = i * nt + tid, r = v >> sh;
-                if (r < r0) {
-                    uint2 *at = reinterpret_cast<uint2 *>(codes + (int64_t) v * 8);
-                    uint2  c  = *at;
+                if (first + i * step < r0) {
+                    uint2 c = at[i * nt];
                     c.x = re.four(c.x), c.y = re.four(c.y);
-                    *at = c;
+                    at[i * nt] = c;
                 }
             }
         }
 #pragma unroll
         for (int i = 0; i < kVec; ++i) {
-            const int v = i * nt + tid, r = v >> sh;
+            const int r = first + i * step;
             if (r >= r0 && r < r1) {
                 float f[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) f[e] = rows[i].get(e);
-                const uint2 c = quant.eight(f);
-                *reinterpret_cast<uint2 *>(codes + (int64_t) v * 8) = c;
+                at[i * nt] = quant.eight(f);
             }
         }
     }
@@ -178,7 +181,7 @@ extern "C" int vkc_kv_append_q8(vkc_ctx *ctx, const void *K, const void *V, void
             p.xs[w][i] = str[w][i];
             if (str[w][i] % per16) p.vec_ok = 0;
         }
-    p.B = B, p.Hkv = Hkv, p.Lmax = Lmax, p.total = total, p.D = (int) D, p.vshift = D == 64 ? 3 : D == 128 ? 4 : 5, p.block = (int) block, p.cu = cu, p.kv_len = kv_len;
+    p.B = B, p.Hkv = Hkv, p.Lmax = Lmax, p.total = total, p.D = (int) D, p.vshift = D == 64 ? 3 : D == 128 ? 4 : 5, p.block = (int) block, p.bshift = block == 32 ? 5 : block == 64 ? 6 : 7, p.cu = cu, p.kv_len = kv_len;
     const dim3 grid((unsigned) (cu ? total / block + 2 * B : B), (unsigned) Hkv, 2);
     const int  threads = (int) (block * D / 64);
     const bool e4m3    = cache_dtype == VKC_E4M3;

@@ -44,32 +44,20 @@ namespace q8 {
     }
     __device__ __forceinline__ int clamp127(int v) { return v > 127 ? 127 : (v < -127 ? -127 : v); }
 
-    // x / s to the nearest code. A scale that this library wrote is a power of two for e4m3, so that the product with its
-    // reciprocal is exact; any other one (a caller's own cache) takes the quotient rounded to fp32. For int8 the product with
-    // the rounded reciprocal is off by less than 2^-15 of a step, which decides every value that is not that close to the
-    // middle between two codes; those few take the correctly rounded quotient, and where even that lies exactly in the middle,
-    // the sign of the remainder.
+    // x / s to the nearest code, ties to even. A scale that this library wrote is a power of two for e4m3, so that the product with
+    // its reciprocal is exact; any other one (a caller's own cache) takes the quotient rounded to fp32. int8: the product with the
+    // rounded reciprocal names a code k that is at most one off, and the remainder x - k * s, which is exact in fp32 (both terms
+    // are multiples of 2^-24 of the power of two above s, and their difference is below s), says whether it is the nearest.
     template <bool kE4m3> struct Quant {
         float s, inv;
-        bool  none, exact; // none: the scale is 0 or NaN, every code is 0; exact: inv is exactly 1 / s
+        bool  none, exact; // none: every code is 0 (the scale is 0 or NaN; one below 2^-126 only goes with zeros); exact: inv is exactly 1 / s
         __device__ __forceinline__ explicit Quant(float scale) : s(scale) {
             const uint32_t bits = __float_as_uint(scale);
-            none                = !(scale > 0.f);
+            none                = !(scale >= __uint_as_float(1u << 23));
             exact               = (bits & 0x7fffffu) == 0 && (bits >> 23) >= 1 && (bits >> 23) <= 253;
             inv                 = kE4m3 && exact ? __uint_as_float(0x7f000000u - bits) : __fdiv_rn(1.0f, scale);
         }
-        static __device__ __noinline__ int near_middle(float x, float s) {
-            const float y = __fdiv_rn(x, s);
-            float       r = rintf(y);
-            if (fabsf(y - truncf(y)) == 0.5f) {
-                const float rest = fmaf(-y, s, x); // x - y * s, rounded once: its sign is the true one
-                if (rest > 0.f) r = ceilf(y);
-                else if (rest < 0.f) r = floorf(y);
-            }
-            return clamp127((int) r);
-        }
-        // Eight values. int8: adding 1.5 * 2^23 leaves the nearest integer in the low bits of the sum; what the values are off
-        // their codes says whether one of them is close to the middle.
+        // Eight values. int8: adding 1.5 * 2^23 leaves the nearest integer in the low bits of the sum.
         __device__ __forceinline__ uint2 eight(const float (&x)[8]) const {
             if (none) return make_uint2(0u, 0u);
             if (kE4m3) {
@@ -79,17 +67,22 @@ namespace q8 {
                                   e4m3x4(__fdiv_rn(x[4], s), __fdiv_rn(x[5], s), __fdiv_rn(x[6], s), __fdiv_rn(x[7], s)));
             }
             constexpr float kMagic = 12582912.0f;
+            const float     half   = 0.5f * s;
             uint32_t        z[8];
-            float           off = 0.f;
+            float           rest[8], most = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const float f = fmaf(x[e], inv, kMagic);
                 z[e]          = __float_as_uint(f);
-                off           = fmaxf(off, fabsf(fmaf(x[e], inv, kMagic - f)));
+                rest[e]       = fmaf(kMagic - f, s, x[e]);
+                most          = fmaxf(most, fabsf(rest[e]));
             }
-            if (off > 0.5f - 3.0517578125e-5f) {
+            if (most >= half) { // some value lies in the middle between two codes, or its code is one off
 #pragma unroll
-                for (int e = 0; e < 8; ++e) z[e] = (uint32_t) near_middle(x[e], s);
+                for (int e = 0; e < 8; ++e) {
+                    const float a = fabsf(rest[e]);
+                    if (a > half || (a == half && (z[e] & 1u))) z[e] += rest[e] > 0.f ? 1u : ~0u;
+                }
             }
             return make_uint2(bytes(z[0], z[1], z[2], z[3]), bytes(z[4], z[5], z[6], z[7]));
         }
