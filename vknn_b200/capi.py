@@ -117,14 +117,17 @@ def _dtype_code(t):
     return {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}[t.dtype]
 
 
-_code_of = {}  # torch dtype -> code, filled by the first call (torch is imported late)
+# torch dtype -> code; this and the two types below are filled by the first call (torch is imported late)
+_code_of, _torch_float32, _torch_int32, _I64x2 = {}, [], [], C.c_int64 * 2
 
 
 def _any_dtype_code(t):
     if not _code_of:
         import torch
+        _torch_float32.append(torch.float32)
+        _torch_int32.append(torch.int32)
         _code_of.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.float8_e4m3fn: E4M3, torch.int8: I8})
-    return _code_of[t.dtype]
+    return _code_of.get(t.dtype, -1)
 
 
 def _np_dtype_code(a):
@@ -235,7 +238,7 @@ class Context:
         if stream is not None:
             return C.c_void_p(stream)
         import torch
-        h = torch.cuda.current_stream(self.device).cuda_stream
+        h = torch._C._cuda_getCurrentRawStream(self.device)  # current_stream(device).cuda_stream without the Python object
         # torch's default stream is the legacy NULL stream; NULL means "the context's own stream" in the C-ABI,
         # so name the legacy stream by its explicit handle (cudaStreamLegacy == 0x1) to keep torch ordering.
         return C.c_void_p(h if h else 1)
@@ -317,81 +320,79 @@ class Context:
         """The pointer of an int32 tensor of n elements on this device, or None."""
         if t is None:
             return None
-        import torch
-        if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() or t.get_device() != self.device:
+        if t.dtype is not _torch_int32[0] or t.shape != (n,) or t.stride(0) != 1 or t.get_device() != self.device:
             raise ValueError("%s must be a contiguous int32 tensor of %d elements on cuda:%d" % (what, n, self.device))
         return t.data_ptr()
-
-    def _here(self, *tensors):
-        for t in tensors:
-            if t.get_device() != self.device:
-                raise ValueError("the context belongs to cuda:%d, a tensor lies on %s" % (self.device, t.device))
 
     def attn_prefill_packed(self, Q, K, V, O, scale, cu_q, cu_k=None, causal=True, stream=None):
         """Attention over sequences of different lengths packed one behind the other: Q/O [total_q,Hq,D], K/V [total_k,Hkv,D], any
         strides with D contiguous (views of a packed qkv projection are fine). Sequence b owns the rows cu_q[b]..cu_q[b+1] of
         Q and O and cu_k[b]..cu_k[b+1] of K and V (int32 device tensors of nseq + 1 offsets; cu_k None = cu_q). Rows of O that
         belong to no sequence are left as they were; a row that sees no key becomes NaN."""
-        total_q, Hq, D = Q.shape
-        total_k, Hkv, _ = K.shape
-        self._here(Q, K, V, O)
-        if K.shape != V.shape or K.shape[2] != D or O.shape != Q.shape or not (Q.dtype == K.dtype == V.dtype == O.dtype):
-            raise ValueError("attn_prefill_packed: Q %s, K %s, V %s and O %s do not go together" % tuple("%s %s" % (tuple(t.shape), t.dtype) for t in (Q, K, V, O)))
-        strides = []
-        for t in (Q, K, V, O):
-            a, b, c = t.stride()
-            if c != 1 and D > 1:
-                raise ValueError("attn_prefill_packed: the last dimension must be contiguous")
-            strides.append((C.c_int64 * 2)(a, b))
-        nseq = cu_q.shape[0] - 1
-        self._check(self.lib.vkc_attn_prefill_packed(self.h, Q.data_ptr(), K.data_ptr(), V.data_ptr(), O.data_ptr(), nseq, Hq, Hkv, D, total_q, total_k,
-                                                     self._int32(cu_q, nseq + 1, "cu_q"), self._int32(cu_k, nseq + 1, "cu_k"), *strides, float(scale),
-                                                     1 if causal else 0, _any_dtype_code(Q), self._stream(stream)))
+        q_shape, k_shape, dtype, dev = Q.shape, K.shape, Q.dtype, self.device
+        total_q, Hq, D = q_shape
+        total_k, Hkv, Dk = k_shape
+        (q0, q1, q2), (k0, k1, k2), (v0, v1, v2), (o0, o1, o2) = Q.stride(), K.stride(), V.stride(), O.stride()
+        if (Dk != D or V.shape != k_shape or O.shape != q_shape or K.dtype is not dtype or V.dtype is not dtype or O.dtype is not dtype or
+                (D > 1 and not q2 == k2 == v2 == o2 == 1)):
+            raise ValueError("attn_prefill_packed: Q %s, K %s, V %s and O %s do not go together, or their last dimension is not contiguous"
+                             % tuple("%s %s" % (tuple(t.shape), t.dtype) for t in (Q, K, V, O)))
+        if Q.get_device() != dev or K.get_device() != dev or V.get_device() != dev or O.get_device() != dev:
+            raise ValueError("attn_prefill_packed: the context belongs to cuda:%d, a tensor lies elsewhere" % dev)
+        code, nseq = _any_dtype_code(Q), cu_q.shape[0] - 1
+        rc = self.lib.vkc_attn_prefill_packed(self.h, Q.data_ptr(), K.data_ptr(), V.data_ptr(), O.data_ptr(), nseq, Hq, Hkv, D, total_q, total_k,
+                                              self._int32(cu_q, nseq + 1, "cu_q"), self._int32(cu_k, nseq + 1, "cu_k") if cu_k is not cu_q else None,
+                                              _I64x2(q0, q1), _I64x2(k0, k1), _I64x2(v0, v1), _I64x2(o0, o1), float(scale), 1 if causal else 0, code,
+                                              self._stream(stream))
+        if rc:
+            self._check(rc)
 
     def _q8_cache(self, Kc, Vc, k_scale, v_scale):
-        """Shape of an 8-bit cache, (B, Hkv, Lmax, D, block, type code), after checking that its four tensors go together."""
-        import torch
-        B, Hkv, Lmax, D = Kc.shape
-        nb = k_scale.shape[-1]
-        self._here(Kc, Vc, k_scale, v_scale)
-        if (Vc.shape != Kc.shape or Vc.dtype != Kc.dtype or k_scale.shape != (B, Hkv, nb) or v_scale.shape != (B, Hkv, nb) or nb < 1 or Lmax % nb or
-                k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32 or not (Kc.is_contiguous() and Vc.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous())):
-            raise ValueError("the cache is Kc, Vc [B,Hkv,Lmax,D] and float32 k_scale, v_scale [B,Hkv,Lmax/block], all contiguous: got %s, %s, %s, %s"
-                             % tuple("%s %s" % (tuple(t.shape), t.dtype) for t in (Kc, Vc, k_scale, v_scale)))
-        code = _any_dtype_code(Kc)
-        if code != E4M3 and code != I8:
-            raise ValueError("the cache holds float8_e4m3fn or int8 codes, not %s" % Kc.dtype)
-        return B, Hkv, Lmax, D, Lmax // nb, code
+        """Shape of an 8-bit cache and its type code, (B, Hkv, Lmax, D), block, code, after checking that its four tensors go together."""
+        code, shape, s_shape, dev = _any_dtype_code(Kc), Kc.shape, k_scale.shape, self.device
+        B, Hkv, Lmax, _ = shape
+        nb = s_shape[2] if len(s_shape) == 3 else 0
+        f32 = _torch_float32[0]
+        if (code < E4M3 or Vc.dtype is not Kc.dtype or Vc.shape != shape or s_shape != (B, Hkv, nb) or v_scale.shape != s_shape or nb < 1 or Lmax % nb or
+                k_scale.dtype is not f32 or v_scale.dtype is not f32 or
+                not (Kc.is_contiguous() and Vc.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous())):
+            raise ValueError("the cache is Kc, Vc [B,Hkv,Lmax,D] of float8_e4m3fn or int8 and k_scale, v_scale [B,Hkv,Lmax/block] of float32, all contiguous: got "
+                             "%s, %s, %s, %s" % tuple("%s %s" % (tuple(t.shape), t.dtype) for t in (Kc, Vc, k_scale, v_scale)))
+        if Kc.get_device() != dev or Vc.get_device() != dev or k_scale.get_device() != dev or v_scale.get_device() != dev:
+            raise ValueError("the context belongs to cuda:%d, the cache lies elsewhere" % dev)
+        return shape, Lmax // nb, code
 
     def kv_append_q8(self, K, V, Kc, Vc, k_scale, v_scale, kv_len=None, cu=None, stream=None):
         """Appends K/V [total,Hkv,D] to an 8-bit cache: Kc/Vc [B,Hkv,Lmax,D] (float8_e4m3fn or int8) with one float32 scale per
         block of Lmax // k_scale.shape[2] tokens and head. kv_len int32 [B]: the tokens each sequence holds (None: none; not
         changed by the call); cu int32 [B+1]: sequence b brings the rows cu[b]..cu[b+1] (None: one row each)."""
-        B, Hkv, Lmax, D, block, code = self._q8_cache(Kc, Vc, k_scale, v_scale)
-        total = K.shape[0]
-        self._here(K, V)
-        if K.shape != (total, Hkv, D) or V.shape != K.shape or V.dtype != K.dtype or K.stride(2) != 1 or V.stride(2) != 1:
-            raise ValueError("kv_append_q8: K and V must be [total,%d,%d] with the last dimension contiguous" % (Hkv, D))
-        self._check(self.lib.vkc_kv_append_q8(self.h, K.data_ptr(), V.data_ptr(), Kc.data_ptr(), Vc.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), B, Hkv,
-                                              Lmax, D, block, total, self._int32(cu, B + 1, "cu"), self._int32(kv_len, B, "kv_len"),
-                                              (C.c_int64 * 2)(K.stride(0), K.stride(1)), (C.c_int64 * 2)(V.stride(0), V.stride(1)), _any_dtype_code(K), code,
-                                              self._stream(stream)))
+        (B, Hkv, Lmax, D), block, code = self._q8_cache(Kc, Vc, k_scale, v_scale)
+        total, heads, dim = shape = K.shape
+        (k0, k1, k2), (v0, v1, v2), dev = K.stride(), V.stride(), self.device
+        if heads != Hkv or dim != D or V.shape != shape or V.dtype is not K.dtype or k2 != 1 or v2 != 1 or K.get_device() != dev or V.get_device() != dev:
+            raise ValueError("kv_append_q8: K and V must be [total,%d,%d] of one type on cuda:%d with the last dimension contiguous" % (Hkv, D, dev))
+        rc = self.lib.vkc_kv_append_q8(self.h, K.data_ptr(), V.data_ptr(), Kc.data_ptr(), Vc.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), B, Hkv, Lmax, D,
+                                       block, total, self._int32(cu, B + 1, "cu"), self._int32(kv_len, B, "kv_len"), _I64x2(k0, k1), _I64x2(v0, v1),
+                                       _any_dtype_code(K), code, self._stream(stream))
+        if rc:
+            self._check(rc)
 
     def attn_decode_q8_workspace_bytes(self, B, Hq, Hkv, Lmax, D):
         return int(self.lib.vkc_attn_decode_q8_workspace_bytes(B, Hq, Hkv, Lmax, D))
 
     def attn_decode_q8(self, Q, Kc, Vc, k_scale, v_scale, O, scale, kv_len=None, workspace=None, stream=None):
         """attn_decode over the 8-bit cache that kv_append_q8 fills: Q/O [B,Hq,D] contiguous, float16 or bfloat16."""
-        B, Hkv, Lmax, D, block, code = self._q8_cache(Kc, Vc, k_scale, v_scale)
-        Hq = Q.shape[1]
-        self._here(Q, O)
-        if Q.shape != (B, Hq, D) or O.shape != Q.shape or O.dtype != Q.dtype or not (Q.is_contiguous() and O.is_contiguous()):
-            raise ValueError("attn_decode_q8: Q and O must be contiguous [%d,Hq,%d] of one type" % (B, D))
-        self._check(self.lib.vkc_attn_decode_q8(self.h, Q.data_ptr(), Kc.data_ptr(), Vc.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), O.data_ptr(), B,
-                                                Hq, Hkv, Lmax, D, block, self._int32(kv_len, B, "kv_len"), float(scale),
-                                                workspace.data_ptr() if workspace is not None else None,
-                                                workspace.numel() * workspace.element_size() if workspace is not None else 0, _any_dtype_code(Q), code,
-                                                self._stream(stream)))
+        (B, Hkv, Lmax, D), block, code = self._q8_cache(Kc, Vc, k_scale, v_scale)
+        shape, dev = Q.shape, self.device
+        if (len(shape) != 3 or shape[0] != B or shape[2] != D or O.shape != shape or O.dtype is not Q.dtype or not (Q.is_contiguous() and O.is_contiguous()) or
+                Q.get_device() != dev or O.get_device() != dev):
+            raise ValueError("attn_decode_q8: Q and O must be contiguous [%d,Hq,%d] of one type on cuda:%d" % (B, D, dev))
+        rc = self.lib.vkc_attn_decode_q8(self.h, Q.data_ptr(), Kc.data_ptr(), Vc.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), O.data_ptr(), B, shape[1], Hkv,
+                                         Lmax, D, block, self._int32(kv_len, B, "kv_len"), float(scale), workspace.data_ptr() if workspace is not None else None,
+                                         workspace.numel() * workspace.element_size() if workspace is not None else 0, _any_dtype_code(Q), code,
+                                         self._stream(stream))
+        if rc:
+            self._check(rc)
 
     def attn_prefill_fanout(self, Q, K, V, dests, flags, state, o_strides, scale, causal=False, kv_len=None, stream=None, mcast=None):
         """attn_prefill whose output rows are stored into every buffer of `dests` (raw device pointers mapped on this GPU,

@@ -64,7 +64,7 @@ namespace {
         __device__ __forceinline__ float get(int i) const { return St<T>::ld(reinterpret_cast<const T *>(v) + i); }
     };
 
-    template <typename T, bool kE4m3> __global__ void __launch_bounds__(512) kv_append_kernel(const AppendParams p) {
+    template <typename T, bool kE4m3> __global__ void __launch_bounds__(512, 2) kv_append_kernel(const AppendParams p) {
         const int     tid = threadIdx.x, nt = blockDim.x, which = blockIdx.z, hk = blockIdx.y;
         const int     D = p.D, block = p.block, sh = p.vshift; // 1 << sh vectors per row
         vkc_grid_dep_wait();
