@@ -131,6 +131,12 @@ namespace {
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     }
+    // ... D = A * B, with no accumulator to clear first
+    __device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+    }
     // four codes -> two f16 pairs, low pair first
     template <bool kE4m3> __device__ __forceinline__ void codes_to_f16(uint32_t x, uint32_t &lo, uint32_t &hi) {
         if (kE4m3) {
@@ -266,21 +272,26 @@ namespace {
             v_at[0] = swz((uint32_t) (2 * t) * D + g * (D / 8)), v_at[1] = swz((uint32_t) (2 * t + 1) * D + g * (D / 8));
 
             // ---- producer (lane 0): the tile at `pa` into stage `ps`
-            At   pa = at;
-            int  ps = 0, left = P1 - P0; // tiles not yet fetched
-            auto fetch = [&]() {
+            At       pa = at;
+            int      left = P1 - P0; // tiles not yet fetched
+            int      row0 = (pa.b * Hkv + pa.hk) * rows_per_unit; // the unit's first row of 128 bytes
+            uint32_t p_bar = bars, p_dst = ring, p_sc = sc_a;       // of the stage
+            auto     fetch = [&]() {
                 if (left == 0) return;
-                const int      unit = pa.b * Hkv + pa.hk, row = unit * rows_per_unit + pa.tile * rows_per_tile;
-                const uint32_t bar = bars + 8u * ps, dst = ring + (uint32_t) ps * 2 * L::TILE;
-                ptx::mbar_expect_tx(bar, 2 * L::TILE);
-                ptx::tma_load_2d(dst, &tmK, 0, row, bar);
-                ptx::tma_load_2d(dst + L::TILE, &tmV, 0, row, bar);
-                const int64_t si = (int64_t) unit * nb + ((pa.tile * kTile) >> p.block_log2);
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sc_a + 8u * ps), "l"(p.q.ks + si) : "memory");
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sc_a + 8u * ps + 4u), "l"(p.q.vs + si) : "memory");
-                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-                ps = ps + 1 == S ? 0 : ps + 1;
-                if (--left > 0 && ++pa.tile == pa.n) next_unit(pa);
+                const int row = row0 + pa.tile * rows_per_tile;
+                ptx::mbar_expect_tx(p_bar, 2 * L::TILE);
+                ptx::tma_load_2d(p_dst, &tmK, 0, row, p_bar);
+                ptx::tma_load_2d(p_dst + L::TILE, &tmV, 0, row, p_bar);
+                const int64_t si = (int64_t) (pa.b * Hkv + pa.hk) * nb + ((pa.tile * kTile) >> p.block_log2);
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(p_sc), "l"(p.q.ks + si) : "memory");
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(p_sc + 4u), "l"(p.q.vs + si) : "memory");
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(p_bar) : "memory");
+                p_bar += 8u, p_dst += 2 * L::TILE, p_sc += 8u;
+                if (p_bar == bars + 8u * S) p_bar = bars, p_dst = ring, p_sc = sc_a;
+                if (--left > 0 && ++pa.tile == pa.n) {
+                    next_unit(pa);
+                    row0 = (pa.b * Hkv + pa.hk) * rows_per_unit;
+                }
             };
             if (lane == 0)
                 for (int i = 0; i < S; ++i) fetch();
@@ -347,8 +358,6 @@ namespace {
                     // scores: four groups of eight keys
                     float s[4][4];
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-#pragma unroll
                     for (int c = 0; c < CH; ++c) {
 #pragma unroll
                         for (int n = 0; n < 4; ++n) {
@@ -358,8 +367,9 @@ namespace {
                             for (int k = 0; k < 4; ++k) {
                                 uint32_t b0, b1;
                                 codes_to_f16<kE4m3>(w[k], b0, b1);
-                                if (NT == 1) mma16816(s[n], qa[0][c * 4 + k][0], 0u, qa[0][c * 4 + k][1], 0u, b0, b1);
-                                else mma16816(s[n], qa[0][c * 4 + k][0], qa[NT - 1][c * 4 + k][0], qa[0][c * 4 + k][1], qa[NT - 1][c * 4 + k][1], b0, b1);
+                                const uint32_t *q0 = qa[0][c * 4 + k], *q1 = qa[NT - 1][c * 4 + k];
+                                if (c == 0 && k == 0) mma16816_first(s[n], q0[0], NT == 1 ? 0u : q1[0], q0[1], NT == 1 ? 0u : q1[1], b0, b1);
+                                else mma16816(s[n], q0[0], NT == 1 ? 0u : q1[0], q0[1], NT == 1 ? 0u : q1[1], b0, b1);
                             }
                         }
                     }
@@ -430,14 +440,15 @@ namespace {
                             for (int half = 0; half < 2; ++half) {
                                 float d[NT][4];
 #pragma unroll
-                                for (int h = 0; h < NT; ++h) d[h][0] = d[h][1] = d[h][2] = d[h][3] = 0.f;
-#pragma unroll
                                 for (int st = 0; st < 2; ++st) {
                                     uint32_t a0, a1, a2, a3;
                                     codes_to_f16<kE4m3>(__byte_perm(x[st][0][w], x[st][1][w], half ? 0x7362 : 0x5140), a0, a1);
                                     codes_to_f16<kE4m3>(__byte_perm(x[st][2][w], x[st][3][w], half ? 0x7362 : 0x5140), a2, a3);
 #pragma unroll
-                                    for (int h = 0; h < NT; ++h) mma16816(d[h], a0, a1, a2, a3, pb[h][2 * st], pb[h][2 * st + 1]);
+                                    for (int h = 0; h < NT; ++h) {
+                                        if (st == 0) mma16816_first(d[h], a0, a1, a2, a3, pb[h][0], pb[h][1]);
+                                        else mma16816(d[h], a0, a1, a2, a3, pb[h][2], pb[h][3]);
+                                    }
                                 }
                                 const int i = (q4 * 4 + w) * 2 + half;
 #pragma unroll
@@ -489,26 +500,25 @@ namespace {
             for (int i = 0; i < 50; ++i) __nanosleep(20000); // aborted: let copies in flight land
     }
 
-    // Joins the partials of unit (sequence blockIdx.y, kv head blockIdx.x) if it was cut: slot 1 of the run it begins in, slot 0 of the
-    // runs behind it. A thread takes four dims of one head over every `groups`-th partial, eight of them on their way at a time;
-    // the groups meet in shared memory, in order.
-    template <typename T, int D> __global__ void __launch_bounds__(1024) attn_decode_q8_join_kernel(const StreamParams p, int lanes) {
-        constexpr int U = 8;
-        extern __shared__ float4 sm4[]; // [threads] O, then [threads] (maximum, sum)
-        float2        *sml = reinterpret_cast<float2 *>(sm4 + blockDim.x);
-        const int      b = blockIdx.y, hk = blockIdx.x, grp = threadIdx.x / lanes, ln = threadIdx.x - grp * lanes, groups = blockDim.x / lanes;
+    // Joins one head's partials of unit (sequence blockIdx.z, kv head blockIdx.y) if it was cut: slot 1 of the run it begins in, slot 0
+    // of the runs behind it. A thread takes four dims over every `groups`-th partial, eight of them on their way at a time; the
+    // groups meet in shared memory, in order.
+    constexpr int kJoinGroups = 16;
+    template <typename T, int D> __global__ void __launch_bounds__(kJoinGroups * D / 4) attn_decode_q8_join_kernel(const StreamParams p) {
+        constexpr int U = 8, LANES = D / 4;
+        __shared__ float4 so[kJoinGroups][LANES];
+        __shared__ float2 sml[kJoinGroups];
+        const int b = blockIdx.z, hk = blockIdx.y, hd = blockIdx.x, grp = threadIdx.x / LANES, ln = threadIdx.x % LANES, groups = blockDim.x / LANES;
         vkc_grid_dep_wait();
         vkc_grid_dep_launch();
         const int t0 = p.line[b], t1 = p.line[b + 1], quota = p.line[p.B + 1];
         const int n = (t1 - t0) / (int) p.q.Hkv, off = t0 + hk * n;
         const int r0 = off / quota, parts = n > 0 ? (off + n - 1) / quota - r0 + 1 : 0;
         if (parts < 2) return;
-        const int  hd = ln * 4 / D, d = ln * 4 - hd * D;
-        const bool in = hd < p.G;
-        auto       row = [&](int k) { return ((int64_t) (r0 + k) * 2 + (k ? 0 : 1)) * p.G + hd; };
-        float      top = -INFINITY, ls = 0.f;
-        float4     acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        auto       merge = [&](const float2 (&ml)[U], const float4 (&v)[U]) {
+        auto   row = [&](int k) { return ((int64_t) (r0 + k) * 2 + (k ? 0 : 1)) * p.G + hd; };
+        float  top = -INFINITY, ls = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto   merge = [&](const float2 (&ml)[U], const float4 (&v)[U]) {
             float now = top;
 #pragma unroll
             for (int u = 0; u < U; ++u) now = fmaxf(now, ml[u].x);
@@ -525,33 +535,35 @@ namespace {
         };
         float2 ml[U];
         float4 v[U];
-        for (int k0 = grp; k0 < parts && in; k0 += U * groups) {
+        for (int k0 = grp; k0 < parts; k0 += U * groups) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int  k    = k0 + u * groups;
                 const bool have = k < parts;
                 ml[u]           = have ? *reinterpret_cast<const float2 *>(p.part_ml + row(k) * 2) : make_float2(-INFINITY, 0.f);
-                v[u]            = have ? *reinterpret_cast<const float4 *>(p.part_o + row(k) * D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+                v[u]            = have ? *reinterpret_cast<const float4 *>(p.part_o + row(k) * D + ln * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
             merge(ml, v);
         }
         if (groups > 1) {
-            sm4[threadIdx.x] = acc, sml[threadIdx.x] = make_float2(top, ls);
+            so[grp][ln] = acc;
+            if (ln == 0) sml[grp] = make_float2(top, ls);
             __syncthreads();
             if (grp != 0) return;
             top = -INFINITY, ls = 0.f, acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int k0 = 0; k0 < groups; k0 += U) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                ml[u] = u < groups ? sml[u * lanes + ln] : make_float2(-INFINITY, 0.f);
-                v[u]  = u < groups ? sm4[u * lanes + ln] : make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int u = 0; u < U; ++u) {
+                    const bool have = k0 + u < groups;
+                    ml[u]           = have ? sml[k0 + u] : make_float2(-INFINITY, 0.f);
+                    v[u]            = have ? so[k0 + u][ln] : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+                merge(ml, v);
             }
-            merge(ml, v);
         }
-        if (in) {
-            const float inv = 1.0f / ls;
-            T          *to  = (T *) p.q.O + ((int64_t) b * p.q.Hq + (int64_t) hk * p.G + hd) * D + d;
-            *reinterpret_cast<uint2 *>(to) = make_uint2(pair16<T>(acc.x * inv, acc.y * inv), pair16<T>(acc.z * inv, acc.w * inv));
-        }
+        const float inv = 1.0f / ls;
+        T          *to  = (T *) p.q.O + ((int64_t) b * p.q.Hq + (int64_t) hk * p.G + hd) * D + ln * 4;
+        *reinterpret_cast<uint2 *>(to) = make_uint2(pair16<T>(acc.x * inv, acc.y * inv), pair16<T>(acc.z * inv, acc.w * inv));
     }
 
     // Runs of a launch that can have tiles, and bytes of the workspace: partials of two cut units for each of them, and the line.
@@ -571,14 +583,11 @@ namespace {
         if (int rc = vkc_configure_smem(ctx, kern, smem)) return rc;
         vkc_launch(ctx, kern, dim3((unsigned) grid), dim3(Stream<D, NT>::W * 32), smem, st, tk, tv, p);
         if (int rc = vkc_post_launch(ctx, "attn_decode_q8")) return rc;
-        // threads of the join: the rows of a unit, times up to eight groups where a unit is cut into many parts (as many as it would
-        // be with sequences of full length)
-        const int     lanes = (p.G * D / 4 + 31) / 32 * 32;
-        const int64_t parts = (int64_t) grid * Stream<D, NT>::W / ((int64_t) p.B * p.q.Hkv);
+        // groups of the join: as many as give each of them eight partials of a unit, were all sequences of full length
+        const int64_t parts  = (int64_t) grid * Stream<D, NT>::W / ((int64_t) p.B * p.q.Hkv);
         int           groups = 1;
-        while (groups < 8 && parts > 8 * groups && lanes * groups * 2 <= 1024) groups *= 2;
-        const int threads = lanes * groups;
-        vkc_launch(ctx, attn_decode_q8_join_kernel<T, D>, dim3((unsigned) p.q.Hkv, (unsigned) p.B), dim3((unsigned) threads), (size_t) threads * 24, st, p, lanes);
+        while (groups < kJoinGroups && parts > 8 * groups) groups *= 2;
+        vkc_launch(ctx, attn_decode_q8_join_kernel<T, D>, dim3((unsigned) p.G, (unsigned) p.q.Hkv, (unsigned) p.B), dim3((unsigned) (groups * D / 4)), 0, st, p);
         return vkc_post_launch(ctx, "attn_decode_q8_join");
     }
     template <typename T, int D> int pick_stream_form(vkc_ctx *ctx, const StreamParams &p, bool e4m3, int grid, const CUtensorMap &tk, const CUtensorMap &tv, cudaStream_t st) {
