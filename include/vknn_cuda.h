@@ -283,8 +283,9 @@ VKC_API int vkc_kv_append_q8(vkc_ctx *ctx, const void *K, const void *V, void *K
  *   a sequence with no key stores NaN, as in vkc_attn_decode. What lies behind kv_len in the cache is never used, whatever
  *   its bits. Sums and softmax statistics are fp32; Q keeps its precision.
  *   workspace: device scratch of at least vkc_attn_decode_q8_workspace_bytes(...) bytes (16-byte aligned) for the partial
- *   results; NULL lets the context keep (and grow) its own. Two calls that may run at the same time need workspaces of their
- *   own. ---- */
+ *   results; NULL lets the context keep (and grow) its own. It may hold anything before the call. Two calls that may run at
+ *   the same time need workspaces of their own, and so do two captured graphs that may be replayed at the same time; calls
+ *   captured without a workspace share the context's. ---- */
 VKC_API size_t vkc_attn_decode_q8_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Lmax, int64_t D);
 VKC_API int    vkc_attn_decode_q8(vkc_ctx *ctx, const void *Q, const void *Kc, const void *Vc, const float *k_scale, const float *v_scale, void *O,
                                   int64_t B, int64_t Hq, int64_t Hkv, int64_t Lmax, int64_t D, int64_t block, const int32_t *kv_len, float scale,

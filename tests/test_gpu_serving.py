@@ -230,6 +230,54 @@ def test_packed_same_bits_again_on_another_stream_and_in_a_graph(ctx):
     assert torch.equal(o2, want)
 
 
+def test_packed_output_strides_that_16_bytes_cannot_follow(ctx):
+    lq, hq, hkv, d = [150, 3, 260], 4, 2, 64
+    q, k, v = packed_case(11, lq, lq, hq, hkv, d, torch.float16)
+    o = torch.full((sum(lq), hq, d + 3), 5.0, dtype=torch.float16, device="cuda")
+    want = torch.zeros_like(q)
+    ctx.attn_prefill_packed(q, k, v, o[:, :, 1:d + 1], d ** -0.5, offsets(lq))
+    ctx.attn_prefill_packed(q, k, v, want, d ** -0.5, offsets(lq))
+    ctx.sync()
+    assert torch.equal(o[:, :, 1:d + 1], want) and bool((o[:, :, 0] == 5).all()) and bool((o[:, :, d + 1:] == 5).all())
+
+
+@pytest.mark.parametrize("hq,hkv,d,nseq,hi", [(32, 8, 128, 300, 60), (20, 20, 64, 300, 60), (18, 6, 128, 280, 70), (4, 2, 64, 900, 5), (6, 6, 128, 700, 6), (64, 2, 64, 40, 300)],
+                         ids=["pairs_many_rounds", "rows_many_rounds", "odd_group", "more_units_than_are_ranked", "rows_more_units", "wide_group"])
+def test_packed_many_sequences(ctx, hq, hkv, d, nseq, hi):
+    """Many rounds per CTA, more units than one CTA ranks, groups of odd and of large size. Against the SIMT kernel, which the tests
+    above compare with 64 bits: each is within its own bound of the exact value, so they differ by the sum of the two."""
+    lq = [int(x) for x in np.random.default_rng(nseq).integers(0, hi + 1, nseq)]
+    q, k, v = packed_case(12, lq, lq, hq, hkv, d, torch.bfloat16)
+    o, want = torch.full_like(q, 9.0), torch.full_like(q, 9.0)
+    ctx.attn_prefill_packed(q, k, v, o, d ** -0.5, offsets(lq))
+    ctx.set_impl(vknn_b200.IMPL_SIMT)
+    ctx.attn_prefill_packed(q, k, v, want, d ** -0.5, offsets(lq))
+    ctx.set_impl(vknn_b200.IMPL_AUTO)
+    ctx.sync()
+    # sum p |v| through the same SIMT kernel
+    a = torch.zeros_like(q)
+    ctx.set_impl(vknn_b200.IMPL_SIMT)
+    ctx.attn_prefill_packed(q, k, v.abs(), a, d ** -0.5, offsets(lq))
+    ctx.set_impl(vknn_b200.IMPL_AUTO)
+    ctx.sync()
+    u = half_step(torch.bfloat16)
+    w, s = want.double(), a.double() * (1 + 2 * u)  # (a is itself rounded)
+    tol = 2 * u * w.abs() * (1 + u) + (u + 2 * SMALL) * s * (1 + u)
+    assert bool(((o.double() - w).abs() <= tol).all())
+
+
+def test_packed_same_offsets_for_queries_and_a_longer_key_buffer(ctx):
+    """cu_k may be the very tensor cu_q while K and V have more rows than Q."""
+    lq, h, d = [30, 41], 2, 64
+    q, _, _ = packed_case(13, lq, lq, h, h, d, torch.float16)
+    _, k, v = packed_case(14, lq, [300], h, h, d, torch.float16)
+    cu, o, want = offsets(lq), torch.zeros_like(q), torch.zeros_like(q)
+    ctx.attn_prefill_packed(q, k, v, o, d ** -0.5, cu, cu_k=cu)
+    ctx.attn_prefill_packed(q, k[:71], v[:71], want, d ** -0.5, cu)
+    ctx.sync()
+    assert torch.equal(o, want)
+
+
 def test_packed_nothing_to_do(ctx):
     e = torch.zeros(0, 2, 64, dtype=torch.float16, device="cuda")
     ctx.attn_prefill_packed(e, e, e, e, 1.0, offsets([0, 0]))
@@ -621,6 +669,66 @@ def test_decode_q8_same_bits_again_with_a_workspace_on_a_stream_and_in_a_graph(c
     torch.cuda.synchronize()
     ref, a = decode64(q, cache, lens.tolist(), d ** -0.5)
     check(got[0], ref, a, torch.bfloat16, torch.float16)
+
+
+def test_decode_q8_more_sequences_than_one_launch_holds(ctx):
+    b, hq, hkv, lmax, d, block = 1500, 4, 2, 128, 64, 32
+    lens = [int(x) for x in np.random.default_rng(9).integers(0, lmax + 1, b)]
+    cache, q = filled(17, b, hkv, lmax, d, block, "i8"), queries(18, b, hq, d, "bf16")
+    check_decode(ctx, q, cache, lens, d ** -0.5)
+
+
+def test_decode_q8_two_calls_at_once(ctx):
+    """Two streams, a workspace each; and one after the other on two streams with the context's own scratch."""
+    d, block = 128, 64
+    cases = [(filled(19 + i, 3, 2, 4096, d, block, "e4m3"), queries(21 + i, 3, 8, d, "f16"), torch.tensor([4000 - 900 * i, 77, 3000], dtype=torch.int32, device="cuda")) for i in range(2)]
+    want = []
+    for c, q, lens in cases:
+        o = torch.zeros_like(q)
+        ctx.attn_decode_q8(q, *c.args, o, d ** -0.5, kv_len=lens)
+        ctx.sync()
+        want.append(o)
+    need, streams = ctx.attn_decode_q8_workspace_bytes(3, 8, 2, 4096, d), [torch.cuda.Stream() for _ in range(2)]
+    spaces = [torch.empty(need, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    torch.cuda.synchronize()
+    for own in (True, False):
+        got = [[torch.zeros_like(q) for _ in range(4)] for _, q, _ in cases]
+        torch.cuda.synchronize()
+        for n in range(4):
+            for i, (c, q, lens) in enumerate(cases):
+                with torch.cuda.stream(streams[i]):
+                    ctx.attn_decode_q8(q, *c.args, got[i][n], d ** -0.5, kv_len=lens, workspace=spaces[i] if own else None)
+        torch.cuda.synchronize()
+        for i in range(2):
+            for o in got[i]:
+                assert torch.equal(o, want[i]), (own, i)
+
+
+def test_cache_beyond_32_bit_offsets(ctx):
+    """Rows of a cache whose codes lie more than 2^32 bytes behind its first. Keys and values are zero but for the last block of each
+    sequence, so that the exact answer is a short sum: the zero keys have score 0 and weigh (length - block) together."""
+    b, hkv, hq, d, block, lmax = 2, 1, 4, 128, 128, (1 << 25) + 256
+    k, v = (torch.zeros(b, hkv, lmax, d, dtype=torch.float8_e4m3fn, device="cuda") for _ in range(2))
+    ks, vs = (torch.zeros(b, hkv, lmax // block, device="cuda") for _ in range(2))
+    assert k[1].data_ptr() - k.data_ptr() > 1 << 32
+    g = torch.Generator(device="cuda").manual_seed(23)
+    n, start = 100, lmax - block
+    new = [(randn(g, b * n, hkv, d) * 2).to(torch.bfloat16) for _ in range(2)]
+    held = torch.tensor([start, start], dtype=torch.int32, device="cuda")
+    ctx.kv_append_q8(*new, k, v, ks, vs, held, cu=offsets([n, n]))
+    held += n
+    q, o = (randn(g, b, hq, d) * 3).to(torch.float16), torch.zeros(b, hq, d, dtype=torch.float16, device="cuda")
+    ctx.attn_decode_q8(q, k, v, ks, vs, o, 0.3, kv_len=held)
+    ctx.sync()
+    for i in range(b):
+        kk, vv = (t[i, 0, start:start + n].double() * s[i, 0, -1].double() for t, s in ((k, ks), (v, vs)))
+        assert float((kk - new[0][i * n:(i + 1) * n, 0].double()).abs().max()) <= 2.0 ** -4 * float(kk.abs().max())
+        x = q[i].double() @ kk.T * 0.3
+        top = x.amax(-1, keepdim=True).clamp(min=0)
+        p = torch.exp(x - top)
+        p = p / (p.sum(-1, keepdim=True) + start * torch.exp(-top))
+        check(o[i], p @ vv, torch.stack([p @ vv.abs(), 2.0 ** -32 * vv.abs().sum(0).expand(hq, -1)]), torch.float16, torch.float16)
+    del k, v
 
 
 # ---- the three together ------------------------------------------------------------------------------------------------

@@ -341,7 +341,7 @@ class Context:
             raise ValueError("attn_prefill_packed: the context belongs to cuda:%d, a tensor lies elsewhere" % dev)
         code, nseq = _any_dtype_code(Q), cu_q.shape[0] - 1
         rc = self.lib.vkc_attn_prefill_packed(self.h, Q.data_ptr(), K.data_ptr(), V.data_ptr(), O.data_ptr(), nseq, Hq, Hkv, D, total_q, total_k,
-                                              self._int32(cu_q, nseq + 1, "cu_q"), self._int32(cu_k, nseq + 1, "cu_k") if cu_k is not cu_q else None,
+                                              self._int32(cu_q, nseq + 1, "cu_q"), self._int32(cu_k, nseq + 1, "cu_k"),
                                               _I64x2(q0, q1), _I64x2(k0, k1), _I64x2(v0, v1), _I64x2(o0, o1), float(scale), 1 if causal else 0, code,
                                               self._stream(stream))
         if rc:

@@ -102,6 +102,7 @@ namespace {
     struct StreamParams {
         DecQ8Params q;
         int         B, G; // sequences of this launch, query heads per kv head
+        int         runs; // partial slots of the workspace hold this many runs
         int         block_log2;
         float      *part_o;  // [runs][2][G][D]
         float      *part_ml; // [runs][2][G][2]
@@ -513,8 +514,9 @@ namespace {
         vkc_grid_dep_launch();
         const int t0 = p.line[b], t1 = p.line[b + 1], quota = p.line[p.B + 1];
         const int n = (t1 - t0) / (int) p.q.Hkv, off = t0 + hk * n;
-        const int r0 = off / quota, parts = n > 0 ? (off + n - 1) / quota - r0 + 1 : 0;
-        if (parts < 2) return;
+        if (n <= 0 || off < 0 || quota < 1) return;
+        const int r0 = off / quota, parts = (off + n - 1) / quota - r0 + 1;
+        if (parts < 2 || r0 + parts > p.runs) return; // (beyond the runs only if another call writes the same workspace: stay inside it)
         auto   row = [&](int k) { return ((int64_t) (r0 + k) * 2 + (k ? 0 : 1)) * p.G + hd; };
         float  top = -INFINITY, ls = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -611,6 +613,7 @@ namespace {
             const int64_t runs = stream_runs(B, q.Hkv, q.Lmax, D), here = stream_runs(p.B, q.Hkv, q.Lmax, D);
             int64_t       grid = ctx->sm_count < kMaxCtas ? ctx->sm_count : kMaxCtas;
             if (grid > here) grid = here;
+            p.runs    = (int) runs;
             p.part_o  = (float *) ws;
             p.part_ml = p.part_o + runs * 2 * G * D;
             p.line    = (int *) (p.part_ml + runs * 2 * G * 2);
