@@ -415,8 +415,8 @@ namespace {
         // setmaxnreg.inc blocks in hardware until the CTA's own pool holds the registers, so the control warpgroup must
         // give up at least what the softmax warpgroups take (checked here: a shortfall would hang the kernel).
         constexpr int kRegsBase    = (65536 / (threads_for(QT) * (QT == 1 ? 2 : 1))) / 8 * 8;
-        constexpr int kRegsControl = QT == 2 ? 88 : 56;
-        constexpr int kRegsSoftmax = QT == 2 ? 208 : 200;
+        constexpr int kRegsControl = QT == 2 ? (kPair ? 104 : 88) : 56;
+        constexpr int kRegsSoftmax = QT == 2 ? (kPair ? 200 : 208) : 200;
         static_assert(QT * (kRegsSoftmax - kRegsBase) <= kRegsBase - kRegsControl, "softmax warpgroups would wait forever for registers");
         (void) kThreads;
         constexpr bool kBf16  = std::is_same<T, __nv_bfloat16>::value;
