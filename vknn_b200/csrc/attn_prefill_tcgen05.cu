@@ -104,7 +104,7 @@ namespace {
         int q0, k0;   // the unit's first query row, the sequence's first key row
         int sq, sk;   // the sequence's query rows from q0 on (0: nothing to do) and its keys
         int lim0;     // keys that the unit's first row sees (each row behind it one more, when causal); may be negative
-        int n[2];     // key tiles of the query tiles
+        int n[2];     // key tiles of the query tiles: those of the unit's last row, for every tile that has rows
         int h, last;  // first query head; whether it is the CTA's last round
     };
 
@@ -243,9 +243,10 @@ namespace {
         const int m0     = (p.causal ? groups - 1 - qg : qg) * kRows; // heavy (late) query tiles first when causal
         x.q0 = q0 + m0, x.sq = qg < 0 || qg >= groups ? 0 : sq - m0;
         x.lim0 = m0 + x.sk - sq + 1;
-        x.n[1] = 0;
-#pragma unroll
-        for (int t = 0; t < QT; ++t) x.n[t] = tile_steps(sq, x.sk, p.causal, (int64_t) m0 + t * (kRows / QT / BM) * BM, x.sk);
+        // (With a causal mask the first tile of 256 rows gets a key tile or two that it does not see: all of its probabilities there are 0.)
+        const bool both = kRows == BM || x.sq > BM;
+        x.n[0] = tile_steps(sq, x.sk, p.causal, (int64_t) m0 + (kRows > BM && both ? BM : 0), x.sk);
+        x.n[1] = QT == 2 && both ? x.n[0] : 0;
         return x;
     }
     template <int QT> __device__ __forceinline__ PackedWork<QT> packed_item(const PackedUnit &x) {
@@ -415,8 +416,8 @@ namespace {
         // setmaxnreg.inc blocks in hardware until the CTA's own pool holds the registers, so the control warpgroup must
         // give up at least what the softmax warpgroups take (checked here: a shortfall would hang the kernel).
         constexpr int kRegsBase    = (65536 / (threads_for(QT) * (QT == 1 ? 2 : 1))) / 8 * 8;
-        constexpr int kRegsControl = QT == 2 ? (kPair ? 104 : 88) : 56;
-        constexpr int kRegsSoftmax = QT == 2 ? (kPair ? 200 : 208) : 200;
+        constexpr int kRegsControl = QT == 2 ? (kPacked ? 104 : 88) : 56;
+        constexpr int kRegsSoftmax = QT == 2 ? (kPacked ? 200 : 208) : 200;
         static_assert(QT * (kRegsSoftmax - kRegsBase) <= kRegsBase - kRegsControl, "softmax warpgroups would wait forever for registers");
         (void) kThreads;
         constexpr bool kBf16  = std::is_same<T, __nv_bfloat16>::value;
@@ -467,8 +468,9 @@ namespace {
                 cached[0] = x;
             }
         }
+        auto unit_at = [&](int pos) { return pos < kCached ? cached[pos] : packed_round<QT, kRows>(p, cta, p.cu_q, p.cu_k, order, ctl[2], kHeads, pos); };
         auto look_up = [&](int pos) { // packed: behind the set-up barrier only
-            if constexpr (kPacked) return packed_item<QT>(pos < kCached ? cached[pos] : packed_round<QT, kRows>(p, cta, p.cu_q, p.cu_k, order, ctl[2], kHeads, pos));
+            if constexpr (kPacked) return packed_item<QT>(unit_at(pos));
             else return work_at<QT>(p, pos, cta);
         };
         Item w_first; // the first item, looked up while the barriers are being set up
@@ -569,9 +571,8 @@ namespace {
                 // Packed: behind the sequence's last key its V tile holds the next sequence's rows, whose values may be infinite or
                 // NaN, which a probability of 0 would not silence. Steps without a key are left out; the rest of the last step's rows
                 // (fewer than 16) is set to zero.
-                auto clear_tail = [&](const Item &w, int j, int g) {
-                    const int nv = (int) (w.len - (int64_t) j * BN);
-                    ksteps       = nv >= BN ? 8 : (nv + 15) / 16;
+                auto clear_tail = [&](int nv, int g) { // nv: keys of the sequence from the tile's first on
+                    ksteps = nv >= BN ? 8 : (nv + 15) / 16;
                     if (nv >= BN || nv % 16 == 0) return;
                     const uint32_t v = sV + (uint32_t) (g & 1) * L::KV_BYTES;
                     const int      rows = ksteps * 16 - nv;
@@ -587,62 +588,66 @@ namespace {
 #pragma unroll
                 for (int t = 0; t < kQTiles; ++t) cs[t] = 0;
                 Item w = w_first;
-                if constexpr (kPacked) w = look_up(0);
-              if constexpr (kPair) {
-                // Both query tiles have the same key tiles in every item, so the items form one stream of steps: behind P.V_t of an item's last
-                // key tile comes Q.K_t of the next item's first, while the softmax warps of tile t still store the rows. The two
-                // tiles stay half a step apart across items.
-                int  pos = 0;
-                auto to_work = [&](Item &x) { // on to the next item that has keys, if there is one
-                    while (x.valid && x.n_max == 0) {
-                        x = next_work(x, pos);
-                        if (x.valid) pos += x.adv;
+              if constexpr (kPacked) {
+                // All query tiles of an item take the same number of key tiles (PackedUnit::n; a tile without rows takes none), so the items form
+                // one stream of steps: behind P.V_t of an item's last key tile comes Q.K_t of the next item's first, while the
+                // softmax warps of tile t still store the rows. The two tiles stay half a step apart across items.
+                struct Steps { // what the issuer needs of an item
+                    int n, len, both; // key tiles, keys of the sequence, whether the second query tile has rows
+                };
+                int  pos  = 0; // the round after the item at hand
+                auto next = [&](Steps &x) { // the next round that has keys (n == 0: there is none)
+                    for (;;) {
+                        const PackedUnit u = unit_at(pos);
+                        x.n = u.sq > 0 ? u.n[0] : 0, x.len = u.sk, x.both = QT == 2 && u.n[QT - 1] > 0;
+                        if (u.sq <= 0 || u.last) pos = INT32_MAX;
+                        else ++pos;
+                        if (x.n > 0 || pos == INT32_MAX) return;
                     }
                 };
-                if (w.valid) pos += w.adv;
-                to_work(w);
-                if (w.valid) {
+                Steps s;
+                next(s);
+                if (s.n > 0) {
                     ok = wait(bKF, 0u) && wait(bQ, 0u);
                     if (ok) {
                         ptx::tc_fence_after();
                         issue_qk(0, 0);
-                        issue_qk(1, 0);
+                        if (s.both) issue_qk(QT - 1, 0);
                         if (leader) {
                             ptx::tc_commit(bar(bKE));
-                            if (w.n_max == 1) ptx::tc_commit(bar(bQE));
+                            if (s.n == 1) ptx::tc_commit(bar(bQE));
                         }
                     }
                 }
-                while (ok && w.valid) {
-                    const int n_max = w.n_max;
-                    Item      nw; // the item behind this one
-                    nw.valid = false;
-                    for (int j = 0; j < n_max && ok; ++j) {
-                        const int  g = g0 + j, vs = g & 1;
-                        const bool last = j + 1 == n_max;
-                        if (last) {
-                            nw = next_work(w, pos);
-                            if (nw.valid) pos += nw.adv;
-                            to_work(nw);
-                        }
-                        const bool more = !last || nw.valid; // another Q.K^T follows
+                int g = 0; // key tiles so far
+                while (ok && s.n > 0) {
+                    Steps ns; // the item behind this one
+                    ns.n = 0;
+                    for (int j = 0; j < s.n && ok; ++j, ++g) {
+                        const int  vs   = g & 1;
+                        const bool last = j + 1 == s.n;
+                        if (last && pos != INT32_MAX) next(ns);
+                        const bool more = !last || ns.n > 0; // another Q.K^T follows
                         ok = wait(bVF + vs, (uint32_t) ((g >> 1) & 1));
                         if (!ok) break;
-                        clear_tail(w, j, g);
+                        clear_tail(s.len - j * BN, g);
 #pragma unroll
-                        for (int t = 0; t < 2 && ok; ++t) {
-                            const uint32_t pp = (uint32_t) (g & 1);
+                        for (int t = 0; t < kQTiles && ok; ++t) {
+                            if (t == 0 || s.both) {
+                                const uint32_t pp = (uint32_t) (cs[t] & 1);
 #pragma unroll
-                            for (int part = 0; part < kPParts && ok; ++part) {
-                                ok = wait(bPF + kPParts * t + part, pp);
-                                if (ok) {
-                                    ptx::tc_fence_after();
-                                    issue_pv(t, j, g, part);
+                                for (int part = 0; part < kPParts && ok; ++part) {
+                                    ok = wait(bPF + kPParts * t + part, pp);
+                                    if (ok) {
+                                        ptx::tc_fence_after();
+                                        issue_pv(t, j, g, part);
+                                    }
                                 }
+                                if (!ok) break;
+                                ++cs[t];
+                                if (last && leader) ptx::tc_commit(bar(bOF + t)); // O_t complete
                             }
-                            if (!ok) break;
-                            if (last && leader) ptx::tc_commit(bar(bOF + t)); // O_t complete
-                            if (more) {
+                            if (more && (t == 0 || (last ? ns.both : s.both))) {
                                 ok = wait(bKF + ((g + 1) & 1), (uint32_t) (((g + 1) >> 1) & 1)) && (!last || wait(bQ, (uint32_t) ((cq + 1) & 1)));
                                 if (!ok) break;
                                 ptx::tc_fence_after();
@@ -655,13 +660,12 @@ namespace {
                             if (more) {
                                 ptx::tc_commit(bar(bKE + ((g + 1) & 1)));
                                 // the last Q.K^T MMAs of their item are issued: Q may be replaced
-                                if (last ? nw.n_max == 1 : j + 2 == n_max) ptx::tc_commit(bar(bQE));
+                                if (last ? ns.n == 1 : j + 2 == s.n) ptx::tc_commit(bar(bQE));
                             }
                         }
                     }
-                    g0 += n_max;
                     ++cq;
-                    w = nw;
+                    s = ns;
                 }
               } else {
                 for (int pos = 0; ok; w = next_work(w, pos)) {
@@ -684,9 +688,6 @@ namespace {
                     for (int j = 0; j < n_max && ok; ++j) {
                         const int g = g0 + j, vs = g & 1;
                         ok = wait(bVF + vs, (uint32_t) ((g >> 1) & 1));
-                        if constexpr (kPacked) {
-                            if (ok) clear_tail(w, j, g);
-                        }
                         const bool more = j + 1 < n_max;
 #pragma unroll
                         for (int t = 0; t < kQTiles && ok; ++t) {
