@@ -144,7 +144,7 @@ VKC_API int vkc_attn_prefill_items(int sm_count, int64_t B, int64_t Hq, int64_t 
  * padding between them. Sequence b owns the rows [cu_q[b], cu_q[b+1]) of Q and O and the rows [cu_k[b], cu_k[b+1]) of K and V;
  * a row attends to the keys of its own sequence only. It has no counterpart in the reference, which runs one batch shape per
  * graph (the arithmetic is vkc_attn_prefill's: ops/matmul.cpp:14-116, ops/softmax.cpp:9-47).
- *   Q/O [total_q,Hq,D], K/V [total_k,Hkv,D]; *_strides = element strides {token, head} with D contiguous, or NULL for dense
+ *   Q/O [total_q,Hq,D], K/V [total_k,Hkv,D]; *_strides = element strides {token, head} with D contiguous, {0, 0} for dense
  *   (views of one packed projection [tokens, Hq+2*Hkv, D] are fine); query head h uses kv head h / (Hq/Hkv);
  *   cu_q, cu_k: device int32 [nseq+1], non-decreasing; cu_k NULL = cu_q (then total_k must equal total_q). Values outside
  *   [0, total] are clamped to it. Rows that belong to no sequence (behind cu_q[nseq]) are left as they were;
@@ -153,10 +153,16 @@ VKC_API int vkc_attn_prefill_items(int sm_count, int64_t B, int64_t Hq, int64_t 
  *   not even infinities or NaN; within a sequence a key that the causal mask hides from a row may, if its V is not finite.
  *   f32, f16, bf16; D <= 256. The tensor-core kernel runs 16-bit storage with D in {64,128}, strides and bases that are
  *   multiples of 16 bytes and scale > 0; other shapes run the SIMT kernel. ---- */
-VKC_API int vkc_attn_prefill_packed(vkc_ctx *ctx, const void *Q, const void *K, const void *V, void *O, int64_t nseq, int64_t Hq, int64_t Hkv,
-                                    int64_t D, int64_t total_q, int64_t total_k, const int32_t *cu_q, const int32_t *cu_k,
-                                    const int64_t *q_strides, const int64_t *k_strides, const int64_t *v_strides, const int64_t *o_strides,
-                                    float scale, int causal, int dtype, vkc_stream stream);
+typedef struct vkc_attn_prefill_packed_args {
+    const void    *Q, *K, *V;
+    void          *O;
+    int64_t        nseq, Hq, Hkv, D, total_q, total_k;
+    const int32_t *cu_q, *cu_k;
+    int64_t        q_strides[2], k_strides[2], v_strides[2], o_strides[2];
+    float          scale;
+    int32_t        causal, dtype;
+} vkc_attn_prefill_packed_args;
+VKC_API int vkc_attn_prefill_packed(vkc_ctx *ctx, const vkc_attn_prefill_packed_args *args, vkc_stream stream);
 
 /* ---- prefill attention with its output fanned out to several GPUs (the all-gather at the attention-output boundary of a
  * head-sharded encoder, done by the kernel that produces the tiles instead of a collective after it). The reference has no
@@ -261,7 +267,7 @@ VKC_API int    vkc_attn_decode_noalloc(vkc_ctx *ctx, const void *Q, const void *
  *   The cache: Kc/Vc [B,Hkv,Lmax,D] of cache_dtype (VKC_E4M3 or VKC_I8) and k_scale/v_scale fp32 [B,Hkv,Lmax/block]: one scale
  *   per `block` consecutive tokens of one head; a stored value stands for code * scale. block is 32, 64 or 128, Lmax a multiple
  *   of it, D 64, 128 or 256; Kc, Vc 16-byte aligned.
- *   The new rows: K/V [total,Hkv,D], `dtype` f32, f16 or bf16, element strides {token, head} with D contiguous (NULL = dense).
+ *   The new rows: K/V [total,Hkv,D], `dtype` f32, f16 or bf16, element strides {token, head} with D contiguous ({0, 0} = dense).
  *   cu: device int32 [B+1], non-decreasing, clamped to [0, total]: sequence b brings the rows [cu[b], cu[b+1]); NULL: every
  *   sequence brings one row (total must equal B). kv_len: device int32 [B], the tokens each sequence holds already (NULL =
  *   none); its rows go to the positions kv_len[b], kv_len[b]+1, ... . Rows at or behind Lmax are dropped, a sequence with a
@@ -273,9 +279,16 @@ VKC_API int    vkc_attn_decode_noalloc(vkc_ctx *ctx, const void *Q, const void *
  *   whose scales are powers of two, this only rounds codes that reach the subnormal range). A block that receives an infinity or NaN gets the scale
  *   NaN and codes 0 for the new tokens, so that attention over it answers NaN; it stays so until it is written from its first
  *   token on. ---- */
-VKC_API int vkc_kv_append_q8(vkc_ctx *ctx, const void *K, const void *V, void *Kc, void *Vc, float *k_scale, float *v_scale, int64_t B,
-                             int64_t Hkv, int64_t Lmax, int64_t D, int64_t block, int64_t total, const int32_t *cu, const int32_t *kv_len,
-                             const int64_t *k_strides, const int64_t *v_strides, int dtype, int cache_dtype, vkc_stream stream);
+typedef struct vkc_kv_append_q8_args {
+    const void    *K, *V;
+    void          *Kc, *Vc;
+    float         *k_scale, *v_scale;
+    int64_t        B, Hkv, Lmax, D, block, total;
+    const int32_t *cu, *kv_len;
+    int64_t        k_strides[2], v_strides[2];
+    int32_t        dtype, cache_dtype;
+} vkc_kv_append_q8_args;
+VKC_API int vkc_kv_append_q8(vkc_ctx *ctx, const vkc_kv_append_q8_args *args, vkc_stream stream);
 
 /* ---- K9: single-query (decode) attention over the 8-bit cache of vkc_kv_append_q8: vkc_attn_decode with
  * K = Kc * k_scale, V = Vc * v_scale (block scales), half the cache bytes.
@@ -287,9 +300,18 @@ VKC_API int vkc_kv_append_q8(vkc_ctx *ctx, const void *K, const void *V, void *K
  *   the same time need workspaces of their own, and so do two captured graphs that may be replayed at the same time; calls
  *   captured without a workspace share the context's. ---- */
 VKC_API size_t vkc_attn_decode_q8_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Lmax, int64_t D);
-VKC_API int    vkc_attn_decode_q8(vkc_ctx *ctx, const void *Q, const void *Kc, const void *Vc, const float *k_scale, const float *v_scale, void *O,
-                                  int64_t B, int64_t Hq, int64_t Hkv, int64_t Lmax, int64_t D, int64_t block, const int32_t *kv_len, float scale,
-                                  void *workspace, size_t workspace_bytes, int dtype, int cache_dtype, vkc_stream stream);
+typedef struct vkc_attn_decode_q8_args {
+    const void    *Q, *Kc, *Vc;
+    const float   *k_scale, *v_scale;
+    void          *O;
+    int64_t        B, Hq, Hkv, Lmax, D, block;
+    const int32_t *kv_len;
+    void          *workspace;
+    size_t         workspace_bytes;
+    float          scale;
+    int32_t        dtype, cache_dtype;
+} vkc_attn_decode_q8_args;
+VKC_API int vkc_attn_decode_q8(vkc_ctx *ctx, const vkc_attn_decode_q8_args *args, vkc_stream stream);
 
 /* ---- K4: LayerNorm over the trailing `norm` elements. Reference: LayerNormCpu::run
  * src/backend/cpu/ops/layernorm.cpp:12-75 (oracle), shaders/flat_layernorm.comp:8-50 + LayerNormOp

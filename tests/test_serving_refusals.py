@@ -1,19 +1,28 @@
 """CPU tests of the serving operators' boundary: what the C entry points refuse without a context, and the argument checks of
 the Python binding, run against a stand-in for the library (nothing is launched)."""
+import ctypes as C
+import os
+import shutil
+import subprocess
+
 import pytest
 import torch
 
 import vknn_b200
+from vknn_b200 import capi
 
 
 class Recorder:
-    """Stands in for the loaded library: notes the calls and succeeds."""
+    """Stands in for the loaded library: notes the calls and their argument structs, and succeeds."""
+
+    STRUCTS = {"vkc_attn_prefill_packed": capi.PACKED_ARGS, "vkc_kv_append_q8": capi.APPEND_ARGS, "vkc_attn_decode_q8": capi.DECODE_Q8_ARGS}
 
     def __init__(self):
         self.calls = []
 
     def __getattr__(self, name):
-        return lambda *a: self.calls.append((name, a)) or 0
+        s = self.STRUCTS[name]
+        return lambda h, at, stream: self.calls.append((name, s.unpack(C.string_at(at, s.size)))) or 0
 
 
 @pytest.fixture
@@ -21,6 +30,7 @@ def fake():
     c = vknn_b200.Context.__new__(vknn_b200.Context)
     c.lib, c.h, c.device = Recorder(), None, -1  # -1 is what CPU tensors answer for their device
     c._stream = lambda stream: None
+    c._make_args()
     return c
 
 
@@ -34,18 +44,41 @@ def cache(b=2, hkv=2, lmax=64, d=64, block=32, dt=torch.float8_e4m3fn):
 
 def test_null_context_is_refused():
     lib = vknn_b200.load_library()
-    assert lib.vkc_attn_prefill_packed(None, None, None, None, None, 1, 1, 1, 64, 1, 1, None, None, None, None, None, None, 1.0, 1, 1, None) == -1
-    assert lib.vkc_kv_append_q8(None, None, None, None, None, None, None, 1, 1, 32, 64, 32, 1, None, None, None, None, 1, 4, None) == -1
-    assert lib.vkc_attn_decode_q8(None, None, None, None, None, None, None, 1, 1, 1, 32, 64, 32, None, 1.0, None, 0, 1, 4, None) == -1
+    args = C.create_string_buffer(256)
+    for f in (lib.vkc_attn_prefill_packed, lib.vkc_kv_append_q8, lib.vkc_attn_decode_q8):
+        assert f(None, C.addressof(args), None) == -1 and f(None, None, None) == -1
     assert lib.vkc_attn_decode_q8_workspace_bytes(0, 1, 1, 32, 64) == 0 and lib.vkc_attn_decode_q8_workspace_bytes(2, 8, 2, 4096, 128) > 0
+
+
+def test_argument_structs_have_the_layout_of_the_c_compiler(tmp_path):
+    if not shutil.which("gcc"):
+        pytest.skip("no C compiler")
+    inc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    # every field gets its own number (the floats and ints too), packed by Python and read by C
+    fields = {"attn_prefill_packed": (capi.PACKED_ARGS, "Q K V O nseq Hq Hkv D total_q total_k cu_q cu_k q_strides[0] q_strides[1] k_strides[0] k_strides[1] "
+                                      "v_strides[0] v_strides[1] o_strides[0] o_strides[1] scale causal dtype"),
+              "kv_append_q8": (capi.APPEND_ARGS, "K V Kc Vc k_scale v_scale B Hkv Lmax D block total cu kv_len k_strides[0] k_strides[1] v_strides[0] v_strides[1] "
+                               "dtype cache_dtype"),
+              "attn_decode_q8": (capi.DECODE_Q8_ARGS, "Q Kc Vc k_scale v_scale O B Hq Hkv Lmax D block kv_len workspace workspace_bytes scale dtype cache_dtype")}
+    body = ""
+    for name, (s, text) in fields.items():
+        names = text.split()
+        (tmp_path / name).write_bytes(s.pack(*(float(i + 1) if n == "scale" else i + 1 for i, n in enumerate(names))) + bytes(16))
+        body += ('{ vkc_%s_args a; FILE *f = fopen("%s", "rb"); if (!f || fread(&a, 1, sizeof a, f) != sizeof a) return 1; fclose(f); long long v[] = {%s}; '
+                 'for (int i = 0; i < %d; ++i) if (v[i] != i + 1) { printf("%s %%d %%lld\\n", i, v[i]); return 2; } }\n'
+                 % (name, tmp_path / name, ", ".join("(long long)%s a.%s" % ("" if n == "scale" else "(intptr_t)", n) for n in names), len(names), name))
+    src, exe = tmp_path / "t.c", tmp_path / "t"
+    src.write_text('#include <stdio.h>\n#include <stdint.h>\n#include "vknn_cuda.h"\nint main(void) {\n%s return 0; }\n' % body)
+    subprocess.check_call(["gcc", "-std=c99", "-Wall", "-Werror", "-I", inc, str(src), "-o", str(exe)])
+    assert subprocess.run([str(exe)], capture_output=True, text=True).stdout == "" and subprocess.call([str(exe)]) == 0
 
 
 def test_packed_arguments_reach_the_library_as_given(fake):
     qkv, o, cu = z(10, 8, 64), z(10, 4, 64), z(3, dt=torch.int32)
     fake.attn_prefill_packed(qkv[:, :4], qkv[:, 4:6], qkv[:, 6:], o, 0.5, cu, causal=False)
     (name, a), = fake.lib.calls
-    assert name == "vkc_attn_prefill_packed" and a[5:11] == (2, 4, 2, 64, 10, 10) and a[11] == cu.data_ptr() and a[12] is None
-    assert [list(s) for s in a[13:17]] == [[512, 64]] * 3 + [[256, 64]] and a[17:20] == (0.5, 0, vknn_b200.F16)
+    assert name == "vkc_attn_prefill_packed" and a[4:10] == (2, 4, 2, 64, 10, 10) and a[10:12] == (cu.data_ptr(), 0)
+    assert a[12:20] == (512, 64) * 3 + (256, 64) and a[20:] == (0.5, 0, vknn_b200.F16)
 
 
 def test_cache_arguments_reach_the_library_as_given(fake):
@@ -54,8 +87,8 @@ def test_cache_arguments_reach_the_library_as_given(fake):
     fake.kv_append_q8(z(3, 2, 64), z(3, 2, 64), *c, lens)
     fake.attn_decode_q8(z(3, 6, 64), *c, z(3, 6, 64), 0.25, kv_len=lens)
     (n1, a), (n2, b) = fake.lib.calls
-    assert n1 == "vkc_kv_append_q8" and a[7:13] == (3, 2, 128, 64, 32, 3) and a[13] is None and a[14] == lens.data_ptr() and a[17:19] == (vknn_b200.F16, vknn_b200.I8)
-    assert n2 == "vkc_attn_decode_q8" and b[7:13] == (3, 6, 2, 128, 64, 32) and b[15:19] == (None, 0, vknn_b200.F16, vknn_b200.I8)
+    assert n1 == "vkc_kv_append_q8" and a[6:14] == (3, 2, 128, 64, 32, 3, 0, lens.data_ptr()) and a[14:] == (128, 64, 128, 64, vknn_b200.F16, vknn_b200.I8)
+    assert n2 == "vkc_attn_decode_q8" and b[6:] == (3, 6, 2, 128, 64, 32, lens.data_ptr(), 0, 0, 0.25, vknn_b200.F16, vknn_b200.I8)
 
 
 def test_packed_refusals(fake):

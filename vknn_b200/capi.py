@@ -5,6 +5,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 import re
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 HEADER = os.path.join(os.path.dirname(HERE), "include", "vknn_cuda.h")
@@ -86,11 +87,11 @@ def load_library():
     L.vkc_attn_decode_noalloc_max_bytes.argtypes = []
     L.vkc_attn_decode_noalloc_max_bytes.restype = sz
     L.vkc_attn_decode_noalloc.argtypes = [vp, vp, vp, vp, vp] + [i64] * 5 + [vp, f32, i32, vp]
-    L.vkc_attn_prefill_packed.argtypes = [vp, vp, vp, vp, vp] + [i64] * 6 + [vp, vp, vp, vp, vp, vp, f32, i32, i32, vp]
-    L.vkc_kv_append_q8.argtypes = [vp, vp, vp, vp, vp, vp, vp] + [i64] * 6 + [vp, vp, vp, vp, i32, i32, vp]
+    L.vkc_attn_prefill_packed.argtypes = [vp, vp, vp]
+    L.vkc_kv_append_q8.argtypes = [vp, vp, vp]
     L.vkc_attn_decode_q8_workspace_bytes.argtypes = [i64] * 5
     L.vkc_attn_decode_q8_workspace_bytes.restype = sz
-    L.vkc_attn_decode_q8.argtypes = [vp, vp, vp, vp, vp, vp, vp] + [i64] * 6 + [vp, f32, vp, sz, i32, i32, vp]
+    L.vkc_attn_decode_q8.argtypes = [vp, vp, vp]
     L.vkc_layernorm.argtypes = [vp, vp, vp, vp, vp, i64, i64, f32, i32, vp]
     L.vkc_pointwise.argtypes = [vp, vp, vp, vp, i32, i32, vp, vp, i32, vp, vp, i32, vp]
     L.vkc_softmax.argtypes = [vp, vp, vp, i64, i64, i32, vp]
@@ -118,7 +119,7 @@ def _dtype_code(t):
 
 
 # torch dtype -> code; this and the two types below are filled by the first call (torch is imported late)
-_code_of, _torch_float32, _torch_int32, _I64x2 = {}, [], [], C.c_int64 * 2
+_code_of, _torch_float32, _torch_int32 = {}, [], []
 
 
 def _any_dtype_code(t):
@@ -148,6 +149,12 @@ class Gate(C.Structure):
     """Mirror of struct vkc_gate (include/vknn_cuda.h)."""
     _fields_ = [("flags", C.c_void_p), ("n", C.c_int), ("state", C.c_void_p)]
 
+
+# The argument structs of include/vknn_cuda.h. They are filled by struct.pack_into and passed by address: one conversion for all
+# fields, where an argument list of that length costs ctypes 2.5 us a call.
+PACKED_ARGS = struct.Struct("@4P6q2P8qf2i")   # vkc_attn_prefill_packed_args
+APPEND_ARGS = struct.Struct("@6P6q2P4q2i")    # vkc_kv_append_q8_args
+DECODE_Q8_ARGS = struct.Struct("@6P6q2PNf2i")  # vkc_attn_decode_q8_args
 
 PEER_HANDLE_BYTES = 64
 
@@ -218,6 +225,12 @@ class Context:
             raise VkcError(rc, "vkc_ctx_create(%d) failed (no usable sm_100 device?)" % device)
         self.h = h
         self.device = int(device)
+        self._make_args()
+
+    def _make_args(self):
+        """Room for one argument struct (a context is driven by one thread at a time, and no call keeps it)."""
+        self._args = C.create_string_buffer(256)
+        self._args_at = C.addressof(self._args)
 
     def close(self):
         if getattr(self, "h", None):
@@ -317,9 +330,9 @@ class Context:
                                               _dtype_code(Q), self._stream(stream)))
 
     def _int32(self, t, n, what):
-        """The pointer of an int32 tensor of n elements on this device, or None."""
+        """The pointer of an int32 tensor of n elements on this device, or 0 for None."""
         if t is None:
-            return None
+            return 0
         if t.dtype is not _torch_int32[0] or t.shape != (n,) or t.stride(0) != 1 or t.get_device() != self.device:
             raise ValueError("%s must be a contiguous int32 tensor of %d elements on cuda:%d" % (what, n, self.device))
         return t.data_ptr()
@@ -340,10 +353,10 @@ class Context:
         if Q.get_device() != dev or K.get_device() != dev or V.get_device() != dev or O.get_device() != dev:
             raise ValueError("attn_prefill_packed: the context belongs to cuda:%d, a tensor lies elsewhere" % dev)
         code, nseq = _any_dtype_code(Q), cu_q.shape[0] - 1
-        rc = self.lib.vkc_attn_prefill_packed(self.h, Q.data_ptr(), K.data_ptr(), V.data_ptr(), O.data_ptr(), nseq, Hq, Hkv, D, total_q, total_k,
-                                              self._int32(cu_q, nseq + 1, "cu_q"), self._int32(cu_k, nseq + 1, "cu_k"),
-                                              _I64x2(q0, q1), _I64x2(k0, k1), _I64x2(v0, v1), _I64x2(o0, o1), float(scale), 1 if causal else 0, code,
-                                              self._stream(stream))
+        PACKED_ARGS.pack_into(self._args, 0, Q.data_ptr(), K.data_ptr(), V.data_ptr(), O.data_ptr(), nseq, Hq, Hkv, D, total_q, total_k,
+                              self._int32(cu_q, nseq + 1, "cu_q"), self._int32(cu_k, nseq + 1, "cu_k"), q0, q1, k0, k1, v0, v1, o0, o1, scale,
+                              1 if causal else 0, code)
+        rc = self.lib.vkc_attn_prefill_packed(self.h, self._args_at, self._stream(stream))
         if rc:
             self._check(rc)
 
@@ -371,9 +384,9 @@ class Context:
         (k0, k1, k2), (v0, v1, v2), dev = K.stride(), V.stride(), self.device
         if heads != Hkv or dim != D or V.shape != shape or V.dtype is not K.dtype or k2 != 1 or v2 != 1 or K.get_device() != dev or V.get_device() != dev:
             raise ValueError("kv_append_q8: K and V must be [total,%d,%d] of one type on cuda:%d with the last dimension contiguous" % (Hkv, D, dev))
-        rc = self.lib.vkc_kv_append_q8(self.h, K.data_ptr(), V.data_ptr(), Kc.data_ptr(), Vc.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), B, Hkv, Lmax, D,
-                                       block, total, self._int32(cu, B + 1, "cu"), self._int32(kv_len, B, "kv_len"), _I64x2(k0, k1), _I64x2(v0, v1),
-                                       _any_dtype_code(K), code, self._stream(stream))
+        APPEND_ARGS.pack_into(self._args, 0, K.data_ptr(), V.data_ptr(), Kc.data_ptr(), Vc.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), B, Hkv, Lmax, D,
+                              block, total, self._int32(cu, B + 1, "cu"), self._int32(kv_len, B, "kv_len"), k0, k1, v0, v1, _any_dtype_code(K), code)
+        rc = self.lib.vkc_kv_append_q8(self.h, self._args_at, self._stream(stream))
         if rc:
             self._check(rc)
 
@@ -387,10 +400,10 @@ class Context:
         if (len(shape) != 3 or shape[0] != B or shape[2] != D or O.shape != shape or O.dtype is not Q.dtype or not (Q.is_contiguous() and O.is_contiguous()) or
                 Q.get_device() != dev or O.get_device() != dev):
             raise ValueError("attn_decode_q8: Q and O must be contiguous [%d,Hq,%d] of one type on cuda:%d" % (B, D, dev))
-        rc = self.lib.vkc_attn_decode_q8(self.h, Q.data_ptr(), Kc.data_ptr(), Vc.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), O.data_ptr(), B, shape[1], Hkv,
-                                         Lmax, D, block, self._int32(kv_len, B, "kv_len"), float(scale), workspace.data_ptr() if workspace is not None else None,
-                                         workspace.numel() * workspace.element_size() if workspace is not None else 0, _any_dtype_code(Q), code,
-                                         self._stream(stream))
+        DECODE_Q8_ARGS.pack_into(self._args, 0, Q.data_ptr(), Kc.data_ptr(), Vc.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), O.data_ptr(), B, shape[1], Hkv,
+                                 Lmax, D, block, self._int32(kv_len, B, "kv_len"), workspace.data_ptr() if workspace is not None else 0,
+                                 workspace.numel() * workspace.element_size() if workspace is not None else 0, scale, _any_dtype_code(Q), code)
+        rc = self.lib.vkc_attn_decode_q8(self.h, self._args_at, self._stream(stream))
         if rc:
             self._check(rc)
 

@@ -648,10 +648,11 @@ extern "C" size_t vkc_attn_decode_q8_workspace_bytes(int64_t B, int64_t Hq, int6
     return stream_ws(B, Hq, Hkv, Lmax, D);
 }
 
-extern "C" int vkc_attn_decode_q8(vkc_ctx *ctx, const void *Q, const void *Kc, const void *Vc, const float *k_scale, const float *v_scale, void *O,
-                                  int64_t B, int64_t Hq, int64_t Hkv, int64_t Lmax, int64_t D, int64_t block, const int32_t *kv_len, float scale,
-                                  void *workspace, size_t workspace_bytes, int dtype, int cache_dtype, vkc_stream stream) {
+extern "C" int vkc_attn_decode_q8(vkc_ctx *ctx, const vkc_attn_decode_q8_args *args, vkc_stream stream) {
     if (!ctx) return VKC_ERR_INVALID;
+    VKC_REQUIRE(ctx, args, "attn_decode_q8: null arguments");
+    const auto [Q, Kc, Vc, k_scale, v_scale, O, B, Hq, Hkv, Lmax, D, block, kv_len, given, workspace_bytes, scale, dtype, cache_dtype] = *args;
+    void *workspace = given;
     VKC_REQUIRE(ctx, B >= 0 && Hq >= 1 && Hkv >= 1 && Lmax >= 1 && D >= 1, "attn_decode_q8: bad extents");
     VKC_REQUIRE(ctx, Hq % Hkv == 0, "attn_decode_q8: Hq=%lld is not a multiple of Hkv=%lld", (long long) Hq, (long long) Hkv);
     if (dtype != VKC_F16 && dtype != VKC_BF16) return vkc_fail(ctx, VKC_ERR_UNSUPPORTED, "attn_decode_q8: Q and O must be f16 or bf16");

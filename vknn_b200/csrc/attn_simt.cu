@@ -209,11 +209,10 @@ extern "C" int vkc_attn_prefill_fanout(vkc_ctx *ctx, const void *Q, const void *
                                     vkc_pick_stream(ctx, stream));
 }
 
-extern "C" int vkc_attn_prefill_packed(vkc_ctx *ctx, const void *Q, const void *K, const void *V, void *O, int64_t nseq, int64_t Hq, int64_t Hkv,
-                                       int64_t D, int64_t total_q, int64_t total_k, const int32_t *cu_q, const int32_t *cu_k,
-                                       const int64_t *q_strides, const int64_t *k_strides, const int64_t *v_strides, const int64_t *o_strides,
-                                       float scale, int causal, int dtype, vkc_stream stream) {
+extern "C" int vkc_attn_prefill_packed(vkc_ctx *ctx, const vkc_attn_prefill_packed_args *args, vkc_stream stream) {
     if (!ctx) return VKC_ERR_INVALID;
+    VKC_REQUIRE(ctx, args, "attn_prefill_packed: null arguments");
+    const auto [Q, K, V, O, nseq, Hq, Hkv, D, total_q, total_k, cu_q, cu_k, q_strides, k_strides, v_strides, o_strides, scale, causal, dtype] = *args;
     VKC_REQUIRE(ctx, nseq >= 0 && Hq >= 1 && Hkv >= 1 && D >= 1 && total_q >= 0 && total_k >= 0, "attn_prefill_packed: bad extents");
     VKC_REQUIRE(ctx, Hq % Hkv == 0, "attn_prefill_packed: Hq=%lld is not a multiple of Hkv=%lld", (long long) Hq, (long long) Hkv);
     VKC_REQUIRE(ctx, dtype == VKC_F32 || dtype == VKC_F16 || dtype == VKC_BF16, "attn_prefill_packed: bad dtype %d", dtype);
@@ -232,7 +231,7 @@ extern "C" int vkc_attn_prefill_packed(vkc_ctx *ctx, const void *Q, const void *
     p.B = nseq, p.Hq = Hq, p.Hkv = Hkv, p.Sq = total_q, p.Skv = total_k, p.D = D;
     const int64_t dq[2] = {Hq * D, D}, dk[2] = {Hkv * D, D}; // {token, head}
     auto          set   = [](int64_t(&to)[3], const int64_t *given, const int64_t *dense) {
-        const int64_t *s = given ? given : dense;
+        const int64_t *s = given[0] || given[1] ? given : dense;
         to[0] = 0, to[1] = s[1], to[2] = s[0];
     };
     set(p.qs, q_strides, dq), set(p.ks, k_strides, dk), set(p.vs, v_strides, dk), set(p.os, o_strides, dq);

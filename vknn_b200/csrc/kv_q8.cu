@@ -155,10 +155,10 @@ namespace {
 
 } // namespace
 
-extern "C" int vkc_kv_append_q8(vkc_ctx *ctx, const void *K, const void *V, void *Kc, void *Vc, float *k_scale, float *v_scale, int64_t B,
-                                int64_t Hkv, int64_t Lmax, int64_t D, int64_t block, int64_t total, const int32_t *cu, const int32_t *kv_len,
-                                const int64_t *k_strides, const int64_t *v_strides, int dtype, int cache_dtype, vkc_stream stream) {
+extern "C" int vkc_kv_append_q8(vkc_ctx *ctx, const vkc_kv_append_q8_args *args, vkc_stream stream) {
     if (!ctx) return VKC_ERR_INVALID;
+    VKC_REQUIRE(ctx, args, "kv_append_q8: null arguments");
+    const auto [K, V, Kc, Vc, k_scale, v_scale, B, Hkv, Lmax, D, block, total, cu, kv_len, k_strides, v_strides, dtype, cache_dtype] = *args;
     VKC_REQUIRE(ctx, B >= 0 && Hkv >= 1 && Lmax >= 1 && D >= 1 && total >= 0, "kv_append_q8: bad extents");
     VKC_REQUIRE(ctx, dtype == VKC_F32 || dtype == VKC_F16 || dtype == VKC_BF16, "kv_append_q8: bad dtype %d", dtype);
     if (int rc = vkc_q8_check(ctx, "kv_append_q8", B, Hkv, Lmax, D, block, cache_dtype)) return rc;
@@ -173,7 +173,7 @@ extern "C" int vkc_kv_append_q8(vkc_ctx *ctx, const void *K, const void *V, void
     p.X[0] = K, p.X[1] = V;
     p.codes[0] = (uint8_t *) Kc, p.codes[1] = (uint8_t *) Vc;
     p.scales[0] = k_scale, p.scales[1] = v_scale;
-    const int64_t dense[2] = {Hkv * D, D}, *str[2] = {k_strides ? k_strides : dense, v_strides ? v_strides : dense};
+    const int64_t dense[2] = {Hkv * D, D}, *str[2] = {k_strides[0] || k_strides[1] ? k_strides : dense, v_strides[0] || v_strides[1] ? v_strides : dense};
     const int64_t per16    = 16 / (int64_t) vkc_dtype_size(dtype);
     p.vec_ok               = !(((uintptr_t) K | (uintptr_t) V) & 15);
     for (int w = 0; w < 2; ++w)
