@@ -266,6 +266,20 @@ def test_packed_many_sequences(ctx, hq, hkv, d, nseq, hi):
     assert bool(((o.double() - w).abs() <= tol).all())
 
 
+def test_packed_keys_shared_by_a_broadcast_stride(ctx):
+    """One kv head expanded over all of them, and one value row for all tokens (strides of 0): the same as the copies."""
+    lq, h, d = [60, 131], 4, 64
+    q, k, v = packed_case(15, lq, lq, h, 1, d, torch.float16)
+    ke, ve = k.expand(-1, h, -1), v[:1].expand(sum(lq), h, d).contiguous()[:, :1].expand(-1, h, -1)
+    o, want = torch.zeros_like(q), torch.zeros_like(q)
+    ctx.attn_prefill_packed(q, ke, ve, o, d ** -0.5, offsets(lq))
+    ctx.attn_prefill_packed(q, ke.contiguous(), ve.contiguous(), want, d ** -0.5, offsets(lq))
+    ctx.sync()
+    ref, a = attention64(q[:60].double(), ke[:60].double(), ve[:60].double(), d ** -0.5, True)
+    check(o[:60], ref, a, torch.float16, torch.float16)
+    check(want[:60], ref, a, torch.float16, torch.float16)
+
+
 def test_packed_same_offsets_for_queries_and_a_longer_key_buffer(ctx):
     """cu_k may be the very tensor cu_q while K and V have more rows than Q."""
     lq, h, d = [30, 41], 2, 64

@@ -98,7 +98,13 @@ def test_packed_refusals(fake):
                        ((q.transpose(0, 2), kv, kv, q.transpose(0, 2), 1.0, lens), {})):
         with pytest.raises(ValueError):
             fake.attn_prefill_packed(*args, **more)
+    wide = z(1, 1, 64)
+    for args in ((q, wide.expand(6, 2, 64), kv, q), (q, kv, wide.expand(6, 2, 64), q), (wide.expand(6, 4, 64), kv, kv, q)):
+        with pytest.raises(ValueError):
+            fake.attn_prefill_packed(*args, 1.0, lens)
     assert not fake.lib.calls
+    fake.attn_prefill_packed(q, z(6, 1, 64).expand(6, 2, 64), kv, q, 1.0, lens)  # one head for all is an ordinary stride
+    assert fake.lib.calls[0][1][14:16] == (64, 0)
 
 
 def test_append_refusals(fake):
@@ -113,6 +119,8 @@ def test_append_refusals(fake):
             fake.kv_append_q8(*args)
     with pytest.raises(ValueError):
         fake.kv_append_q8(k, k, kc, vc, ks, vs, lens, cu=lens)  # three offsets are wanted
+    with pytest.raises(ValueError):
+        fake.kv_append_q8(z(1, 1, 64).expand(2, 2, 64), k, kc, vc, ks, vs, lens)
     assert not fake.lib.calls
 
 
@@ -124,6 +132,8 @@ def test_decode_refusals(fake):
             fake.attn_decode_q8(*args, kv_len=lens)
     with pytest.raises(ValueError):
         fake.attn_decode_q8(q, *c, z(2, 4, 64), 1.0, kv_len=lens.float())
+    with pytest.raises(ValueError):
+        fake.attn_decode_q8(q, *c, z(2, 4, 64), 1.0, kv_len=lens, workspace=z(64, 64).t()[::2])
     fake.device = 0  # tensors that lie somewhere else
     with pytest.raises(ValueError):
         fake.attn_decode_q8(q, *c, z(2, 4, 64), 1.0, kv_len=lens)

@@ -350,6 +350,10 @@ class Context:
                 (D > 1 and not q2 == k2 == v2 == o2 == 1)):
             raise ValueError("attn_prefill_packed: Q %s, K %s, V %s and O %s do not go together, or their last dimension is not contiguous"
                              % tuple("%s %s" % (tuple(t.shape), t.dtype) for t in (Q, K, V, O)))
+        if not ((q0 or q1) and (k0 or k1) and (v0 or v1) and (o0 or o1)):  # strides {0, 0} stand for the dense layout
+            for t in (Q, K, V, O):
+                if t.stride()[:2] == (0, 0) and t.shape[0] * t.shape[1] > 1:
+                    raise ValueError("attn_prefill_packed: a tensor that repeats one row over all tokens and heads; make it contiguous")
         if Q.get_device() != dev or K.get_device() != dev or V.get_device() != dev or O.get_device() != dev:
             raise ValueError("attn_prefill_packed: the context belongs to cuda:%d, a tensor lies elsewhere" % dev)
         code, nseq = _any_dtype_code(Q), cu_q.shape[0] - 1
@@ -384,6 +388,8 @@ class Context:
         (k0, k1, k2), (v0, v1, v2), dev = K.stride(), V.stride(), self.device
         if heads != Hkv or dim != D or V.shape != shape or V.dtype is not K.dtype or k2 != 1 or v2 != 1 or K.get_device() != dev or V.get_device() != dev:
             raise ValueError("kv_append_q8: K and V must be [total,%d,%d] of one type on cuda:%d with the last dimension contiguous" % (Hkv, D, dev))
+        if not ((k0 or k1) and (v0 or v1)) and total * Hkv > 1:  # strides {0, 0} stand for the dense layout
+            raise ValueError("kv_append_q8: a tensor that repeats one row over all tokens and heads; make it contiguous")
         APPEND_ARGS.pack_into(self._args, 0, K.data_ptr(), V.data_ptr(), Kc.data_ptr(), Vc.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), B, Hkv, Lmax, D,
                               block, total, self._int32(cu, B + 1, "cu"), self._int32(kv_len, B, "kv_len"), k0, k1, v0, v1, _any_dtype_code(K), code)
         rc = self.lib.vkc_kv_append_q8(self.h, self._args_at, self._stream(stream))
@@ -400,6 +406,8 @@ class Context:
         if (len(shape) != 3 or shape[0] != B or shape[2] != D or O.shape != shape or O.dtype is not Q.dtype or not (Q.is_contiguous() and O.is_contiguous()) or
                 Q.get_device() != dev or O.get_device() != dev):
             raise ValueError("attn_decode_q8: Q and O must be contiguous [%d,Hq,%d] of one type on cuda:%d" % (B, D, dev))
+        if workspace is not None and (workspace.get_device() != dev or not workspace.is_contiguous()):
+            raise ValueError("attn_decode_q8: the workspace must be contiguous memory of cuda:%d" % dev)
         DECODE_Q8_ARGS.pack_into(self._args, 0, Q.data_ptr(), Kc.data_ptr(), Vc.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), O.data_ptr(), B, shape[1], Hkv,
                                  Lmax, D, block, self._int32(kv_len, B, "kv_len"), workspace.data_ptr() if workspace is not None else 0,
                                  workspace.numel() * workspace.element_size() if workspace is not None else 0, scale, _any_dtype_code(Q), code)

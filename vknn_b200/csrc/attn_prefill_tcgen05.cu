@@ -476,7 +476,8 @@ namespace {
             else return work_at<QT>(p, pos, cta);
         };
         Item w_first; // the first item, looked up while the barriers are being set up
-        if constexpr (!kPacked) w_first = look_up(0);
+        if constexpr (kPacked) w_first.valid = false; // (packed: every role looks its first item up behind the barrier)
+        else w_first = look_up(0);
         // the item after `cur` (which began at step `pos` minus its length); none behind the CTA's last
         auto next_work = [&](const Item &cur, int pos) {
             if (!cur.last) return look_up(pos);
@@ -1047,9 +1048,7 @@ namespace {
                                 if (from + 4 * i < isq) ptx::st_global_v4(at, o4[i]);
                                 at += 4 * p.os[2];
                             }
-                            __syncwarp(); // the staging lines are rewritten by the next 64 columns
-                            continue;
-                        }
+                        } else {
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             const int     rr   = i * 4 + (lane >> 3), ch = lane & 7;
@@ -1060,6 +1059,7 @@ namespace {
                                 if (ndest == 0) *reinterpret_cast<uint4 *>(obase + off) = o4;
                                 else vkc_fanout_store16<T>(p.fan, off, o4);
                             }
+                        }
                         }
                         __syncwarp(); // the staging lines are rewritten by the next 64 columns
                     }
