@@ -296,8 +296,8 @@ VKC_API int vkc_kv_append_q8(vkc_ctx *ctx, const vkc_kv_append_q8_args *args, vk
  *   a sequence with no key stores NaN, as in vkc_attn_decode. What lies behind kv_len in the cache is never used, whatever
  *   its bits. Sums and softmax statistics are fp32; Q keeps its precision.
  *   workspace: device scratch of at least vkc_attn_decode_q8_workspace_bytes(...) bytes (16-byte aligned) for the partial
- *   results; NULL lets the context keep (and grow) its own. It may hold anything before the call. Two calls that may run at
- *   the same time need workspaces of their own, and so do two captured graphs that may be replayed at the same time; calls
+ *   results (short caches leave it alone); NULL lets the context keep (and grow) its own. It may hold anything before the call.
+ *   Two calls that may run at the same time need workspaces of their own, and so do two captured graphs that may be replayed at the same time; calls
  *   captured without a workspace share the context's. ---- */
 VKC_API size_t vkc_attn_decode_q8_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Lmax, int64_t D);
 typedef struct vkc_attn_decode_q8_args {

@@ -576,6 +576,52 @@ def test_decode_q8_shapes(impl_ctx, d, block, group, dt, codes):
 
 
 @pytest.mark.parametrize("codes", ["e4m3", "i8"])
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("group", [1, 3, 8, 12, 16])
+@pytest.mark.parametrize("d,block", [(64, 32), (128, 64), (256, 128)])
+def test_decode_q8_shapes_of_a_longer_cache(ctx, d, block, group, dt, codes):
+    """The same with room for so many keys that the work is split over the keys."""
+    lens = [1, 0, 31, 32, 33, block, 300, 1407, 1408, 4 * block - 1]
+    cache = filled(1, len(lens), 2, 1408, d, block, codes)
+    check_decode(ctx, queries(2, len(lens), 2 * group, d, dt), cache, lens, d ** -0.5)
+
+
+@pytest.mark.parametrize("room", [768, 1024, 1280])
+@pytest.mark.parametrize("hkv", [1, 37, 38, 74, 75, 148, 149])
+def test_decode_q8_around_the_number_of_multiprocessors(ctx, hkv, room):
+    """Where the choice between a block of threads per kv head and equal shares changes; the first tokens of a cache of any room."""
+    for d, block, b in ((64, 32, 2), (128, 128, 4), (256, 64, 1)):
+        for lmax in (room, room // 2):
+            lens = [lmax, lmax // 3, 0, 1][:b]
+            check_decode(ctx, queries(23, b, hkv, d, "bf16"), filled(22, b, hkv, lmax, d, block, "e4m3"), lens, d ** -0.5, (d, lmax))
+
+
+@pytest.mark.parametrize("codes,fill", [("e4m3", 0x7f), ("i8", 0x80)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_decode_q8_never_uses_what_lies_behind_in_a_longer_cache(ctx, codes, fill, d):
+    lens, block = [1, 33, 90, 1290, 0, 2048], 64
+    cache = filled(24, 6, 2, 2048, d, block, codes)
+    for i, n in enumerate(lens):
+        for t in (cache.k, cache.v):
+            t.view(torch.uint8)[i, :, n:] = fill
+        for s in (cache.ks, cache.vs):
+            s[i, :, -(-n // block):] = float("nan")
+    q = queries(25, 6, 4, d, "f16")
+    o = torch.zeros_like(q)
+    ctx.attn_decode_q8(q, *cache.args, o, d ** -0.5, kv_len=torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    ctx.sync()
+    ref, a = decode64(q, cache, lens, d ** -0.5)
+    check(o, ref, a, torch.float16, torch.float16)
+    cache.ks[0, 1, 0] = float("nan")  # a marked block in use
+    cache.vs[3, 0, 20] = float("nan")
+    ctx.attn_decode_q8(q, *cache.args, o, d ** -0.5, kv_len=torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    ctx.sync()
+    bad = torch.isnan(o).all(-1)
+    assert bad.tolist() == [[False, False, True, True], [False] * 4, [False] * 4, [True, True, False, False], [True] * 4, [False] * 4]
+    assert int(torch.isnan(o).any(-1).sum()) == int(bad.sum())
+
+
+@pytest.mark.parametrize("codes", ["e4m3", "i8"])
 @pytest.mark.parametrize("b,hq,hkv,lmax,lens", [
     (1, 8, 1, 16384, [16001]), (1, 12, 12, 512, [331]), (3, 16, 8, 4096, [4096, 1, 2500]), (40, 4, 2, 2048, None), (2, 8, 2, 32768, [32768, 70]), (70, 8, 8, 128, None)],
     ids=["one_long", "one_short", "uneven", "batch", "long_and_short", "many_short"])

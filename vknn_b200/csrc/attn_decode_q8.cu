@@ -24,6 +24,8 @@
 // A unit that lies in one run is finished there; one that is cut leaves a partial (maximum, sum, O) per run in the workspace
 // (slot 0: the unit began in an earlier run, slot 1: in this one) and a second kernel joins them in the order of the runs.
 // (Joined by the warp whose partial arrives last instead, the batch took 73 us, not 67: the fences hold up the stream.)
+// Short caches take one CTA per unit instead (kUnit, one_cta_per_unit): its warps share the unit's tiles, merge once in shared
+// memory and store O; one kernel and no workspace.
 #include "kv_q8.cuh"
 #include "ptx.cuh"
 #include "tensormap.cuh"
@@ -104,6 +106,7 @@ namespace {
         DecQ8Params q;
         int         B, G; // sequences of this launch, query heads per kv head
         int         runs; // partial slots of the workspace hold this many runs
+        bool        unit; // one CTA per unit
         int         block_log2;
         float      *part_o;  // [runs][2][G][D]
         float      *part_ml; // [runs][2][G][2]
@@ -125,6 +128,7 @@ namespace {
         static constexpr uint32_t oTab  = oCtl + 16;                             // first line position of each sequence
         static constexpr uint32_t total = oTab + (kSliceB + 1) * 4 + 1024;
         static_assert(total <= 227 * 1024, "shared memory budget");
+        static_assert(W * NT * 8 * (D + 2) * 4 <= (int) oBar, "the warps' partials fit into the ring");
     };
 
     // D[16x8] += A[16x16] * B[16x8], f16 operands, fp32 accumulator
@@ -174,7 +178,8 @@ namespace {
         int b, hk, tile, n;
     };
 
-    template <typename T, int D, int NT, bool kE4m3>
+    // kUnit: one CTA per unit, its warps take the unit's tiles in turn and meet in shared memory; no line, no workspace, no second kernel.
+    template <typename T, int D, int NT, bool kE4m3, bool kUnit>
     __global__ void __launch_bounds__(Stream<D, NT>::W * 32, 1)
         attn_decode_q8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ StreamParams p) {
         using L          = Stream<D, NT>;
@@ -198,49 +203,60 @@ namespace {
         }
         vkc_grid_dep_wait();
         vkc_grid_dep_launch();
-        // line positions: sequence b begins at tab[b] and has Hkv * ceil(len / 32) tiles
-        {
-            __shared__ int wsum[W];
-            int            run = 0;
-            for (int b0 = 0; b0 < p.B; b0 += W * 32) {
-                const int b = b0 + threadIdx.x;
-                int       n = b < p.B ? (int) ((q8_len(p.q, b) + kTile - 1) / kTile) * Hkv : 0, incl = n;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int up = __shfl_up_sync(0xffffffffu, incl, o);
-                    if (lane >= o) incl += up;
-                }
-                if (lane == 31) wsum[warp] = incl;
-                __syncthreads();
-                int before = run, all = run;
-#pragma unroll
-                for (int w = 0; w < W; ++w) {
-                    if (w < warp) before += wsum[w];
-                    all += wsum[w];
-                }
-                if (b < p.B) tab[b] = before + incl - n;
-                run = all;
-                __syncthreads();
+        int  P0 = 0, P1 = 0, quota = 1, run = 0; // this warp's run [P0, P1) of the line, tiles of a run, number of the run
+        At   at;                                 // its first tile
+        bool ok = true;
+        if constexpr (kUnit) {
+            at.b = blockIdx.x / Hkv, at.hk = blockIdx.x - at.b * Hkv, at.tile = warp;
+            at.n = (int) ((q8_len(p.q, at.b) + kTile - 1) / kTile);
+            P1   = at.n > warp ? (at.n - warp + W - 1) / W : 0;
+            if (at.n == 0) { // no key: 0 / 0
+                for (int i = threadIdx.x; i < p.G * D; i += W * 32) St<T>::st((T *) p.q.O + ((int64_t) at.b * p.q.Hq + at.hk * p.G) * D + i, q8::nan_value());
+                return;
             }
-            if (threadIdx.x == 0) tab[p.B] = run;
-        }
-        __syncthreads();
-        // sequences without a key: 0 / 0
-        for (int b = blockIdx.x; b < p.B; b += gridDim.x)
-            if (tab[b] == tab[b + 1])
-                for (int i = threadIdx.x; i < (int) p.q.Hq * D; i += W * 32) St<T>::st((T *) p.q.O + (int64_t) b * p.q.Hq * D + i, q8::nan_value());
-        // This warp's run [P0, P1) of the line. Neighbouring runs go to different SMs, so that a short line still uses all of them.
-        const int total = tab[p.B], runs = (int) gridDim.x * W, run = warp * (int) gridDim.x + (int) blockIdx.x;
-        int       quota = (total + runs - 1) / runs;
-        if (quota < kMinTiles) quota = kMinTiles;
-        if (blockIdx.x == 0)
-            for (int i = threadIdx.x; i <= p.B + 1; i += W * 32) p.line[i] = i <= p.B ? tab[i] : quota;
-        const int64_t c0 = (int64_t) run * quota;
-        const int     P0 = c0 < total ? (int) c0 : total, P1 = c0 + quota < total ? (int) (c0 + quota) : total;
-        bool          ok  = true;
-        if (P0 < P1) {
-            At at; // of P0
+            __syncthreads(); // the barriers are set up
+        } else {
+            // line positions: sequence b begins at tab[b] and has Hkv * ceil(len / 32) tiles
             {
+                __shared__ int wsum[W];
+                int            sum = 0;
+                for (int b0 = 0; b0 < p.B; b0 += W * 32) {
+                    const int b = b0 + threadIdx.x;
+                    int       n = b < p.B ? (int) ((q8_len(p.q, b) + kTile - 1) / kTile) * Hkv : 0, incl = n;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const int up = __shfl_up_sync(0xffffffffu, incl, o);
+                        if (lane >= o) incl += up;
+                    }
+                    if (lane == 31) wsum[warp] = incl;
+                    __syncthreads();
+                    int before = sum, all = sum;
+#pragma unroll
+                    for (int w = 0; w < W; ++w) {
+                        if (w < warp) before += wsum[w];
+                        all += wsum[w];
+                    }
+                    if (b < p.B) tab[b] = before + incl - n;
+                    sum = all;
+                    __syncthreads();
+                }
+                if (threadIdx.x == 0) tab[p.B] = sum;
+            }
+            __syncthreads();
+            // sequences without a key: 0 / 0
+            for (int b = blockIdx.x; b < p.B; b += gridDim.x)
+                if (tab[b] == tab[b + 1])
+                    for (int i = threadIdx.x; i < (int) p.q.Hq * D; i += W * 32) St<T>::st((T *) p.q.O + (int64_t) b * p.q.Hq * D + i, q8::nan_value());
+            // This warp's run [P0, P1) of the line. Neighbouring runs go to different SMs, so that a short line still uses all of them.
+            const int total = tab[p.B], runs = (int) gridDim.x * W;
+            run   = warp * (int) gridDim.x + (int) blockIdx.x;
+            quota = (total + runs - 1) / runs;
+            if (quota < kMinTiles) quota = kMinTiles;
+            if (blockIdx.x == 0)
+                for (int i = threadIdx.x; i <= p.B + 1; i += W * 32) p.line[i] = i <= p.B ? tab[i] : quota;
+            const int64_t c0 = (int64_t) run * quota;
+            P0 = c0 < total ? (int) c0 : total, P1 = c0 + quota < total ? (int) (c0 + quota) : total;
+            if (P0 < P1) {
                 int lo = 0, hi = p.B;
                 while (hi - lo > 1) {
                     const int mid = (lo + hi) >> 1;
@@ -250,6 +266,8 @@ namespace {
                 at.b = lo, at.n = (tab[lo + 1] - tab[lo]) / Hkv;
                 at.hk = (P0 - tab[lo]) / at.n, at.tile = P0 - tab[lo] - at.hk * at.n;
             }
+        }
+        if (kUnit || P0 < P1) {
             auto next_unit = [&](At &x) { // to the beginning of the next unit (there is one)
                 x.tile = 0;
                 if (++x.hk == Hkv) {
@@ -290,7 +308,10 @@ namespace {
                 asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(p_bar) : "memory");
                 p_bar += 8u, p_dst += 2 * L::TILE, p_sc += 8u;
                 if (p_bar == bars + 8u * S) p_bar = bars, p_dst = ring, p_sc = sc_a;
-                if (--left > 0 && ++pa.tile == pa.n) {
+                --left;
+                if constexpr (kUnit) {
+                    pa.tile += W;
+                } else if (left > 0 && ++pa.tile == pa.n) {
                     next_unit(pa);
                     row0 = (pa.b * Hkv + pa.hk) * rows_per_unit;
                 }
@@ -301,9 +322,9 @@ namespace {
 
             int      stage = 0;
             uint32_t phase = 0;
-            for (int todo = P1 - P0; todo > 0 && ok;) { // one item: the part of a unit in this run
+            for (int todo = kUnit ? 1 : P1 - P0; todo > 0 && ok;) { // one item: the part of a unit in this run
                 const int len = (int) q8_len(p.q, at.b), hq0 = at.hk * p.G, first = at.tile;
-                const int end = at.n - first < todo ? at.n : first + todo; // its tiles: [first, end)
+                const int end = kUnit || at.n - first < todo ? at.n : first + todo; // its tiles: [first, end)
                 float     o[NT][MT][4], m[NT], l[NT], fac[NT];
                 uint32_t  qa[NT][D / 16][2];
                 // Q of this kv head's group: row g (and g + 8) of the A fragments, dims in the order the key chunks are read in
@@ -350,7 +371,7 @@ namespace {
 #pragma unroll
                     for (int i = 0; i < MT; ++i) o[h][i][0] = o[h][i][1] = o[h][i][2] = o[h][i][3] = 0.f;
                 }
-                for (int tile = first; tile < end; ++tile) {
+                for (int tile = first; tile < end; tile += kUnit ? W : 1) {
                     ok = ptx::mbar_wait(bars + 8u * stage, phase, ctl, p.dev_err);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
@@ -462,6 +483,42 @@ namespace {
                     __syncwarp(); // every lane has read the stage
                     if (lane == 0) fetch();
                     if (++stage == S) stage = 0, phase ^= 1;
+                }
+                if constexpr (kUnit) {
+                    // ---- the warps' (m, l, O) meet in the ring's memory: [warp][head][D], then [warp][head] (m, l)
+                    float *image = (float *) (gb + L::oRing), *ml = image + W * NT * 8 * D;
+                    __syncthreads(); // every tile has been read
+#pragma unroll
+                    for (int h = 0; h < NT; ++h) {
+                        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+                        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+                        if (t == 0) ml[((warp * NT + h) * 8 + g) * 2] = m[h], ml[((warp * NT + h) * 8 + g) * 2 + 1] = l[h];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float4 *to = reinterpret_cast<float4 *>(image + ((warp * NT + h) * 8 + 2 * t + e) * D + g * (D / 8));
+#pragma unroll
+                            for (int i = 0; i < MT / 2; ++i) to[i] = make_float4(o[h][2 * i][e], o[h][2 * i][2 + e], o[h][2 * i + 1][e], o[h][2 * i + 1][2 + e]);
+                        }
+                    }
+                    __syncthreads();
+                    for (int i = threadIdx.x; i < p.G * (D / 4); i += W * 32) {
+                        const int hd = i * 4 / D, d = i * 4 - hd * D;
+                        float     top = -INFINITY, ls = 0.f;
+#pragma unroll
+                        for (int w = 0; w < W; ++w) top = fmaxf(top, ml[(w * NT * 8 + hd) * 2]);
+                        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                        for (int w = 0; w < W; ++w) {
+                            const float  mw = ml[(w * NT * 8 + hd) * 2], lw = ml[(w * NT * 8 + hd) * 2 + 1], a = mw == -INFINITY && lw == 0.f ? 0.f : ex2(mw - top);
+                            const float4 v  = *reinterpret_cast<const float4 *>(image + (w * NT * 8 + hd) * D + d);
+                            ls              = fmaf(lw, a, ls);
+                            acc.x = fmaf(v.x, a, acc.x), acc.y = fmaf(v.y, a, acc.y), acc.z = fmaf(v.z, a, acc.z), acc.w = fmaf(v.w, a, acc.w);
+                        }
+                        const float inv = 1.0f / ls;
+                        *reinterpret_cast<uint2 *>((T *) p.q.O + ((int64_t) at.b * p.q.Hq + hq0 + hd) * D + d) =
+                            make_uint2(pair16<T>(acc.x * inv, acc.y * inv), pair16<T>(acc.z * inv, acc.w * inv));
+                    }
+                    break;
                 }
                 if (!ok) break;
                 // ---- the item's rows: a thread holds D / 8 consecutive dims, from g * D / 8 on, of the heads 2t and 2t + 1
@@ -581,8 +638,14 @@ namespace {
 
     template <typename T, int D, int NT, bool kE4m3>
     int launch_stream(vkc_ctx *ctx, const StreamParams &p, int grid, const CUtensorMap &tk, const CUtensorMap &tv, cudaStream_t st) {
-        auto          kern = attn_decode_q8_kernel<T, D, NT, kE4m3>;
         constexpr int smem = (int) Stream<D, NT>::total;
+        if (p.unit) {
+            auto kern = attn_decode_q8_kernel<T, D, NT, kE4m3, true>;
+            if (int rc = vkc_configure_smem(ctx, kern, smem)) return rc;
+            vkc_launch(ctx, kern, dim3((unsigned) (p.B * p.q.Hkv)), dim3(Stream<D, NT>::W * 32), smem, st, tk, tv, p);
+            return vkc_post_launch(ctx, "attn_decode_q8");
+        }
+        auto kern = attn_decode_q8_kernel<T, D, NT, kE4m3, false>;
         if (int rc = vkc_configure_smem(ctx, kern, smem)) return rc;
         vkc_launch(ctx, kern, dim3((unsigned) grid), dim3(Stream<D, NT>::W * 32), smem, st, tk, tv, p);
         if (int rc = vkc_post_launch(ctx, "attn_decode_q8")) return rc;
@@ -598,8 +661,19 @@ namespace {
         return e4m3 ? launch_stream<T, D, 2, true>(ctx, p, grid, tk, tv, st) : launch_stream<T, D, 2, false>(ctx, p, grid, tk, tv, st);
     }
 
-    // The streaming form for the whole call, kSliceB sequences per launch.
-    int run_stream(vkc_ctx *ctx, const DecQ8Params &q, int64_t B, int64_t D, bool e4m3, int dtype, void *ws, cudaStream_t st) {
+    // Whether one CTA per unit beats equal runs over all warps, by the cache's length (the sequences' own are on the device): up to four
+    // tiles per warp in one round of CTAs, two in two rounds. It saves the line, the partials and the second kernel, but its rounds do
+    // not overlap and it does not even out lengths. Measured in a graph, us, unit against runs, D = 128 where not said: 12 units of 512
+    // keys at D = 64 4.3 / 6.7, 32 of 1024 7.5 / 7.8, 128 of 1024 7.9 / 12.2, 64 of 512 at D = 256 9.3 / 11.5 (4 of them 9.1 / 8.1, but
+    // the call costs the host 1.6 us less), 256 of 512 9.0 / 11.0; beyond: 32 of 1536 9.7 / 8.5, 32 of 2048 11.8 / 8.9, 160 of 1024
+    // 16.6 / 15.8, 400 of 512 17.6 / 17.5, 960 of 256 at D = 64 20 / 15.4.
+    bool one_cta_per_unit(int64_t B, int64_t Hkv, int64_t Lmax, int64_t D, int sms) {
+        const int64_t W = D == 256 ? 4 : 8, rounds = (B * Hkv + sms - 1) / sms;
+        return B <= kSliceB && rounds <= 2 && rounds * (Lmax / kTile) <= 4 * W;
+    }
+
+    // The tensor-core forms for the whole call, kSliceB sequences per launch.
+    int run_stream(vkc_ctx *ctx, const DecQ8Params &q, int64_t B, int64_t D, bool e4m3, int dtype, bool unit, void *ws, cudaStream_t st) {
         const int64_t G = q.Hq / q.Hkv;
         for (int64_t b0 = 0; b0 < B; b0 += kSliceB) {
             StreamParams p;
@@ -615,6 +689,7 @@ namespace {
             int64_t       grid = ctx->sm_count < kMaxCtas ? ctx->sm_count : kMaxCtas;
             if (grid > here) grid = here;
             p.runs    = (int) runs;
+            p.unit    = unit;
             p.part_o  = (float *) ws;
             p.part_ml = p.part_o + runs * 2 * G * D;
             p.line    = (int *) (p.part_ml + runs * 2 * G * 2);
@@ -676,11 +751,12 @@ extern "C" int vkc_attn_decode_q8(vkc_ctx *ctx, const vkc_attn_decode_q8_args *a
     // The streaming form holds a group of up to 16 query heads and counts line positions and 128-byte rows in 32 bits.
     const bool fits = Hq / Hkv <= 16 && (B < kSliceB ? B : kSliceB) * Hkv * (Lmax / kTile) < INT32_MAX / 2 && (B < kSliceB ? B : kSliceB) * Hkv * Lmax * (D / 64) < INT32_MAX;
     if (fits && ctx->impl != VKC_IMPL_SIMT) {
-        if (!workspace) {
+        const bool unit = one_cta_per_unit(B, Hkv, Lmax, D, ctx->sm_count);
+        if (!workspace && !unit) {
             if (int rc = vkc_ensure_scratch(ctx, need, st)) return rc;
             workspace = ctx->scratch;
         }
-        return run_stream(ctx, p, B, D, e4m3, dtype, workspace, st);
+        return run_stream(ctx, p, B, D, e4m3, dtype, unit, workspace, st);
     }
     if (ctx->impl == VKC_IMPL_TCGEN05) return vkc_fail(ctx, VKC_ERR_UNSUPPORTED, "attn_decode_q8: more than 16 query heads per kv head, or too large a cache, for the tensor-core form");
 #define VKC_Q8_SIMT(T)                                              \
