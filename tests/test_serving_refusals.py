@@ -22,7 +22,7 @@ class Recorder:
 
     def __getattr__(self, name):
         s = self.STRUCTS[name]
-        return lambda h, at, stream: self.calls.append((name, s.unpack(C.string_at(at, s.size)))) or 0
+        return lambda h, args, stream: self.calls.append((name, s.unpack(args))) or 0
 
 
 @pytest.fixture
@@ -30,7 +30,6 @@ def fake():
     c = vknn_b200.Context.__new__(vknn_b200.Context)
     c.lib, c.h, c.device = Recorder(), None, -1  # -1 is what CPU tensors answer for their device
     c._stream = lambda stream: None
-    c._make_args()
     return c
 
 
@@ -48,6 +47,15 @@ def test_null_context_is_refused():
     for f in (lib.vkc_attn_prefill_packed, lib.vkc_kv_append_q8, lib.vkc_attn_decode_q8):
         assert f(None, C.addressof(args), None) == -1 and f(None, None, None) == -1
     assert lib.vkc_attn_decode_q8_workspace_bytes(0, 1, 1, 32, 64) == 0 and lib.vkc_attn_decode_q8_workspace_bytes(2, 8, 2, 4096, 128) > 0
+
+
+def test_lengths_of_a_single_sequence_may_come_from_a_column(fake):
+    k, v, ks, vs = cache(b=1)
+    lens = z(3, 2, dt=torch.int32)[:1, 1]
+    fake.kv_append_q8(z(1, 2, 64), z(1, 2, 64), k, v, ks, vs, kv_len=lens)
+    assert fake.lib.calls[0][1][13] == lens.data_ptr()
+    with pytest.raises(ValueError):
+        fake.kv_append_q8(z(2, 2, 64), z(2, 2, 64), *cache(), kv_len=z(2, 2, dt=torch.int32)[:, 1])
 
 
 def test_argument_structs_have_the_layout_of_the_c_compiler(tmp_path):

@@ -150,7 +150,7 @@ class Gate(C.Structure):
     _fields_ = [("flags", C.c_void_p), ("n", C.c_int), ("state", C.c_void_p)]
 
 
-# The argument structs of include/vknn_cuda.h. They are filled by struct.pack_into and passed by address: one conversion for all
+# The argument structs of include/vknn_cuda.h. They are packed into a bytes object that is passed by address: one conversion for all
 # fields, where an argument list of that length costs ctypes 2.5 us a call.
 PACKED_ARGS = struct.Struct("@4P6q2P8qf2i")   # vkc_attn_prefill_packed_args
 APPEND_ARGS = struct.Struct("@6P6q2P4q2i")    # vkc_kv_append_q8_args
@@ -225,12 +225,6 @@ class Context:
             raise VkcError(rc, "vkc_ctx_create(%d) failed (no usable sm_100 device?)" % device)
         self.h = h
         self.device = int(device)
-        self._make_args()
-
-    def _make_args(self):
-        """Room for one argument struct (a context is driven by one thread at a time, and no call keeps it)."""
-        self._args = C.create_string_buffer(256)
-        self._args_at = C.addressof(self._args)
 
     def close(self):
         if getattr(self, "h", None):
@@ -333,7 +327,7 @@ class Context:
         """The pointer of an int32 tensor of n elements on this device, or 0 for None."""
         if t is None:
             return 0
-        if t.dtype is not _torch_int32[0] or t.shape != (n,) or t.stride(0) != 1 or t.get_device() != self.device:
+        if t.dtype is not _torch_int32[0] or t.shape != (n,) or not t.is_contiguous() or t.get_device() != self.device:
             raise ValueError("%s must be a contiguous int32 tensor of %d elements on cuda:%d" % (what, n, self.device))
         return t.data_ptr()
 
@@ -357,10 +351,10 @@ class Context:
         if Q.get_device() != dev or K.get_device() != dev or V.get_device() != dev or O.get_device() != dev:
             raise ValueError("attn_prefill_packed: the context belongs to cuda:%d, a tensor lies elsewhere" % dev)
         code, nseq = _any_dtype_code(Q), cu_q.shape[0] - 1
-        PACKED_ARGS.pack_into(self._args, 0, Q.data_ptr(), K.data_ptr(), V.data_ptr(), O.data_ptr(), nseq, Hq, Hkv, D, total_q, total_k,
-                              self._int32(cu_q, nseq + 1, "cu_q"), self._int32(cu_k, nseq + 1, "cu_k"), q0, q1, k0, k1, v0, v1, o0, o1, scale,
-                              1 if causal else 0, code)
-        rc = self.lib.vkc_attn_prefill_packed(self.h, self._args_at, self._stream(stream))
+        args = PACKED_ARGS.pack(Q.data_ptr(), K.data_ptr(), V.data_ptr(), O.data_ptr(), nseq, Hq, Hkv, D, total_q, total_k,
+                                self._int32(cu_q, nseq + 1, "cu_q"), self._int32(cu_k, nseq + 1, "cu_k"), q0, q1, k0, k1, v0, v1, o0, o1, scale,
+                                1 if causal else 0, code)
+        rc = self.lib.vkc_attn_prefill_packed(self.h, args, self._stream(stream))
         if rc:
             self._check(rc)
 
@@ -390,9 +384,9 @@ class Context:
             raise ValueError("kv_append_q8: K and V must be [total,%d,%d] of one type on cuda:%d with the last dimension contiguous" % (Hkv, D, dev))
         if not ((k0 or k1) and (v0 or v1)) and total * Hkv > 1:  # strides {0, 0} stand for the dense layout
             raise ValueError("kv_append_q8: a tensor that repeats one row over all tokens and heads; make it contiguous")
-        APPEND_ARGS.pack_into(self._args, 0, K.data_ptr(), V.data_ptr(), Kc.data_ptr(), Vc.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), B, Hkv, Lmax, D,
-                              block, total, self._int32(cu, B + 1, "cu"), self._int32(kv_len, B, "kv_len"), k0, k1, v0, v1, _any_dtype_code(K), code)
-        rc = self.lib.vkc_kv_append_q8(self.h, self._args_at, self._stream(stream))
+        args = APPEND_ARGS.pack(K.data_ptr(), V.data_ptr(), Kc.data_ptr(), Vc.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), B, Hkv, Lmax, D,
+                                block, total, self._int32(cu, B + 1, "cu"), self._int32(kv_len, B, "kv_len"), k0, k1, v0, v1, _any_dtype_code(K), code)
+        rc = self.lib.vkc_kv_append_q8(self.h, args, self._stream(stream))
         if rc:
             self._check(rc)
 
@@ -408,10 +402,10 @@ class Context:
             raise ValueError("attn_decode_q8: Q and O must be contiguous [%d,Hq,%d] of one type on cuda:%d" % (B, D, dev))
         if workspace is not None and (workspace.get_device() != dev or not workspace.is_contiguous()):
             raise ValueError("attn_decode_q8: the workspace must be contiguous memory of cuda:%d" % dev)
-        DECODE_Q8_ARGS.pack_into(self._args, 0, Q.data_ptr(), Kc.data_ptr(), Vc.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), O.data_ptr(), B, shape[1], Hkv,
-                                 Lmax, D, block, self._int32(kv_len, B, "kv_len"), workspace.data_ptr() if workspace is not None else 0,
-                                 workspace.numel() * workspace.element_size() if workspace is not None else 0, scale, _any_dtype_code(Q), code)
-        rc = self.lib.vkc_attn_decode_q8(self.h, self._args_at, self._stream(stream))
+        args = DECODE_Q8_ARGS.pack(Q.data_ptr(), Kc.data_ptr(), Vc.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), O.data_ptr(), B, shape[1], Hkv,
+                                   Lmax, D, block, self._int32(kv_len, B, "kv_len"), workspace.data_ptr() if workspace is not None else 0,
+                                   workspace.numel() * workspace.element_size() if workspace is not None else 0, scale, _any_dtype_code(Q), code)
+        rc = self.lib.vkc_attn_decode_q8(self.h, args, self._stream(stream))
         if rc:
             self._check(rc)
 
