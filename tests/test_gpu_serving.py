@@ -241,29 +241,49 @@ def test_packed_output_strides_that_16_bytes_cannot_follow(ctx):
     assert torch.equal(o[:, :, 1:d + 1], want) and bool((o[:, :, 0] == 5).all()) and bool((o[:, :, d + 1:] == 5).all())
 
 
+def check_like_simt(ctx, lq, lk, hq, hkv, d, causal=True):
+    """Against the SIMT kernel, which the tests above compare with 64 bits: each is within its own bound of the exact value, so they
+    differ by the sum of the two."""
+    q, k, v = packed_case(12, lq, lk, hq, hkv, d, torch.bfloat16)
+    o, want, a = torch.full_like(q, 9.0), torch.full_like(q, 9.0), torch.zeros_like(q)
+    cu_q, cu_k = offsets(lq), offsets(lk)
+    ctx.attn_prefill_packed(q, k, v, o, d ** -0.5, cu_q, cu_k, causal)
+    ctx.set_impl(vknn_b200.IMPL_SIMT)
+    ctx.attn_prefill_packed(q, k, v, want, d ** -0.5, cu_q, cu_k, causal)
+    ctx.attn_prefill_packed(q, k, v.abs(), a, d ** -0.5, cu_q, cu_k, causal)  # sum p |v|
+    ctx.set_impl(vknn_b200.IMPL_AUTO)
+    ctx.sync()
+    assert torch.equal(torch.isnan(o), torch.isnan(want))  # rows without a key
+    u = half_step(torch.bfloat16)
+    o, w, s = (torch.nan_to_num(x.double()) for x in (o, want, a))
+    s = s * (1 + 2 * u)  # (a is itself rounded)
+    tol = 2 * u * w.abs() * (1 + u) + (u + 2 * SMALL) * s * (1 + u)
+    assert bool(((o - w).abs() <= tol).all())
+
+
 @pytest.mark.parametrize("hq,hkv,d,nseq,hi", [(32, 8, 128, 300, 60), (20, 20, 64, 300, 60), (18, 6, 128, 280, 70), (4, 2, 64, 900, 5), (6, 6, 128, 700, 6), (64, 2, 64, 40, 300)],
                          ids=["pairs_many_rounds", "rows_many_rounds", "odd_group", "more_units_than_are_ranked", "rows_more_units", "wide_group"])
 def test_packed_many_sequences(ctx, hq, hkv, d, nseq, hi):
-    """Many rounds per CTA, more units than one CTA ranks, groups of odd and of large size. Against the SIMT kernel, which the tests
-    above compare with 64 bits: each is within its own bound of the exact value, so they differ by the sum of the two."""
+    """Many rounds per CTA, more units than one CTA ranks, groups of odd and of large size."""
     lq = [int(x) for x in np.random.default_rng(nseq).integers(0, hi + 1, nseq)]
-    q, k, v = packed_case(12, lq, lq, hq, hkv, d, torch.bfloat16)
-    o, want = torch.full_like(q, 9.0), torch.full_like(q, 9.0)
-    ctx.attn_prefill_packed(q, k, v, o, d ** -0.5, offsets(lq))
-    ctx.set_impl(vknn_b200.IMPL_SIMT)
-    ctx.attn_prefill_packed(q, k, v, want, d ** -0.5, offsets(lq))
-    ctx.set_impl(vknn_b200.IMPL_AUTO)
-    ctx.sync()
-    # sum p |v| through the same SIMT kernel
-    a = torch.zeros_like(q)
-    ctx.set_impl(vknn_b200.IMPL_SIMT)
-    ctx.attn_prefill_packed(q, k, v.abs(), a, d ** -0.5, offsets(lq))
-    ctx.set_impl(vknn_b200.IMPL_AUTO)
-    ctx.sync()
-    u = half_step(torch.bfloat16)
-    w, s = want.double(), a.double() * (1 + 2 * u)  # (a is itself rounded)
-    tol = 2 * u * w.abs() * (1 + u) + (u + 2 * SMALL) * s * (1 + u)
-    assert bool(((o.double() - w).abs() <= tol).all())
+    check_like_simt(ctx, lq, lq, hq, hkv, d)
+
+
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "full"])
+@pytest.mark.parametrize("hq,hkv,d,nseq,hi,some", [(64, 2, 64, 130, 60, 20), (32, 8, 128, 700, 6, 50), (6, 6, 128, 700, 6, 50), (6, 6, 64, 700, 200, 50)],
+                         ids=["ranked", "pairs", "rows", "rows64"])
+def test_packed_long_runs_of_sequences_without_keys(ctx, hq, hkv, d, nseq, hi, some, causal):
+    """Keys for the first sequences and (beyond what is ranked) the last; dozens of rounds of a CTA in between have nothing to compute."""
+    lq = [int(x) for x in np.random.default_rng(nseq).integers(1, hi + 1, nseq)]
+    lk = [n + 3 if i < some or i >= nseq - some // 2 else 0 for i, n in enumerate(lq)]
+    check_like_simt(ctx, lq, lk, hq, hkv, d, causal)
+    check_like_simt(ctx, lq, [0] * (nseq - 1) + [5], hq, hkv, d, causal)
+    check_like_simt(ctx, lq, [5] + [0] * (nseq - 1), hq, hkv, d, causal)
+
+
+def test_packed_a_sequence_of_more_units_than_are_ranked(ctx):
+    check_like_simt(ctx, [66000, 40], [66000, 40], 2, 1, 64)
+    check_like_simt(ctx, [40, 33100, 1], [50, 33100, 900], 2, 2, 128)
 
 
 def test_packed_keys_shared_by_a_broadcast_stride(ctx):

@@ -93,7 +93,7 @@ namespace {
         // Skv above are the totals, O's rows follow os[2] from the first row of the first sequence.
         const int32_t *cu_q, *cu_k;
         int64_t        nseq;
-        int            ranked; // units to rank (at most kRanked), or 0: one CTA per unit
+        int            units;  // unit numbers (some of them empty), or 0: one CTA per unit
         int            turns;  // query heads, or pairs of them (kPack == 2): a unit's rows come once for each
     };
     // Packed sequences, more units than SMs: persistent CTAs take them longest first. Every CTA ranks the units by itself (their
@@ -101,7 +101,11 @@ namespace {
     // that outlives it); round r of CTA c is the unit and head number r * CTAs + c, and c counted from the other end in odd
     // rounds, which evens out the lengths.
     constexpr int kRanked = 512;
-    constexpr int kCached = 24; // rounds whose units are looked up in advance
+    // Rounds are described in shared memory before anyone gets to them, in a ring of two halves of kHalf rounds: every role of the
+    // CTA says when it is done with a half, and a warp that has nothing else to do looks the next kHalf rounds up, a lane for each (a look-up
+    // is a chain of dependent loads, 1500 to 2500 cycles; made by each role for itself it held up every item).
+    constexpr int kHalf = 8, kCached = 2 * kHalf;
+    constexpr long long kRingLimit = 64 * ptx::kWaitLimitCycles; // the rounds of a half may be long
     struct PackedUnit {
         int q0, k0;   // the unit's first query row, the sequence's first key row
         int sq, sk;   // the sequence's query rows from q0 on (0: nothing to do) and its keys
@@ -253,7 +257,7 @@ namespace {
     }
     template <int QT> __device__ __forceinline__ PackedWork<QT> packed_item(const PackedUnit &x) {
         PackedWork<QT> w;
-        w.valid = x.sq > 0;
+        w.valid = x.h >= 0;
         if (!w.valid) return w;
         w.b = 0, w.h = x.h, w.qg = 0;
         w.j0 = 0, w.slot = -1, w.adv = 1, w.last = x.last;
@@ -261,20 +265,22 @@ namespace {
         w.n_max = 0;
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
-            w.n_t[t] = x.n[t];
-            w.n_max  = x.n[t] > w.n_max ? x.n[t] : w.n_max;
+            w.n_t[t] = x.sq > 0 ? x.n[t] : 0;
+            w.n_max  = w.n_t[t] > w.n_max ? w.n_t[t] : w.n_max;
         }
         return w;
     }
-    // What CTA c does in a round, when `n` units are ranked in `order`. cu_q, cu_k: the offsets, in global or shared memory.
+    // What CTA c does in a round, of `n` units, ranked in `order` or (more than kRanked) taken as they are numbered. cu_q, cu_k: the
+    // offsets, in global or shared memory.
     template <int QT, int kRows> __device__ __forceinline__ PackedUnit packed_round(const AttnParams &p, const CtaId c, const int32_t *cu_q, const int32_t *cu_k,
                                                                            const uint16_t *order, int n, int heads, int round) {
         auto       turn = [&](int r) { return r * c.nx + (r & 1 ? c.nx - 1 - c.x : c.x); };
         const int  i = turn(round);
         PackedUnit x;
-        x.sq = 0;
+        x.h = -1;
         if (i < n * p.turns) {
-            x   = packed_unit<QT, kRows>(p, cu_q, cu_k, order[i / p.turns]);
+            const int k = i / p.turns;
+            x   = packed_unit<QT, kRows>(p, cu_q, cu_k, n > kRanked ? k : order[k]);
             x.h = i % p.turns * heads, x.last = turn(round + 1) >= n * p.turns;
         }
         return x;
@@ -285,19 +291,19 @@ namespace {
         int32_t *cq = tmp, *ck = cq + kRanked + 1, *key = tmp + 2 * kRanked + 4;
         for (int i = threadIdx.x; i <= (int) p.nseq; i += blockDim.x) cq[i] = p.cu_q[i], ck[i] = p.cu_k[i];
         __syncthreads();
-        const int pad = (p.ranked + 3) / 4 * 4;
+        const int pad = (p.units + 3) / 4 * 4;
         int       n   = 0;
         for (int u0 = 0; u0 < pad; u0 += blockDim.x) {
             const int u = u0 + threadIdx.x;
             int       k = -1;
-            if (u < p.ranked) {
+            if (u < p.units) {
                 const PackedUnit x = packed_unit<QT, kRows>(p, cq, ck, u);
                 if (x.sq > 0) k = x.n[0] + x.n[1];
             }
             if (u < pad) key[u] = k;
             n += __syncthreads_count(k >= 0);
         }
-        for (int u = threadIdx.x; u < p.ranked; u += blockDim.x) {
+        for (int u = threadIdx.x; u < p.units; u += blockDim.x) {
             const int k = key[u];
             if (k < 0) continue;
             int rank = 0;
@@ -325,7 +331,7 @@ namespace {
         // barriers: q_full, q_read, k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full[QT], p_full[QT][kPParts], o_final[QT]
         static constexpr int nBar = 2 + 2 * KS + 2 * VS + QT * (2 + kPParts);
         static constexpr uint32_t oCtl  = oBar + 8 * nBar;
-        static constexpr uint32_t oCached = oCtl + 16, oOrder = oCached + kCached * sizeof(PackedUnit); // packed sequences only
+        static constexpr uint32_t oPackBar = oCtl + 16, oCached = oPackBar + 32, oOrder = oCached + kCached * sizeof(PackedUnit); // packed sequences only
         static constexpr uint32_t total = oCtl + 16 + 1024, total_packed = oOrder + kRanked * 2 + 1024;
     };
 
@@ -412,7 +418,7 @@ namespace {
         static_assert(KS == 2 && VS == 2, "stage selection assumes two-stage rings");
         using L               = Smem<D, KS, VS, QT>;
         constexpr int kQTiles = QT, kThreads = threads_for(QT);
-        constexpr int kWarpTma = 4 * QT, kWarpMma = 4 * QT + 1; // the other two warps of the control warpgroup only give up registers
+        constexpr int kWarpTma = 4 * QT, kWarpMma = 4 * QT + 1; // the other two warps of the control warpgroup only give up registers (packed: one looks rounds up)
         constexpr int kTmemCols = QT == 2 ? 512 : 256;
         // Register re-partitioning. The CTA is launched with kRegsBase registers per thread (what the launch bounds allow);
         // setmaxnreg.inc blocks in hardware until the CTA's own pool holds the registers, so the control warpgroup must
@@ -445,6 +451,8 @@ namespace {
         if (threadIdx.x == (kWarpMma + 1) * 32) { // a thread of an idle warp, so that the set-up runs beside the look-up above
             for (int i = 0; i < L::nBar; ++i) ptx::mbar_init(bar(i), (i >= bPF && i < bOF) ? 4 : 1); // p_full: one arrival per softmax warp of the tile
             ctl[1] = 0;
+            if constexpr (kPacked)
+                for (int i = 0; i < 4; ++i) ptx::mbar_init(base + L::oPackBar + 8u * (uint32_t) i, i < 2 ? 1 : 4 * QT + 2); // all softmax warps, the producer, the issuer
             ptx::fence_mbar_init();
             ptx::prefetch_tmap(&tmQ);
             ptx::prefetch_tmap(&tmK);
@@ -460,17 +468,32 @@ namespace {
         constexpr int     kHeads = kPair ? 2 : 1; // query heads of a unit
         if constexpr (kPacked) {
             vkc_grid_dep_wait(); // the offsets may be the previous kernel's
-            if (p.ranked) {
+            if (p.units > kRanked) {
+                for (int r = threadIdx.x; r < kCached; r += blockDim.x) cached[r] = packed_round<QT, kRows>(p, cta, p.cu_q, p.cu_k, order, p.units, kHeads, r);
+                if (threadIdx.x == 0) ctl[2] = p.units;
+            } else if (p.units) {
                 const int n = packed_rank<QT, kRows>(p, cta, kHeads, (int *) (gbase + L::oQ), order, cached);
                 if (threadIdx.x == 0) ctl[2] = n;
                 ptx::fence_proxy_async(); // the scratch of the ranking lies where the Q tiles will be copied to
             } else if (threadIdx.x == (kWarpMma + 2) * 32) {
                 PackedUnit x = packed_unit<QT, kRows>(p, p.cu_q, p.cu_k, cta.x);
-                x.h = cta.y * kHeads, x.last = 1;
+                x.h = x.sq > 0 ? cta.y * kHeads : -1, x.last = 1;
                 cached[0] = x;
             }
         }
-        auto unit_at = [&](int pos) { return pos < kCached ? cached[pos] : packed_round<QT, kRows>(p, cta, p.cu_q, p.cu_k, order, ctl[2], kHeads, pos); };
+        auto unit_at = [&](int pos) { return cached[pos % kCached]; };
+        // Halves of the ring: [0, 1] described, [2, 3] no longer needed by any role. Half number c holds the rounds from c * kHalf on.
+        auto half_bar = [&](int i) { return base + L::oPackBar + 8u * (uint32_t) i; };
+        // A role goes on to round `pos`: by a whole warp, or by one thread (`solo`).
+        auto enter = [&](int pos, bool solo) {
+            if (pos % kHalf) return true;
+            const int c = pos / kHalf;
+            if (!solo) __syncwarp();
+            if (solo || lane == 0) ptx::mbar_arrive(half_bar(2 + ((c - 1) & 1)));
+            if (c < 2) return true;
+            const bool there = ptx::mbar_wait(half_bar(c & 1), (uint32_t) ((c / 2 - 1) & 1), ctl + 1, p.dev_err, kRingLimit);
+            return solo ? there : (bool) __all_sync(0xffffffffu, there);
+        };
         auto look_up = [&](int pos) { // packed: behind the set-up barrier only
             if constexpr (kPacked) return packed_item<QT>(unit_at(pos));
             else return work_at<QT>(p, pos, cta);
@@ -480,7 +503,11 @@ namespace {
         else w_first = look_up(0);
         // the item after `cur` (which began at step `pos` minus its length); none behind the CTA's last
         auto next_work = [&](const Item &cur, int pos) {
-            if (!cur.last) return look_up(pos);
+            if constexpr (kPacked) {
+                if (!cur.last && enter(pos, true)) return look_up(pos);
+            } else {
+                if (!cur.last) return look_up(pos);
+            }
             Item none;
             none.valid = false;
             return none;
@@ -579,8 +606,8 @@ namespace {
                     if (nv >= BN || nv % 16 == 0) return;
                     const uint32_t v = sV + (uint32_t) (g & 1) * L::KV_BYTES;
                     const int      rows = ksteps * 16 - nv;
-                    for (int i = threadIdx.x & 31; i < rows * DCH * 8; i += 32)
-                        ptx::st_shared_v4(v + (uint32_t) (i / (rows * 8)) * (BN * 128) + (uint32_t) (nv * 128 + i % (rows * 8) * 16), 0u, 0u, 0u, 0u);
+                    for (int i = lane; i < rows * DCH * 8; i += 32)
+                        ptx::st_shared_v4(v + (uint32_t) (i % DCH * (BN * 128) + nv * 128 + i / DCH * 16), 0u, 0u, 0u, 0u);
                     ptx::fence_proxy_async();
                     __syncwarp();
                 };
@@ -597,78 +624,83 @@ namespace {
                 // softmax warps of tile t still store the rows. The two tiles stay half a step apart across items.
                 struct Steps { // what the issuer needs of an item
                     int n, len, both; // key tiles, keys of the sequence, whether the second query tile has rows
+                    int half;         // the half of the ring that follows its own
                 };
                 int  pos  = 0; // the round after the item at hand
-                auto next = [&](Steps &x) { // the next round that has keys (n == 0: there is none)
-                    for (;;) {
+                auto next = [&](Steps &x, int upto) { // the next round that has keys, of the halves up to `upto` (n == 0: there is none)
+                    for (x.n = 0; x.n == 0 && pos != INT32_MAX && pos / kHalf <= upto;) {
+                        if (pos > 0 && !enter(pos, false)) {
+                            pos = INT32_MAX;
+                            break;
+                        }
                         const PackedUnit u = unit_at(pos);
-                        x.n = u.sq > 0 ? u.n[0] : 0, x.len = u.sk, x.both = QT == 2 && u.n[QT - 1] > 0;
-                        if (u.sq <= 0 || u.last) pos = INT32_MAX;
-                        else ++pos;
-                        if (x.n > 0 || pos == INT32_MAX) return;
+                        x.n = u.h >= 0 && u.sq > 0 ? u.n[0] : 0, x.len = u.sk, x.both = QT == 2 && u.n[QT - 1] > 0, x.half = pos / kHalf + 1;
+                        pos = u.h < 0 || u.last ? INT32_MAX : pos + 1;
                     }
                 };
-                Steps s;
-                next(s);
-                if (s.n > 0) {
-                    ok = wait(bKF, 0u) && wait(bQ, 0u);
+                int g = 0; // key tiles so far
+                for (Steps s; ok;) { // a stream
+                    next(s, INT32_MAX);
+                    if (s.n == 0) break;
+                    ok = wait(bKF + (g & 1), (uint32_t) ((g >> 1) & 1)) && wait(bQ, (uint32_t) (cq & 1));
                     if (ok) {
                         ptx::tc_fence_after();
-                        issue_qk(0, 0);
-                        if (s.both) issue_qk(QT - 1, 0);
+                        issue_qk(0, g);
+                        if (s.both) issue_qk(QT - 1, g);
                         if (leader) {
-                            ptx::tc_commit(bar(bKE));
+                            ptx::tc_commit(bar(bKE + (g & 1)));
                             if (s.n == 1) ptx::tc_commit(bar(bQE));
                         }
                     }
-                }
-                int g = 0; // key tiles so far
-                while (ok && s.n > 0) {
-                    Steps ns; // the item behind this one
-                    ns.n = 0;
-                    for (int j = 0; j < s.n && ok; ++j, ++g) {
-                        const int  vs   = g & 1;
-                        const bool last = j + 1 == s.n;
-                        if (last && pos != INT32_MAX) next(ns);
-                        const bool more = !last || ns.n > 0; // another Q.K^T follows
-                        ok = wait(bVF + vs, (uint32_t) ((g >> 1) & 1));
-                        if (!ok) break;
-                        clear_tail(s.len - j * BN, g);
+                    while (ok && s.n > 0) {
+                        Steps ns; // the item behind this one
+                        ns.n = 0;
+                        for (int j = 0; j < s.n && ok; ++j, ++g) {
+                            const int  vs   = g & 1;
+                            const bool last = j + 1 == s.n;
+                            // (Only as far as the other roles can follow: they are held up at this item until its P.V are issued, and the
+                            // ring's half behind the next one is described when they have left this one.)
+                            if (last) next(ns, s.half);
+                            const bool more = !last || ns.n > 0; // another Q.K^T follows
+                            ok = wait(bVF + vs, (uint32_t) ((g >> 1) & 1));
+                            if (!ok) break;
+                            clear_tail(s.len - j * BN, g);
 #pragma unroll
-                        for (int t = 0; t < kQTiles && ok; ++t) {
-                            if (t == 0 || s.both) {
-                                const uint32_t pp = (uint32_t) (cs[t] & 1);
+                            for (int t = 0; t < kQTiles && ok; ++t) {
+                                if (t == 0 || s.both) {
+                                    const uint32_t pp = (uint32_t) (cs[t] & 1);
 #pragma unroll
-                                for (int part = 0; part < kPParts && ok; ++part) {
-                                    ok = wait(bPF + kPParts * t + part, pp);
-                                    if (ok) {
-                                        ptx::tc_fence_after();
-                                        issue_pv(t, j, g, part);
+                                    for (int part = 0; part < kPParts && ok; ++part) {
+                                        ok = wait(bPF + kPParts * t + part, pp);
+                                        if (ok) {
+                                            ptx::tc_fence_after();
+                                            issue_pv(t, j, g, part);
+                                        }
                                     }
+                                    if (!ok) break;
+                                    ++cs[t];
+                                    if (last && leader) ptx::tc_commit(bar(bOF + t)); // O_t complete
                                 }
-                                if (!ok) break;
-                                ++cs[t];
-                                if (last && leader) ptx::tc_commit(bar(bOF + t)); // O_t complete
+                                if (more && (t == 0 || (last ? ns.both : s.both))) {
+                                    ok = wait(bKF + ((g + 1) & 1), (uint32_t) (((g + 1) >> 1) & 1)) && (!last || wait(bQ, (uint32_t) ((cq + 1) & 1)));
+                                    if (!ok) break;
+                                    ptx::tc_fence_after();
+                                    issue_qk(t, g + 1);
+                                }
                             }
-                            if (more && (t == 0 || (last ? ns.both : s.both))) {
-                                ok = wait(bKF + ((g + 1) & 1), (uint32_t) (((g + 1) >> 1) & 1)) && (!last || wait(bQ, (uint32_t) ((cq + 1) & 1)));
-                                if (!ok) break;
-                                ptx::tc_fence_after();
-                                issue_qk(t, g + 1);
-                            }
-                        }
-                        if (!ok) break;
-                        if (leader) {
-                            ptx::tc_commit(bar(bVE + vs));
-                            if (more) {
-                                ptx::tc_commit(bar(bKE + ((g + 1) & 1)));
-                                // the last Q.K^T MMAs of their item are issued: Q may be replaced
-                                if (last ? ns.n == 1 : j + 2 == s.n) ptx::tc_commit(bar(bQE));
+                            if (!ok) break;
+                            if (leader) {
+                                ptx::tc_commit(bar(bVE + vs));
+                                if (more) {
+                                    ptx::tc_commit(bar(bKE + ((g + 1) & 1)));
+                                    // the last Q.K^T MMAs of their item are issued: Q may be replaced
+                                    if (last ? ns.n == 1 : j + 2 == s.n) ptx::tc_commit(bar(bQE));
+                                }
                             }
                         }
+                        ++cq;
+                        s = ns;
                     }
-                    ++cq;
-                    s = ns;
                 }
               } else {
                 for (int pos = 0; ok; w = next_work(w, pos)) {
@@ -733,6 +765,21 @@ namespace {
                     ++cq;
                 }
               }
+            }
+          } else if (kPacked && warp == kWarpMma + 1 && p.units) {
+            // ------------------------------------------------------------------ look-up of the rounds behind the first kCached
+            bool more = cached[kCached - 1].h >= 0 && !cached[kCached - 1].last;
+            for (int c = 2; more; ++c) {
+                if (!__all_sync(0xffffffffu, ptx::mbar_wait(half_bar(2 + (c & 1)), (uint32_t) ((c / 2 - 1) & 1), ctl + 1, p.dev_err, kRingLimit))) break;
+                PackedUnit x;
+                x.h = -1;
+                if (lane < kHalf) {
+                    x = packed_round<QT, kRows>(p, cta, p.cu_q, p.cu_k, order, ctl[2], kHeads, c * kHalf + lane);
+                    cached[(c & 1) * kHalf + lane] = x;
+                }
+                more = __all_sync(0xffffffffu, lane >= kHalf || (x.h >= 0 && !x.last));
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(half_bar(c & 1));
             }
           }
         } else {
@@ -1085,6 +1132,8 @@ namespace {
                 ptx::tc_fence_before();
             }
             if (w.last) break;
+            if constexpr (kPacked)
+                if (!enter(pos, false)) break;
             prepare(look_up(pos));
           }
         }
@@ -1303,11 +1352,15 @@ namespace {
         constexpr int smem = (int) Smem<D, 2, 2, QT>::total_packed, rows = kPair ? BM : QT * BM;
         static_assert(smem * (QT == 1 && D == 64 ? 2 : 1) <= 227 * 1024, "shared memory budget");
         if (int rc = vkc_configure_smem(ctx, kern, smem)) return rc;
-        // unit numbers of a head or pair of heads (a few of them empty); persistent CTAs when they are more than fit the SMs at once
+        // Unit numbers of a head or pair of heads (a few of them empty). Persistent CTAs when they are more than fit the SMs at once, and
+        // either few enough to rank or not mostly of very long sequences: next to a CTA for each unit they save the set-up, but
+        // without a ranking they do not even out lengths. 1000 sequences of 20 to 40 tokens 440 us against 950, 600 of 10 to 500
+        // 1110 against 1850, 24 of 1000 to 4000 1650 against 1720, 12 of 4000 to 10000 5.78 ms against 5.86; but 8 of 8000 to
+        // 20000 16.7 ms against 15.9.
         const int64_t units = p.Sq / rows + p.nseq, slots = (int64_t) ctx->sm_count * (QT == 1 ? 2 : 1);
         p.turns             = (int) (kPair ? p.Hq / 2 : p.Hq);
         dim3 grid((unsigned) units, (unsigned) p.turns, 1);
-        if (units * p.turns > slots && units <= kRanked) p.ranked = (int) units, grid = dim3((unsigned) slots, 1, 1);
+        if (units * p.turns > slots && (units <= kRanked || units <= 64 * p.nseq) && units * p.turns < 1 << 30) p.units = (int) units, grid = dim3((unsigned) slots, 1, 1);
         vkc_launch(ctx, kern, grid, dim3(threads_for(QT)), smem, st, tq, tk, tv, p);
         return vkc_post_launch(ctx, "attn_prefill_packed_tcgen05");
     }

@@ -53,13 +53,13 @@ namespace ptx {
     constexpr long long kWaitLimitCycles = 2000000000LL; // ~1 s at 2 GHz
 
     // Bounded wait. `abort_flag` lives in shared memory and is shared by every waiter of the CTA.
-    __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *dev_err) {
+    __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *dev_err, long long limit = kWaitLimitCycles) {
         if (mbar_try_wait(bar, parity)) return true;
         const long long t0 = clock64();
         for (;;) {
             if (mbar_try_wait(bar, parity)) return true;
             if (*abort_flag) return false;
-            if (clock64() - t0 > kWaitLimitCycles) {
+            if (clock64() - t0 > limit) {
                 *abort_flag = 1;
                 atomicCAS(dev_err, 0, 1 /* VKC_DEVERR_WAIT_TIMEOUT */);
                 return false;
