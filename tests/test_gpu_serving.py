@@ -281,6 +281,37 @@ def test_packed_long_runs_of_sequences_without_keys(ctx, hq, hkv, d, nseq, hi, s
     check_like_simt(ctx, lq, [5] + [0] * (nseq - 1), hq, hkv, d, causal)
 
 
+@pytest.mark.parametrize("nseq,hi", [(120, 90), (700, 20)], ids=["ranked", "unranked"])
+def test_packed_many_sequences_replayed_with_other_offsets(ctx, nseq, hi):
+    hq, hkv, d, r = 32, 8, 64, np.random.default_rng(6)
+    first = [int(x) for x in r.integers(0, hi + 1, nseq)]
+    total = sum(first)
+    q, k, v = packed_case(14, first, first, hq, hkv, d, torch.float16)
+    cu, o, want = offsets(first), torch.zeros_like(q), torch.zeros_like(q)
+    ctx.attn_prefill_packed(q, k, v, o, d ** -0.5, cu)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ctx.attn_prefill_packed(q, k, v, o, d ** -0.5, cu)
+    far = 2.0 ** -32 * float(v.double().abs().sum(0).max())
+    cuts = [sorted(int(x) for x in r.integers(0, total + 1, nseq - 1)) for _ in range(2)] + [[total] * (nseq - 1), [0] * (nseq - 1)]
+    for cut in cuts:
+        cu.copy_(torch.tensor([0] + cut + [total], dtype=torch.int32))
+        graph.replay()
+        ctx.attn_prefill_packed(q, k, v, want, d ** -0.5, cu)  # launched, not replayed
+        torch.cuda.synchronize()
+        assert torch.equal(o, want)
+        ctx.set_impl(vknn_b200.IMPL_SIMT)
+        a = torch.zeros_like(q)
+        ctx.attn_prefill_packed(q, k, v, want, d ** -0.5, cu)
+        ctx.attn_prefill_packed(q, k, v.abs(), a, d ** -0.5, cu)
+        ctx.set_impl(vknn_b200.IMPL_AUTO)
+        ctx.sync()
+        # both within half a step of fp16 and of P in fp16 of the exact value, which loses 2^-32 |v| per key where P is subnormal
+        u = half_step(torch.float16)
+        w, s = want.double(), a.double() * (1 + 2 * u)
+        assert bool(((o.double() - w).abs() <= 2 * u * w.abs() * (1 + u) + (u + 2 * SMALL) * s * (1 + u) + 1.2e-7 + far).all())
+
+
 def test_packed_a_sequence_of_more_units_than_are_ranked(ctx):
     check_like_simt(ctx, [66000, 40], [66000, 40], 2, 1, 64)
     check_like_simt(ctx, [40, 33100, 1], [50, 33100, 900], 2, 2, 128)
