@@ -34,7 +34,7 @@
 // finished and O_t may be rescaled; Q.K_t(j+1) overwrites the columns P_t(j) lives in and is issued after
 // P.V_t(j) by the same thread, which the tensor pipe executes in order.
 // Packed sequences (kPack): the same kernel with units looked up in the sequence offsets, see AttnParams, PackedUnit and the issuer's
-// loop. 16 x 1024 tokens, 32/8 heads x 128, causal: 172 us (800 TFLOP/s), the dense call 292; 4 x 4096: 490 us (1120), dense 530.
+// loop. 16 x 1024 tokens, 32/8 heads x 128, causal: 169 us (815 TFLOP/s), the dense call 292; 4 x 4096: 481 us (1140), dense 530.
 // Masking: keys >= kv_len[b] (or >= Skv) and, for causal, keys > row + (Skv - Sq) get probability 0; key tiles
 // entirely above a query tile's diagonal are skipped for that tile.
 #include <type_traits>
