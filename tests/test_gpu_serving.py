@@ -748,8 +748,9 @@ def test_decode_q8_maximum_grows_late(impl_ctx):
     check_decode(impl_ctx, queries(14, 2, 4, 64, "f16"), cache, [2048, 1999], 0.125)
 
 
-def test_decode_q8_same_bits_again_with_a_workspace_on_a_stream_and_in_a_graph(ctx):
-    b, hq, hkv, lmax, d, block = 5, 8, 2, 4096, 128, 64
+@pytest.mark.parametrize("lmax", [4096, 768])  # (lengths beyond the cache count as its length)
+def test_decode_q8_same_bits_again_with_a_workspace_on_a_stream_and_in_a_graph(ctx, lmax):
+    b, hq, hkv, d, block = 5, 8, 2, 128, 64
     cache, q = filled(15, b, hkv, lmax, d, block, "e4m3"), queries(16, b, hq, d, "bf16")
     lens = torch.tensor([4096, 1, 0, 3000, 777], dtype=torch.int32, device="cuda")
     want = torch.zeros_like(q)
@@ -789,17 +790,18 @@ def test_decode_q8_more_sequences_than_one_launch_holds(ctx):
     check_decode(ctx, q, cache, lens, d ** -0.5)
 
 
-def test_decode_q8_two_calls_at_once(ctx):
+@pytest.mark.parametrize("lmax", [4096, 1024])
+def test_decode_q8_two_calls_at_once(ctx, lmax):
     """Two streams, a workspace each; and one after the other on two streams with the context's own scratch."""
     d, block = 128, 64
-    cases = [(filled(19 + i, 3, 2, 4096, d, block, "e4m3"), queries(21 + i, 3, 8, d, "f16"), torch.tensor([4000 - 900 * i, 77, 3000], dtype=torch.int32, device="cuda")) for i in range(2)]
+    cases = [(filled(19 + i, 3, 2, lmax, d, block, "e4m3"), queries(21 + i, 3, 8, d, "f16"), torch.tensor([4000 - 900 * i, 77, 3000], dtype=torch.int32, device="cuda")) for i in range(2)]
     want = []
     for c, q, lens in cases:
         o = torch.zeros_like(q)
         ctx.attn_decode_q8(q, *c.args, o, d ** -0.5, kv_len=lens)
         ctx.sync()
         want.append(o)
-    need, streams = ctx.attn_decode_q8_workspace_bytes(3, 8, 2, 4096, d), [torch.cuda.Stream() for _ in range(2)]
+    need, streams = ctx.attn_decode_q8_workspace_bytes(3, 8, 2, lmax, d), [torch.cuda.Stream() for _ in range(2)]
     spaces = [torch.empty(need, dtype=torch.uint8, device="cuda") for _ in range(2)]
     torch.cuda.synchronize()
     for own in (True, False):
