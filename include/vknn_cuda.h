@@ -239,6 +239,11 @@ VKC_API size_t vkc_attn_decode_workspace_bytes(int64_t B, int64_t Hq, int64_t Hk
  * VKC_ERR_INVALID for bad arguments. Used by the CPU test that checks exact coverage and the slot bound. */
 VKC_API int vkc_attn_decode_items(int sm_count, int64_t B, int64_t Hq, int64_t Hkv, int64_t Lmax, int64_t D, const int32_t *kv_len_host, int cta,
                                   int32_t *items, int max_items, int32_t *plan);
+/* Who works on the key tiles of a CTA with these items (as vkc_attn_decode_items lists them), in the order they are
+ * streamed, three numbers each: softmax group (0 or 1), score buffer (0 to 3), and which use of that buffer the tile is.
+ * Returns the number of tiles (which may exceed max_tiles), VKC_ERR_INVALID for bad arguments. Used by the CPU test that
+ * checks that a group meets the uses of a buffer one after the other, as its waits need it. */
+VKC_API int vkc_attn_decode_tiles(const int32_t *items, int n_items, int32_t *tiles, int max_tiles);
 VKC_API int    vkc_attn_decode(vkc_ctx *ctx, const void *Q, const void *Kc, const void *Vc, void *O, int64_t B, int64_t Hq, int64_t Hkv,
                                int64_t Lmax, int64_t D, const int32_t *kv_len, float scale, void *workspace, size_t workspace_bytes,
                                int dtype, vkc_stream stream);

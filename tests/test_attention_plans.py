@@ -239,3 +239,42 @@ def test_decode_items_refuses_what_the_kernel_does_not_take():
         capi.attn_decode_items(SMS, 4, 64, 2, 1024, 128)    # 32 query heads per kv head
     with pytest.raises(capi.VkcError):
         capi.attn_decode_items(SMS, 4, 8, 3, 1024, 128)     # Hq not a multiple of Hkv
+
+
+def check_waits(B, Hq, Hkv, Lmax, lens):
+    """A softmax group waits for a use of a score buffer by the parity of its number. Asked for use n + 2 while use n is still to
+    come, such a wait answers at once; so every group has to wait for all uses of the buffers it reads, one after the other."""
+    _, per_cta = capi.attn_decode_items(SMS, B, Hq, Hkv, Lmax, 128, lens)
+    for c, items in enumerate(per_cta):
+        roles = capi.attn_decode_tiles(items)
+        assert len(roles) == sum((it["end"] - it["start"] + 127) // 128 for it in items)
+        seen = {}
+        for g, (group, buffer, use) in enumerate(roles):
+            assert buffer == g % 4 and use == g // 4, (c, g)  # the issuer fills the buffers in turn
+            assert use == seen.get((group, buffer), 0), (c, g, "a group would wait for use %d of buffer %d next, not %d" % (seen.get((group, buffer), 0), buffer, use))
+            seen[group, buffer] = use + 1
+        at = 0
+        for it in items:  # within an item each group has every second tile
+            n = (it["end"] - it["start"] + 127) // 128
+            mine = [g for g, _, _ in roles[at:at + n]]
+            assert all(a != b for a, b in zip(mine, mine[1:])), (c, it)
+            at += n
+
+
+def test_decode_groups_meet_every_use_of_their_buffers():
+    import numpy as np
+    rng = np.random.default_rng(len("many_short"))
+    check_waits(40, 16, 4, 640, [int(x) for x in rng.integers(0, 641, 40)])
+    check_waits(200, 8, 8, 1024, [1] * 100 + [1000] * 100)       # beginnings of many conversations ahead of longer ones
+    check_waits(200, 8, 8, 1024, ([128] * 9 + [129] * 1) * 20)
+    r = random.Random(12)
+    for _ in range(60):
+        B, Hkv = r.choice((1, 3, 40, 200, 600)), r.choice((1, 2, 8))
+        Lmax = r.choice((128, 640, 4096))
+        check_waits(B, Hkv * 4, Hkv, Lmax, [r.choice((0, 1, 100, 128, 129, r.randint(0, Lmax))) for _ in range(B)])
+
+
+def test_decode_tiles_refuses_bad_arguments():
+    lib = capi.load_library()
+    assert lib.vkc_attn_decode_tiles(None, 1, None, 0) == -1 and lib.vkc_attn_decode_tiles(None, -1, None, 0) == -1
+    assert lib.vkc_attn_decode_tiles(None, 0, None, 0) == 0 and capi.attn_decode_tiles([]) == []

@@ -881,3 +881,39 @@ def test_invalid_arguments(ctx):
         ctx.attn_decode(torch.zeros(1, 4, 96, dtype=torch.float16, device="cuda"), torch.zeros(1, 4, 8, 96, dtype=torch.float16, device="cuda"),
                         torch.zeros(1, 4, 8, 96, dtype=torch.float16, device="cuda"), torch.zeros(1, 4, 96, dtype=torch.float16, device="cuda"), 1.0)
     assert ctx.launch_count() == n0
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+def test_decode_short_sequences_ahead_of_longer_ones(ctx, dt):
+    """Runs of sequences of a single key tile ahead of longer ones, as when many conversations begin: a softmax group of the
+    tensor-core kernel meets its score buffers in order whatever the items' lengths are. Against 64 bits: the output's own rounding,
+    that of a probability to the storage type (both half a step) and 2e-4 for 2^x and the fp32 scores; the same bits every time."""
+    t, D, Hkv, G, L = DT[dt], 128, 4, 4, 640
+    u, g, rng = torch.finfo(t).eps / 2, torch.Generator(device="cuda").manual_seed(31), np.random.default_rng(31)
+    cases = [[1] * 60 + [640] * 20, [128] * 30 + [129, 300] * 10, [5, 100, 128, 1, 60, 77, 640] * 12]
+    cases += [[int(x) for x in rng.choice([1, 17, 128, 200, 640], 90, p=[0.3, 0.2, 0.3, 0.1, 0.1])] for _ in range(5)]
+    ctx.set_impl(vknn_b200.IMPL_TCGEN05)
+    try:
+        for lens in cases:
+            B = len(lens)
+            q = torch.randn(B, Hkv * G, D, generator=g, device="cuda").to(t)
+            k, v = (torch.randn(B, Hkv, L, D, generator=g, device="cuda").to(t) for _ in range(2))
+            kv_len = torch.tensor(lens, dtype=torch.int32, device="cuda")
+            hidden = torch.arange(L, device="cuda") >= kv_len[:, None]
+            for x in (k, v):
+                x.masked_fill_(hidden[:, None, :, None], float("nan"))
+            outs = [torch.full_like(q, 7.0) for _ in range(6)]
+            for o in outs:
+                ctx.attn_decode(q, k, v, o, D ** -0.5, kv_len=kv_len)
+            ctx.sync()
+            kd, vd = (x.masked_fill(hidden[:, None, :, None], 0).double() for x in (k, v))
+            s = torch.einsum("bhgd,bhld->bhgl", q.double().reshape(B, Hkv, G, D), kd) * D ** -0.5
+            p = torch.softmax(s.masked_fill(hidden[:, None, None], -torch.inf), -1)
+            ref, a = (torch.einsum("bhgl,bhld->bhgd", p, x).reshape(B, Hkv * G, D) for x in (vd, vd.abs()))
+            # (a probability below 2^-14 of the running maximum, which may lie 2^8 under the true one, is subnormal in f16)
+            far = 2.0 ** -25 * vd.abs().sum(2).repeat_interleave(G, 1) if t == torch.float16 else 0.0
+            off = (outs[0].double() - ref).abs()
+            assert bool((off <= u * ref.abs() + (u + 2e-4) * a + far + 6e-8).all()), lens
+            assert all(torch.equal(o, outs[0]) for o in outs[1:]), lens
+    finally:
+        ctx.set_impl(vknn_b200.IMPL_AUTO)

@@ -81,6 +81,7 @@ def load_library():
     L.vkc_attn_prefill_plan.argtypes = [i32] + [i64] * 5 + [i32, i32, C.POINTER(C.c_int32)]
     L.vkc_attn_prefill_items.argtypes = [i32] + [i64] * 5 + [i32, i32, i32, C.POINTER(C.c_int32), i32]
     L.vkc_attn_decode_workspace_bytes.argtypes = [i64] * 5
+    L.vkc_attn_decode_tiles.argtypes = [C.POINTER(C.c_int32), i32, C.POINTER(C.c_int32), i32]
     L.vkc_attn_decode_items.argtypes = [i32] + [i64] * 5 + [C.POINTER(C.c_int32), i32, C.POINTER(C.c_int32), i32, C.POINTER(C.c_int32)]
     L.vkc_attn_decode_workspace_bytes.restype = sz
     L.vkc_attn_decode.argtypes = [vp, vp, vp, vp, vp] + [i64] * 5 + [vp, f32, vp, sz, i32, vp]
@@ -211,6 +212,18 @@ def attn_decode_items(sm_count, B, Hq, Hkv, Lmax, D, kv_len=None):
         cta += 1
         if cta >= plan[0]:
             return dict(grid=plan[0], slots=plan[1], min_tiles=plan[2]), per_cta
+
+
+def attn_decode_tiles(items):
+    """(softmax group, score buffer, use of the buffer) of every key tile of a CTA with these items (one of attn_decode_items' lists).
+    Host arithmetic; needs no GPU."""
+    lib = load_library()
+    flat = [int(it[f]) for it in items for f in DECODE_ITEM_FIELDS]
+    src = (C.c_int32 * len(flat))(*flat)
+    n = lib.vkc_attn_decode_tiles(src, len(items), None, 0)
+    buf = (C.c_int32 * (3 * n))()
+    lib.vkc_attn_decode_tiles(src, len(items), buf, n)
+    return [tuple(buf[3 * i:3 * i + 3]) for i in range(n)]
 
 
 class Context:

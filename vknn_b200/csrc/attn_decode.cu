@@ -323,6 +323,13 @@ extern "C" int vkc_attn_decode_items(int sm_count, int64_t B, int64_t Hq, int64_
     return n < 0 ? (grid > 0 ? VKC_ERR_INVALID : VKC_ERR_UNSUPPORTED) : n;
 }
 
+int vkc_attn_decode_tc_tiles(const int32_t *items, int n_items, int32_t *tiles, int max_tiles);
+
+extern "C" int vkc_attn_decode_tiles(const int32_t *items, int n_items, int32_t *tiles, int max_tiles) {
+    if (n_items < 0 || (!items && n_items > 0) || (!tiles && max_tiles > 0)) return VKC_ERR_INVALID;
+    return vkc_attn_decode_tc_tiles(items, n_items, tiles, max_tiles);
+}
+
 extern "C" int vkc_attn_decode(vkc_ctx *ctx, const void *Q, const void *Kc, const void *Vc, void *O, int64_t B, int64_t Hq, int64_t Hkv,
                                int64_t Lmax, int64_t D, const int32_t *kv_len, float scale, void *workspace, size_t workspace_bytes, int dtype,
                                vkc_stream stream) {

@@ -15,8 +15,8 @@
 //
 //   warp 0    producer: Q_g tile per item (double buffered), K and V tiles of 128 keys per ring stage.
 //   warp 1    MMA issuer + TMEM owner (S^T x4, O^T x4: 128 columns in all); Q.K^T runs two tiles ahead of P.V.
-//   warps 2-5 softmax group 0 (even tiles of an item), warps 6-9 softmax group 1 (odd tiles). Each group keeps its
-//             own running maximum, row sums and O^T accumulator and emits its own partial, so the two groups never
+//   warps 2-5 softmax group 0 (even tiles of the CTA, counted over all of its items), warps 6-9 softmax group 1 (odd
+//             tiles). Each group keeps its own running maximum, row sums and O^T accumulator and emits its own partial, so the two groups never
 //             exchange data and their latency chains overlap. Thread r of a group owns key r of its current tile (a
 //             TMEM lane of S^T) and, in the item epilogue, output dimension r (a TMEM lane of O^T). Per tile: read 16 columns of S^T, per-head maximum over the
 //             tile (warp shuffles + one shared-memory exchange), lazily raised running maximum, p = exp2(s*scale*log2e - m),
@@ -114,6 +114,17 @@ namespace {
         it.valid            = true;
         return it;
     }
+
+    // Who works on tile g of a CTA (counted over all of its items): the softmax groups take turns, whatever item the tile is
+    // of, and so do the score buffers, four tiles each. A group thus meets the uses of "its" two buffers one after the other,
+    // which the waits need: a barrier is asked for the parity of a phase, and a group that left uses out (one that sat out
+    // items of a single tile, with the turns counted within the item) would ask two phases ahead and be let through at once.
+    struct TileRole {
+        int group, buffer, use; // softmax group, score buffer and which use of that buffer it is
+    };
+    __host__ __device__ __forceinline__ TileRole tile_role(int64_t g) { return {(int) (g & 1), (int) (g & 3), (int) (g >> 2)}; }
+    // First tile, within an item that begins at tile g0, of softmax group wg (every second one follows): 0 or 1.
+    __host__ __device__ __forceinline__ int first_tile(int wg, int64_t g0) { return wg ^ tile_role(g0).group; }
 
     __device__ __forceinline__ float fast_exp2(float x) {
         float y;
@@ -250,7 +261,7 @@ namespace {
                 };
                 int  pc[2] = {0, 0}; // items each softmax group has taken part in so far (selects its O^T buffer)
                 auto issue_pv = [&](const Cur &c) -> bool {
-                    const int s = (int) (c.g % kStages), pb = (int) (c.g & 3), wg = c.t & 1, ob = pc[wg] & 1;
+                    const int s = (int) (c.g % kStages), pb = (int) (c.g & 3), wg = tile_role(c.g).group, ob = pc[wg] & 1;
                     if (c.t < 2 && !ptx::mbar_wait(bar(bOE + wg * 2 + ob), (uint32_t) (((pc[wg] >> 1) & 1) ^ 1), ctl + 1, p.dev_err)) return false;
                     if (!ptx::mbar_wait(bar(bVF + s), (uint32_t) ((c.g / kStages) & 1), ctl + 1, p.dev_err)) return false;
                     if (!ptx::mbar_wait(bar(bPF + pb), (uint32_t) ((c.g >> 2) & 1), ctl + 1, p.dev_err)) return false;
@@ -314,8 +325,9 @@ namespace {
                 if (!it.valid) break;
                 pos += it.ntiles;
                 if (it.last && wg == 0 && r == 0) p.nslots[it.b * p.Hkv + it.hk] = 2 * (it.split + 1);
-                const int64_t prow = ((int64_t) it.b * Hq + (int64_t) it.hk * G) * p.parts_stride + (int64_t) it.split * 2 + wg;
-                if (wg >= it.ntiles) {
+                const int     t0   = first_tile(wg, g0); // also the partial's place in the pair: that of the item's tiles t0, t0 + 2, ...
+                const int64_t prow = ((int64_t) it.b * Hq + (int64_t) it.hk * G) * p.parts_stride + (int64_t) it.split * 2 + t0;
+                if (t0 >= it.ntiles) {
                     // this group has no tile in the item: an empty partial (weight 0 in the merge)
                     for (int h = 0; h < G; ++h) {
                         p.part_o[(prow + (int64_t) h * p.parts_stride) * DH + r] = 0.f;
@@ -335,10 +347,10 @@ namespace {
                     m[h]  = -INFINITY;
                     lp[h] = 0.f;
                 }
-                for (int t = wg; t < it.ntiles; t += 2, ++cnt) {
+                for (int t = t0; t < it.ntiles; t += 2, ++cnt) {
                     const int64_t g  = g0 + t;
-                    const int     sb = (int) (g & 3), rb = (int) (cnt & 1);
-                    ok = ptx::mbar_wait(bar(bSF + sb), (uint32_t) ((g >> 2) & 1), ctl + 1, p.dev_err);
+                    const int     sb = tile_role(g).buffer, rb = (int) (cnt & 1);
+                    ok = ptx::mbar_wait(bar(bSF + sb), (uint32_t) (tile_role(g).use & 1), ctl + 1, p.dev_err);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     ptx::tc_fence_after();
@@ -511,6 +523,26 @@ int vkc_attn_decode_tc_items(int sm_count, int64_t B, int64_t Hq, int64_t Hkv, i
         }
         ++n;
         pos += it.ntiles;
+    }
+    return n;
+}
+
+// The tiles of the CTA whose items are given (as above), three numbers each: softmax group, score buffer, use of that buffer.
+// Returns their number, which may exceed max_tiles.
+int vkc_attn_decode_tc_tiles(const int32_t *items, int n_items, int32_t *tiles, int max_tiles) {
+    int n = 0;
+    for (int i = 0; i < n_items; ++i) {
+        const int64_t g0 = n;
+        const int     nt = (items[6 * i + 3] - items[6 * i + 2] + TK - 1) / TK;
+        for (int wg = 0; wg < 2; ++wg)
+            for (int t = first_tile(wg, g0); t < nt; t += 2) {
+                const TileRole x = tile_role(g0 + t);
+                if (g0 + t < max_tiles) {
+                    int32_t *row = tiles + 3 * (g0 + t);
+                    row[0] = wg, row[1] = x.buffer, row[2] = x.use;
+                }
+            }
+        n += nt;
     }
     return n;
 }
