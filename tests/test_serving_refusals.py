@@ -146,3 +146,19 @@ def test_decode_refusals(fake):
     with pytest.raises(ValueError):
         fake.attn_decode_q8(q, *c, z(2, 4, 64), 1.0, kv_len=lens)
     assert not fake.lib.calls
+
+
+def test_argument_structs_are_as_long_as_the_c_compilers(tmp_path):
+    """The library copies its argument struct whole, the padding at its end included."""
+    if not shutil.which("gcc"):
+        pytest.skip("no C compiler")
+    inc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    structs = {"attn_prefill_packed": capi.PACKED_ARGS, "kv_append_q8": capi.APPEND_ARGS, "attn_decode_q8": capi.DECODE_Q8_ARGS}
+    src, exe = tmp_path / "t.c", tmp_path / "t"
+    src.write_text('#include <stdio.h>\n#include "vknn_cuda.h"\nint main(void) {\n%s return 0; }\n' %
+                   "".join('printf("%s %%d\\n", (int) sizeof(vkc_%s_args));\n' % (n, n) for n in structs))
+    subprocess.check_call(["gcc", "-std=c99", "-Wall", "-Werror", "-I", inc, str(src), "-o", str(exe)])
+    sizes = dict(line.split() for line in subprocess.check_output([str(exe)], text=True).splitlines())
+    assert {n: int(x) for n, x in sizes.items()} == {n: s.size for n, s in structs.items()}
+    for s in structs.values():
+        assert s.size % s.__class__("@P").size == 0

@@ -152,10 +152,10 @@ class Gate(C.Structure):
 
 
 # The argument structs of include/vknn_cuda.h. They are packed into a bytes object that is passed by address: one conversion for all
-# fields, where an argument list of that length costs ctypes 2.5 us a call.
-PACKED_ARGS = struct.Struct("@4P6q2P8qf2i")   # vkc_attn_prefill_packed_args
-APPEND_ARGS = struct.Struct("@6P6q2P4q2i")    # vkc_kv_append_q8_args
-DECODE_Q8_ARGS = struct.Struct("@6P6q2PNf2i")  # vkc_attn_decode_q8_args
+# fields, where an argument list of that length costs ctypes 2.5 us a call. "0q": the padding at the end, which the library copies too.
+PACKED_ARGS = struct.Struct("@4P6q2P8qf2i0q")   # vkc_attn_prefill_packed_args
+APPEND_ARGS = struct.Struct("@6P6q2P4q2i0q")    # vkc_kv_append_q8_args
+DECODE_Q8_ARGS = struct.Struct("@6P6q2PNf2i0q")  # vkc_attn_decode_q8_args
 
 PEER_HANDLE_BYTES = 64
 
