@@ -532,6 +532,58 @@ def test_append_onto_scales_of_the_callers_own(ctx):
         append_both(ctx, cache, k, v, [10] * 4)
 
 
+def nearest_e4m3(x, s):
+    """The e4m3 code nearest to x / s, ties to even, by exact comparisons: x is compared with (middle between two codes) * s, of at
+    most 5 + 24 bits, in float64. x: float64 of at most 28 bits, s: float32, broadcast."""
+    values = torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).double().numpy()  # codes 0 to 126, ascending
+    mids = (values[1:] + values[:-1]) / 2
+    a, s = np.broadcast_arrays(np.abs(x), np.asarray(s, dtype=np.float64))
+    code = np.zeros(a.shape, dtype=np.uint8)
+    for c, mid in enumerate(mids):  # from code c on to c + 1
+        code += ((a > mid * s) | ((a == mid * s) & (c % 2 == 1))).astype(np.uint8)
+    return code | (np.signbit(x).astype(np.uint8) << 7)
+
+
+def test_append_e4m3_rounds_once_with_any_scale(ctx):
+    """Scales that are not powers of two: quotients so close to the middle between two codes that they round to it in fp32."""
+    r, hkv, b, d, block = np.random.default_rng(17), 64, 4, 64, 32
+    # new rows beside a token whose block has such a scale
+    s = (2.0 ** r.integers(-20, 20, (b, hkv)) * r.uniform(1.0, 2.0, (b, hkv))).astype(np.float32)
+    mid = np.array([17, 19, 21, 23, 25, 27, 29, 31, 1.0625, 1.1875, 3.25, 5.75, 0.4375 + 1 / 64, 3 * 2.0 ** -10, 2.0 ** -10, 5 * 2.0 ** -10], dtype=np.float64)
+    x = (mid * s[..., None].astype(np.float64)).astype(np.float32)
+    x = np.concatenate([x, np.nextafter(x, np.float32(0)), np.nextafter(x, np.float32(np.inf)), -x], -1)  # [b, hkv, 64]
+    cache = Cache(b, hkv, block, d, block, "e4m3")
+    cache.ks.copy_(torch.from_numpy(s)[..., None])
+    cache.vs.copy_(torch.from_numpy(s)[..., None])
+    k, one = torch.from_numpy(x).cuda(), torch.ones(b, dtype=torch.int32, device="cuda")
+    ctx.kv_append_q8(k, -k, *cache.args, one)
+    ctx.sync()
+    for t, y in ((cache.k, x), (cache.v, -x)):
+        got, want = t[:, :, 1].view(torch.uint8).cpu().numpy(), nearest_e4m3(y.astype(np.float64), s[..., None])
+        assert np.array_equal(got, want), int((got != want).sum())
+    assert np.array_equal(cache.ks[..., 0].cpu().numpy(), s)
+    # older codes whose scale grows to a power of two
+    v = 1 + np.arange(1, 8, dtype=np.float64) / 8
+    pairs = [(m, c) for m in mid[:8] / 16 for c in v if m < c][: b * hkv]
+    s = np.array([np.float32(m / c) for m, c in pairs], dtype=np.float32)
+    s = np.concatenate([s, np.nextafter(s, np.float32(0)), np.nextafter(s, np.float32(1))])
+    s = np.resize(s, (b, hkv))
+    held = np.resize(np.concatenate([np.arange(0x20, 0x50), 0x80 + np.arange(0x30, 0x40)]), d).astype(np.uint8)
+    cache = Cache(b, hkv, block, d, block, "e4m3")
+    for t, z in ((cache.k, cache.ks), (cache.v, cache.vs)):
+        t.view(torch.uint8)[:, :, 0] = torch.from_numpy(held).cuda()
+        z.copy_(torch.from_numpy(s)[..., None])
+    k = torch.full((b, hkv, d), 300.0, device="cuda")  # asks for the scale 1
+    ctx.kv_append_q8(k, k, *cache.args, one)
+    ctx.sync()
+    assert bool((cache.ks == 1).all()) and bool((cache.vs == 1).all())
+    value = torch.from_numpy(held).view(torch.float8_e4m3fn).double().numpy()
+    want = nearest_e4m3(value * s[..., None].astype(np.float64), np.float32(1))
+    for t in (cache.k, cache.v):
+        got = t[:, :, 0].view(torch.uint8).cpu().numpy()
+        assert np.array_equal(got, want), int((got != want).sum())
+
+
 def test_append_rows_that_do_not_fit_and_idle_sequences(ctx):
     cache = Cache(5, 2, 64, 64, 32, "e4m3")
     k, v = rows(5, 5, 2, 64, torch.float16)

@@ -44,8 +44,14 @@ namespace q8 {
     }
     __device__ __forceinline__ int clamp127(int v) { return v > 127 ? 127 : (v < -127 ? -127 : v); }
 
+    // `q`, the quotient that was asked for cut off towards zero, with its last bit set when something was cut off. Rounded to fewer bits
+    // (two at least) from there it gives what the exact quotient gives: a value in the middle between two codes has that bit clear,
+    // so one beside the middle keeps its side.
+    __device__ __forceinline__ float odd(float q, bool cut) { return __uint_as_float(__float_as_uint(q) | (cut ? 1u : 0u)); }
+
     // x / s to the nearest code, ties to even. A scale that this library wrote is a power of two for e4m3, so that the product with
-    // its reciprocal is exact; any other one (a caller's own cache) takes the quotient rounded to fp32. int8: the product with the
+    // its reciprocal is exact; any other one (a caller's own cache) takes the quotient cut off to fp32 (odd; the product that tells
+    // whether something was cut off is exact in double: 24 bits by 24). int8: the product with the
     // rounded reciprocal names a code k that is at most one off, and the remainder x - k * s, which is exact in fp32 (both terms
     // are multiples of 2^-24 of the power of two above s, and their difference is below s), says whether it is the nearest.
     template <bool kE4m3> struct Quant {
@@ -63,8 +69,8 @@ namespace q8 {
             if (kE4m3) {
                 if (exact)
                     return make_uint2(e4m3x4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv), e4m3x4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv));
-                return make_uint2(e4m3x4(__fdiv_rn(x[0], s), __fdiv_rn(x[1], s), __fdiv_rn(x[2], s), __fdiv_rn(x[3], s)),
-                                  e4m3x4(__fdiv_rn(x[4], s), __fdiv_rn(x[5], s), __fdiv_rn(x[6], s), __fdiv_rn(x[7], s)));
+                return make_uint2(e4m3x4(quotient(x[0]), quotient(x[1]), quotient(x[2]), quotient(x[3])),
+                                  e4m3x4(quotient(x[4]), quotient(x[5]), quotient(x[6]), quotient(x[7])));
             }
             constexpr float kMagic = 12582912.0f;
             const float     half   = 0.5f * s;
@@ -86,12 +92,17 @@ namespace q8 {
             }
             return make_uint2(bytes(z[0], z[1], z[2], z[3]), bytes(z[4], z[5], z[6], z[7]));
         }
+        __device__ __forceinline__ float quotient(float x) const {
+            const float q = __fdiv_rz(x, s);
+            return odd(q, (double) q * (double) s != (double) x);
+        }
         static __device__ __forceinline__ uint32_t bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { // the low byte of each
             return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
         }
     };
 
-    // code * s_old / s to the nearest code, s > s_old >= 0. e4m3 with powers of two: the product is exact. int8: as above, the
+    // code * s_old / s to the nearest code, s > s_old >= 0. e4m3 with powers of two: the product is exact; with others the quotient of
+    // the product (28 bits) is cut off in double, whose remainder is exact, and then to fp32. int8: as above, the
     // close cases in double, where the quotient of the 31-bit product by the 24-bit scale keeps its side of the middle.
     template <bool kE4m3> struct Requant {
         float  ratio;
@@ -108,7 +119,10 @@ namespace q8 {
         }
         __device__ __forceinline__ float e4m3(uint32_t code) const {
             const float v = e4m3_value(code);
-            return exact ? v * ratio : (float) ((double) v * s_old / s);
+            if (exact) return v * ratio;
+            const double p = (double) v * s_old, q = __ddiv_rz(p, s);
+            const float  f = __double2float_rz(q);
+            return odd(f, (double) f != q || fma(-q, s, p) != 0.0);
         }
         __device__ __forceinline__ uint32_t four(uint32_t c) const {
             if (kE4m3) return e4m3x4(e4m3(c), e4m3(c >> 8), e4m3(c >> 16), e4m3(c >> 24));
