@@ -302,6 +302,8 @@ VKC_API int vkc_kv_append_q8(vkc_ctx *ctx, const vkc_kv_append_q8_args *args, vk
  *   its bits. Sums and softmax statistics are fp32; Q keeps its precision.
  *   workspace: device scratch of at least vkc_attn_decode_q8_workspace_bytes(...) bytes (16-byte aligned) for the partial
  *   results (short caches leave it alone); NULL lets the context keep (and grow) its own. It may hold anything before the call.
+ *   The context's own cannot grow while the stream is being captured: the call then returns VKC_ERR_INVALID and launches nothing,
+ *   unless a call that needs as many bytes was made on the context before. Capture with a workspace, or after one ordinary call of the shape.
  *   Two calls that may run at the same time need workspaces of their own, and so do two captured graphs that may be replayed at the same time; calls
  *   captured without a workspace share the context's. ---- */
 VKC_API size_t vkc_attn_decode_q8_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Lmax, int64_t D);

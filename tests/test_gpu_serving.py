@@ -842,6 +842,55 @@ def test_decode_q8_more_sequences_than_one_launch_holds(ctx):
     check_decode(ctx, q, cache, lens, d ** -0.5)
 
 
+def test_decode_q8_captured_without_a_workspace():
+    """The context's own scratch does not grow during a capture: a clean error, nothing launched, and the context goes on working.
+    After one ordinary call of the shape the same capture is fine; short caches need no scratch at all."""
+    fresh = vknn_b200.Context(0)
+    try:
+        hq, hkv, d, block, lens = 8, 2, 128, 64, torch.tensor([4000, 77, 300], dtype=torch.int32, device="cuda")
+        cache, short, q = filled(31, 3, hkv, 4096, d, block, "e4m3"), filled(32, 3, hkv, 256, d, block, "e4m3"), queries(33, 3, hq, d, "f16")
+        want, o = torch.zeros_like(q), torch.full_like(q, 5.0)
+        attend = lambda c, out, **kw: fresh.attn_decode_q8(q, *c.args, out, d ** -0.5, kv_len=lens, **kw)  # noqa: E731
+        attend(short, want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            attend(short, o)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, want)
+        n0, graph, mark = fresh.launch_count(), torch.cuda.CUDAGraph(), torch.zeros(1, device="cuda")
+        with torch.cuda.graph(graph):
+            mark += 1
+            with pytest.raises(vknn_b200.VkcError) as e:
+                attend(cache, o)
+        assert e.value.code == -1 and fresh.launch_count() == n0
+        attend(cache, want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            attend(cache, o)
+        graph.replay()
+        fresh.sync()
+        torch.cuda.synchronize()
+        assert torch.equal(o, want)
+        ref, a = decode64(q, cache, lens.tolist(), d ** -0.5)
+        check(o, ref, a, torch.float16, torch.float16)
+        # with a workspace a context that has none of its own captures at once
+        other = vknn_b200.Context(0)
+        try:
+            ws, graph = torch.empty(other.attn_decode_q8_workspace_bytes(3, hq, hkv, 4096, d), dtype=torch.uint8, device="cuda"), torch.cuda.CUDAGraph()
+            o.zero_()
+            torch.cuda.synchronize()
+            with torch.cuda.graph(graph):
+                other.attn_decode_q8(q, *cache.args, o, d ** -0.5, kv_len=lens, workspace=ws)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(o, want)
+        finally:
+            other.close()
+    finally:
+        fresh.close()
+
+
 @pytest.mark.parametrize("lmax", [4096, 1024])
 def test_decode_q8_two_calls_at_once(ctx, lmax):
     """Two streams, a workspace each; and one after the other on two streams with the context's own scratch."""

@@ -407,7 +407,8 @@ class Context:
         return int(self.lib.vkc_attn_decode_q8_workspace_bytes(B, Hq, Hkv, Lmax, D))
 
     def attn_decode_q8(self, Q, Kc, Vc, k_scale, v_scale, O, scale, kv_len=None, workspace=None, stream=None):
-        """attn_decode over the 8-bit cache that kv_append_q8 fills: Q/O [B,Hq,D] contiguous, float16 or bfloat16."""
+        """attn_decode over the 8-bit cache that kv_append_q8 fills: Q/O [B,Hq,D] contiguous, float16 or bfloat16. `workspace` None: the
+        context's own scratch, which cannot grow while the stream is being captured (VkcError); call the shape once before, or pass one."""
         (B, Hkv, Lmax, D), block, code = self._q8_cache(Kc, Vc, k_scale, v_scale)
         shape, dev = Q.shape, self.device
         if (len(shape) != 3 or shape[0] != B or shape[2] != D or O.shape != shape or O.dtype is not Q.dtype or not (Q.is_contiguous() and O.is_contiguous()) or
