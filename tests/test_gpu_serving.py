@@ -689,6 +689,15 @@ def test_decode_q8_shapes_of_a_longer_cache(ctx, d, block, group, dt, codes):
     check_decode(ctx, queries(2, len(lens), 2 * group, d, dt), cache, lens, d ** -0.5)
 
 
+@pytest.mark.parametrize("codes", ["e4m3", "i8"])
+@pytest.mark.parametrize("hq,d,block,dt", [(17, 64, 32, "bf16"), (32, 128, 64, "f16"), (71, 256, 128, "bf16")])
+def test_decode_q8_large_groups_over_a_long_cache(ctx, hq, d, block, dt, codes):
+    """More than 16 query heads on one kv head: the SIMT form, here with thousands of keys for every warp to walk."""
+    lens = [9001, 0, 1, 8192]
+    cache = filled(41, len(lens), 1, 9216, d, block, codes)
+    check_decode(ctx, queries(42, len(lens), hq, d, dt), cache, lens, d ** -0.5)
+
+
 @pytest.mark.parametrize("room", [768, 1024, 1280])
 @pytest.mark.parametrize("hkv", [1, 37, 38, 74, 75, 148, 149])
 def test_decode_q8_around_the_number_of_multiprocessors(ctx, hkv, room):

@@ -20,7 +20,10 @@
 // of the issue slots and 0.29 of their own pipe for that (profiles) and keep scores and probabilities in registers, where
 // the tensor-memory route would carry every tile through it twice; the tensor rate is of no concern at 8 or 16 columns.
 // Measured: 32 sequences of 1024 to 8192 tokens, 32/8 heads x 128, 339 MB of e4m3: 64 us with the join, 5.8 TB/s while
-// streaming (0.89 of the copy rate); two sequences of up to 131000 tokens, 509 MB: 89 to 91 us.
+// streaming (0.89 of the copy rate); two sequences of up to 131000 tokens, 509 MB: 88 us. Such a batch of 154000 tokens in all,
+// 8 kv heads, us and TB/s with the join, groups of 1, 8 and 16 query heads, e4m3: D = 64 (157 MB) 40 / 41 / 49 (3.9, 3.8, 3.2),
+// D = 128 59 / 62 / 76 (5.3, 5.1, 4.2), D = 256 103 / 107 / 194 (6.1, 5.9, 3.2). Groups of 9 to 16 keep two sets of Q fragments
+// and accumulators in registers and spill 80 to 92 bytes a thread at D = 128 and 420 to 452 at D = 256.
 // A unit that lies in one run is finished there; one that is cut leaves a partial (maximum, sum, O) per run in the workspace
 // (slot 0: the unit began in an earlier run, slot 1: in this one) and a second kernel joins them in the order of the runs.
 // (Joined by the warp whose partial arrives last instead, the batch took 73 us, not 67: the fences hold up the stream.)
@@ -51,7 +54,10 @@ namespace {
 
     constexpr int kSimtWarps = 8;
 
-    // SIMT form: one CTA per (query head, sequence), the warps take keys round-robin, a lane holds D / 32 dims of the row.
+    // SIMT form: one CTA per (query head, sequence), the warps take keys round-robin, a lane holds D / 32 dims of the row. It is the
+    // form of groups of more than 16 query heads, which the streaming form's fragments do not hold, and reads the cache once per head,
+    // a byte at a time, with no cut along the keys: 32 heads on one kv head, D = 128, 32 sequences of 1024 to 8192 tokens 848 us, one
+    // of 131072 tokens 8.7 ms (16 heads in the streaming form: 34 us).
     template <typename T, int D, bool kE4m3> __global__ void __launch_bounds__(kSimtWarps * 32) attn_decode_q8_simt_kernel(const DecQ8Params p) {
         constexpr int DL = D / 32;
         const int     warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
