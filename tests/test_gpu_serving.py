@@ -13,6 +13,7 @@ import pytest
 import torch
 
 import vknn_b200
+from vknn_b200 import capi
 
 pytestmark = pytest.mark.gpu
 
@@ -1029,4 +1030,23 @@ def test_refusals_of_the_serving_operators(ctx):
         with pytest.raises(vknn_b200.VkcError) as e:
             call()
         assert e.value.code == code
+    assert ctx.launch_count() == n0
+
+
+def test_misaligned_pointers_are_refused(ctx):
+    """C callers only: a tensor cannot lie at such an address. Nothing is launched."""
+    n0, lib = ctx.launch_count(), ctx.lib
+    z = lambda *s, dt=torch.float16: torch.zeros(*s, dtype=dt, device="cuda")  # noqa: E731
+    q, kv, lens, cache = z(2, 4, 64), z(2, 2, 64), z(3, dt=torch.int32), Cache(2, 2, 64, 64, 32, "e4m3")
+    p, codes, scales, n = q.data_ptr(), [t.data_ptr() for t in (cache.k, cache.v)], [t.data_ptr() for t in (cache.ks, cache.vs)], lens.data_ptr()
+    kvp = [kv.data_ptr()] * 2
+    calls = [(lib.vkc_attn_prefill_packed, capi.PACKED_ARGS, [p, *kvp, p, 2, 4, 2, 64, 2, 2, n, n, *[0] * 8, 1.0, 1, vknn_b200.F16], (0, 1, 2, 3, 10, 11)),
+             (lib.vkc_kv_append_q8, capi.APPEND_ARGS, [*kvp, *codes, *scales, 2, 2, 64, 64, 32, 2, n, n, *[0] * 4, vknn_b200.F16, vknn_b200.E4M3], (0, 1, 2, 3, 4, 5, 12, 13)),
+             (lib.vkc_attn_decode_q8, capi.DECODE_Q8_ARGS, [p, *codes, *scales, p, 2, 4, 2, 64, 64, 32, n, 0, 0, 1.0, vknn_b200.F16, vknn_b200.E4M3], (0, 1, 2, 3, 4, 5, 12))]
+    for f, struct, args, pointers in calls:
+        for i in pointers:
+            bad = list(args)
+            bad[i] += 1
+            assert f(ctx.h, struct.pack(*bad), 1) == -1, (f, i)
+            assert b"aligned" in lib.vkc_last_error(ctx.h)
     assert ctx.launch_count() == n0

@@ -743,6 +743,7 @@ extern "C" int vkc_attn_decode_q8(vkc_ctx *ctx, const vkc_attn_decode_q8_args *a
     if (B == 0) return VKC_OK;
     VKC_REQUIRE(ctx, Q && Kc && Vc && k_scale && v_scale && O, "attn_decode_q8: null tensor");
     VKC_REQUIRE(ctx, !(((uintptr_t) Q | (uintptr_t) O | (uintptr_t) Kc | (uintptr_t) Vc) & 15), "attn_decode_q8: Q, O and the cache must be 16-byte aligned");
+    VKC_REQUIRE(ctx, !(((uintptr_t) k_scale | (uintptr_t) v_scale | (uintptr_t) kv_len) & 3), "attn_decode_q8: scales or lengths are not aligned to their type");
     const size_t need = vkc_attn_decode_q8_workspace_bytes(B, Hq, Hkv, Lmax, D);
     VKC_REQUIRE(ctx, !workspace || (workspace_bytes >= need && !((uintptr_t) workspace & 15)),
                 "attn_decode_q8: workspace of %zu bytes is smaller than the %zu required, or not 16-byte aligned", workspace_bytes, need);

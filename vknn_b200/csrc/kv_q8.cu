@@ -173,6 +173,7 @@ extern "C" int vkc_kv_append_q8(vkc_ctx *ctx, const vkc_kv_append_q8_args *args,
     VKC_REQUIRE(ctx, K && V && Kc && Vc && k_scale && v_scale, "kv_append_q8: null tensor");
     VKC_REQUIRE(ctx, !(((uintptr_t) Kc | (uintptr_t) Vc) & 15), "kv_append_q8: the cache must be 16-byte aligned");
     VKC_REQUIRE(ctx, !(((uintptr_t) K | (uintptr_t) V) & (vkc_dtype_size(dtype) - 1)), "kv_append_q8: K/V are not aligned to their type");
+    VKC_REQUIRE(ctx, !(((uintptr_t) k_scale | (uintptr_t) v_scale | (uintptr_t) cu | (uintptr_t) kv_len) & 3), "kv_append_q8: scales, offsets or lengths are not aligned to their type");
     VkcDeviceGuard guard(ctx);
     AppendParams   p;
     p.X[0] = K, p.X[1] = V;
