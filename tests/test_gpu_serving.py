@@ -1000,6 +1000,56 @@ def test_prompts_then_tokens_as_a_server_runs_them(ctx, codes):
         check(o[s], ref, a, dt, dt)
 
 
+@pytest.mark.parametrize("lmax", [256, 4096])
+@pytest.mark.parametrize("codes", ["e4m3", "i8"])
+def test_steps_behind_the_product_that_writes_their_rows(ctx, codes, lmax):
+    """Projection, append and attention of several steps one right behind the other, over the same buffers: each kernel may start while
+    the one before it still runs, and has to see what that one wrote. The same bits as with a wait after every call."""
+    b, hq, hkv, d, block, dt, steps, width = 6, 8, 2, 128, 32, torch.bfloat16, 12, 512
+    g = torch.Generator(device="cuda").manual_seed(51)
+    x, w = (randn(g, *s).to(dt) * 0.2 for s in ((steps, b, width), (width, (hq + 2 * hkv) * d)))
+    lens = [torch.tensor([1, 31, 100, 0, 5, 64], dtype=torch.int32, device="cuda") + s for s in range(steps + 1)]
+    ws = torch.zeros(ctx.attn_decode_q8_workspace_bytes(b, hq, hkv, lmax, d), dtype=torch.uint8, device="cuda")
+    start, qkv = filled(52, b, hkv, lmax, d, block, codes), torch.zeros(b, (hq + 2 * hkv) * d, dtype=dt, device="cuda")
+    q, out = torch.zeros(b, hq, d, dtype=dt, device="cuda"), torch.zeros(steps, b, hq, d, dtype=dt, device="cuda")
+
+    def run(cache, between):
+        for s in range(steps):
+            ctx.gemm(x[s], w, qkv)
+            between()
+            rows3 = qkv.view(b, hq + 2 * hkv, d)
+            ctx.kv_append_q8(rows3[:, hq:hq + hkv], rows3[:, hq + hkv:], *cache.args, lens[s])
+            between()
+            ctx.gemm(x[s], wq, q.view(b, hq * d))
+            between()
+            ctx.attn_decode_q8(q, *cache.args, out[s], d ** -0.5, kv_len=lens[s + 1], workspace=ws)
+            between()
+
+    idle, wq = lambda: None, w[:, :hq * d].contiguous()
+    cache = start.clone()
+    run(cache, torch.cuda.synchronize)
+    want, kept = out.clone(), cache.clone()
+    graph, cache = torch.cuda.CUDAGraph(), start.clone()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        run(cache, idle)
+    for _ in range(5):
+        for t, s in zip(cache.args, start.args):
+            t.copy_(s)
+        out.zero_()
+        qkv.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and cache.same(kept)
+        for t, s in zip(cache.args, start.args):
+            t.copy_(s)
+        out.zero_()
+        run(cache, idle)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and cache.same(kept)
+    assert bool(torch.isfinite(want).all())
+
+
 # ---- refusals -----------------------------------------------------------------------------------------------------------
 
 def test_refusals_of_the_serving_operators(ctx):

@@ -343,8 +343,9 @@ namespace {
                     for (int c = 0; c < CH; ++c) {
                         const int chunk = D == 256 ? (c >> 1) * 8 + (t & 1) + (t >> 1) * 4 + 2 * (c & 1) : t * CH + c;
                         uint4     v[2]; // 16 dims
-                        v[0] = have ? __ldg(reinterpret_cast<const uint4 *>(qr + chunk * 16)) : make_uint4(0, 0, 0, 0);
-                        v[1] = have ? __ldg(reinterpret_cast<const uint4 *>(qr + chunk * 16) + 1) : make_uint4(0, 0, 0, 0);
+                        // (plain loads, not the read-only path: the kernel before may still have been writing Q when this one started)
+                        v[0] = have ? *reinterpret_cast<const uint4 *>(qr + chunk * 16) : make_uint4(0, 0, 0, 0);
+                        v[1] = have ? *(reinterpret_cast<const uint4 *>(qr + chunk * 16) + 1) : make_uint4(0, 0, 0, 0);
                         const uint32_t *w = reinterpret_cast<const uint32_t *>(v);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) qa[h][c * 4 + k][0] = w[2 * k], qa[h][c * 4 + k][1] = w[2 * k + 1];

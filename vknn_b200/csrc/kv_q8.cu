@@ -7,7 +7,7 @@
 // (loaded together) between the maximum and the quotients, and no second pass or second kernel is needed. 64 registers a
 // thread keep 1024 threads with 128 bytes each on their way per SM: 43 k tokens of 8 heads x 128 (K and V, bf16 to e4m3, blocks
 // of 128) in 52 to 56 us back to back, 5.1 to 4.8 TB/s; with 84 registers 67 us. 32 single tokens 2.9 us in a graph.
-// The bound of 64 registers is made for 16-bit rows, which take 32 of them (56 bytes of spills, all addresses). Rows in fp32 take all
+// The bound of 64 registers is made for 16-bit rows, which take 32 of them (40 to 56 bytes of spills a thread). Rows in fp32 take all
 // 64, so that a part of them goes through local memory (440 bytes of spills a thread for int8, 532 for e4m3): 40 k tokens of 8
 // heads x 128 in blocks of 128 take 98 us (e4m3) and 107 us (int8), 4.1 and 3.8 TB/s, where bf16 rows take 47 and 54 us (5.2, 4.5).
 //
@@ -32,13 +32,14 @@ namespace {
         int            vec_ok; // bases and strides of K and V allow 16-byte loads
     };
 
-    // Eight values as fp32, from one 16-byte vector of a 16-bit type or two of fp32.
+    // Eight values as fp32, from one 16-byte vector of a 16-bit type or two of fp32. (Plain loads: the read-only path is for memory that
+    // nobody writes while the kernel runs, and the kernel before this one may still be writing the rows when this one starts.)
     template <typename T> struct Row8 {
         uint4 v[sizeof(T) == 4 ? 2 : 1];
         __device__ __forceinline__ void load(const T *p, bool vec_ok) {
             if (vec_ok) {
 #pragma unroll
-                for (int i = 0; i < (int) (sizeof(v) / 16); ++i) v[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+                for (int i = 0; i < (int) (sizeof(v) / 16); ++i) v[i] = reinterpret_cast<const uint4 *>(p)[i];
             } else {
                 T *e = reinterpret_cast<T *>(v);
 #pragma unroll
