@@ -145,7 +145,8 @@ VKC_API int vkc_attn_prefill_items(int sm_count, int64_t B, int64_t Hq, int64_t 
  * a row attends to the keys of its own sequence only. It has no counterpart in the reference, which runs one batch shape per
  * graph (the arithmetic is vkc_attn_prefill's: ops/matmul.cpp:14-116, ops/softmax.cpp:9-47).
  *   Q/O [total_q,Hq,D], K/V [total_k,Hkv,D]; *_strides = element strides {token, head} with D contiguous, {0, 0} for dense
- *   (views of one packed projection [tokens, Hq+2*Hkv, D] are fine); query head h uses kv head h / (Hq/Hkv);
+ *   (views of one packed projection [tokens, Hq+2*Hkv, D] are fine; a stride of 0 repeats a row of Q, K or V, but not of O);
+ *   query head h uses kv head h / (Hq/Hkv);
  *   cu_q, cu_k: device int32 [nseq+1], non-decreasing; cu_k NULL = cu_q (then total_k must equal total_q). Values outside
  *   [0, total] are clamped to it. Rows that belong to no sequence (behind cu_q[nseq]) are left as they were;
  *   causal masks key j > i + (len_k - len_q), i and j counted within the sequence: a sequence with more keys than queries

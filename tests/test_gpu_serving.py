@@ -1083,6 +1083,20 @@ def test_refusals_of_the_serving_operators(ctx):
     assert ctx.launch_count() == n0
 
 
+def test_outputs_that_share_memory_are_refused(ctx):
+    """Rows of O under one another's address: whichever is stored last would stay."""
+    q, kv = (torch.zeros(*s, dtype=torch.float16, device="cuda") for s in ((6, 4, 64), (6, 2, 64)))
+    cu, n0 = torch.tensor([0, 2, 6], dtype=torch.int32, device="cuda"), ctx.launch_count()
+    for o in (q[:, :1].expand(6, 4, 64), q[:1].expand(6, 4, 64)):
+        with pytest.raises(vknn_b200.VkcError) as e:
+            ctx.attn_prefill_packed(q, kv, kv, o, 1.0, cu)
+        assert e.value.code == -1 and "share memory" in str(e.value)
+    assert ctx.launch_count() == n0
+    one = torch.zeros(1, 4, 64, dtype=torch.float16, device="cuda")  # a single token: its stride is of no account
+    ctx.attn_prefill_packed(one, one, one, torch.zeros_like(one).as_strided((1, 4, 64), (0, 64, 1)), 1.0, torch.tensor([0, 1], dtype=torch.int32, device="cuda"))
+    ctx.sync()
+
+
 def test_misaligned_pointers_are_refused(ctx):
     """C callers only: a tensor cannot lie at such an address. Nothing is launched."""
     n0, lib = ctx.launch_count(), ctx.lib

@@ -225,6 +225,8 @@ extern "C" int vkc_attn_prefill_packed(vkc_ctx *ctx, const vkc_attn_prefill_pack
     VKC_REQUIRE(ctx, Q && O && (total_k == 0 || (K && V)), "attn_prefill_packed: null tensor");
     VKC_REQUIRE(ctx, !(((uintptr_t) Q | (uintptr_t) K | (uintptr_t) V | (uintptr_t) O) & (vkc_dtype_size(dtype) - 1)) && !(((uintptr_t) cu_q | (uintptr_t) cu_k) & 3),
                 "attn_prefill_packed: a tensor is not aligned to its type");
+    VKC_REQUIRE(ctx, (!o_strides[0] && !o_strides[1]) || ((o_strides[0] || total_q == 1) && (o_strides[1] || Hq == 1)),
+                "attn_prefill_packed: rows of O share memory (a stride of 0)");
     VKC_REQUIRE(ctx, Hq <= 65535 && nseq <= (1 << 24), "attn_prefill_packed: grid too large");
     VkcDeviceGuard guard(ctx);
     cudaStream_t   st = vkc_pick_stream(ctx, stream);
