@@ -41,6 +41,19 @@ def cache(b=2, hkv=2, lmax=64, d=64, block=32, dt=torch.float8_e4m3fn):
     return z(b, hkv, lmax, d, dt=dt), z(b, hkv, lmax, d, dt=dt), z(b, hkv, lmax // block, dt=torch.float32), z(b, hkv, lmax // block, dt=torch.float32)
 
 
+def test_the_current_stream_with_and_without_torchs_private_function(monkeypatch):
+    c = vknn_b200.Context.__new__(vknn_b200.Context)
+    c.h, c.device = None, 3
+    seen = []
+    for handle, want in ((0x1234, 0x1234), (0, 1)):  # 0, the legacy stream, goes by its explicit handle
+        monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: seen.append(d) or handle, raising=False)
+        assert c._stream(None).value == want
+        monkeypatch.delattr(torch._C, "_cuda_getCurrentRawStream")
+        monkeypatch.setattr(torch.cuda, "current_stream", lambda d: seen.append(d) or type("S", (), {"cuda_stream": handle}))
+        assert c._stream(None).value == want
+    assert seen == [3] * 4 and c._stream(77).value == 77
+
+
 def test_null_context_is_refused():
     lib = vknn_b200.load_library()
     args = C.create_string_buffer(256)

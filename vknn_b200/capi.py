@@ -258,7 +258,9 @@ class Context:
         if stream is not None:
             return C.c_void_p(stream)
         import torch
-        h = torch._C._cuda_getCurrentRawStream(self.device)  # current_stream(device).cuda_stream without the Python object
+        # the handle without building a Stream object (1 us a call less), where this torch has that; it is not a public function
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        h = raw(self.device) if raw else torch.cuda.current_stream(self.device).cuda_stream
         # torch's default stream is the legacy NULL stream; NULL means "the context's own stream" in the C-ABI,
         # so name the legacy stream by its explicit handle (cudaStreamLegacy == 0x1) to keep torch ordering.
         return C.c_void_p(h if h else 1)
