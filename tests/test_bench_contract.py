@@ -31,6 +31,19 @@ def test_reference_arm_prints_the_contract_line():
 import pytest
 
 
+def test_reference_arm_is_never_this_repositorys_own_restatement():
+    """Where the compiled reference is missing the arm says so and loads none of the library's own code for it."""
+    from oracle import vko
+    if vko.have_ref():
+        pytest.skip("the compiled reference is in the tree")
+    p = subprocess.run([sys.executable, "-c", "import runpy, sys; sys.argv = ['bench.py', '--impl', 'reference', '--steps', '2', '--warmup', '1']\n"
+                        "try:\n    runpy.run_path('bench.py', run_name='__main__')\nexcept SystemExit as e:\n    assert not e.code\n"
+                        "assert 'libvknn' not in open('/proc/self/maps').read()"], cwd=ROOT, capture_output=True, text=True, timeout=600)
+    assert p.returncode == 0, p.stderr[-2000:]
+    line = json.loads(p.stdout.strip().splitlines()[-1])
+    assert line["impl"] == "reference" and line["unavailable"] and "value" not in line
+
+
 @pytest.mark.gpu
 def test_cuda_arm_prints_the_contract_line():
     """The CUDA arm on one GPU, shortened (three steps, no extra legs, no two-second sustained run): every key the line must
