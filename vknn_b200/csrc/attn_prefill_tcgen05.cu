@@ -34,7 +34,8 @@
 // finished and O_t may be rescaled; Q.K_t(j+1) overwrites the columns P_t(j) lives in and is issued after
 // P.V_t(j) by the same thread, which the tensor pipe executes in order.
 // Packed sequences (kPack): the same kernel with units looked up in the sequence offsets, see AttnParams, PackedUnit and the issuer's
-// loop. 16 x 1024 tokens, 32/8 heads x 128, causal: 169 us (815 TFLOP/s), the dense call 292; 4 x 4096: 481 us (1140), dense 530.
+// loop. Back to back, 32/8 heads x 128, causal: 16 x 1024 tokens 158 to 169 us (867 to 815 TFLOP/s), the dense call 278 to 296; 4 x 4096
+// 470 to 501 us (1170 to 1098), dense 515 to 615 (the power cap decides where in these ranges). Without a mask, 4 x 4096: 957 to 1032, dense 946 to 966.
 // Masking: keys >= kv_len[b] (or >= Skv) and, for causal, keys > row + (Skv - Sq) get probability 0; key tiles
 // entirely above a query tile's diagonal are skipped for that tile.
 #include <type_traits>

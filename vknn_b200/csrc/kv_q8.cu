@@ -6,10 +6,10 @@
 // latency. One CTA does one block of one head, so that the rows are read once: each thread keeps its 64 values
 // (loaded together) between the maximum and the quotients, and no second pass or second kernel is needed. 64 registers a
 // thread keep 1024 threads with 128 bytes each on their way per SM: 43 k tokens of 8 heads x 128 (K and V, bf16 to e4m3, blocks
-// of 128) in 52 to 56 us back to back, 5.1 to 4.8 TB/s; with 84 registers 67 us. 32 single tokens 2.9 us in a graph.
+// of 128) in 49 to 52 us back to back, 5.4 to 5.1 TB/s; with 84 registers 67 us. 32 single tokens 2.9 to 3.1 us in a graph.
 // The bound of 64 registers is made for 16-bit rows, which take 32 of them (40 to 56 bytes of spills a thread). Rows in fp32 take all
 // 64, so that a part of them goes through local memory (440 bytes of spills a thread for int8, 532 for e4m3): 40 k tokens of 8
-// heads x 128 in blocks of 128 take 98 us (e4m3) and 107 us (int8), 4.1 and 3.8 TB/s, where bf16 rows take 47 and 54 us (5.2, 4.5).
+// heads x 128 in blocks of 128 take 99 us (e4m3) and 107 us (int8), 4.1 and 3.8 TB/s, where bf16 rows take 44 and 50 us (5.5, 4.9).
 //
 // The scale of e4m3 codes is a power of two: the format carries its own exponent, so a finer scale would not make a code more
 // precise, and multiplying by 2^-e is exact — the code is the value rounded once. int8 codes take a / 127, which spreads the
